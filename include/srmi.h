@@ -61,6 +61,10 @@ extern "C" {
                                `add([shortcut, conv])` -> ReLU of res_conv_block (Res-U-SRGAN/untitled0.py:67-72).  Served by the
                                generic kernel and, for bf16 3x3 convs, the K-chunked bf16 kernel; residual == NULL makes
                                it a plain ReLU */
+/* the row operators' further activations (srmi_linear_*; the convolutions refuse them) */
+#define SRMI_ACT_GELU 7      /* z Phi(z), Phi the normal distribution function */
+#define SRMI_ACT_GELU_TANH 8 /* its tanh form: z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
+#define SRMI_ACT_SILU 9      /* z / (1 + exp(-z)) */
 /* sub-pixel store orders (shuffle > 1) */
 #define SRMI_SHUFFLE_CRD 0 /* nn.PixelShuffle: conv channel = c*r*r + i*r + j   (P/ops.py:75) */
 #define SRMI_SHUFFLE_DCR 1 /* tf.nn.depth_to_space: conv channel = (i*r + j)*C + c (ESRGAN/untitled0.py:60) */
@@ -483,6 +487,65 @@ int srmi_tv_loss_bwd(const float* x, const float* gout, int32_t N, int32_t C, in
  * parameters, gradients and moments live in flat buffers (srmi/optim.py) instead of a dozen multi-tensor launches. */
 int srmi_adam_step(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, size_t n, double lr,
                    double beta1, double beta2, double eps, int32_t step, void* stream);
+
+/* ---- Row operators ----------------------------------------------------------------------------------------------------
+ * Operators on rows of features: a row is one token, or one pixel of a channels-last (NHWC) map, so a map between two convs
+ * is passed as [N*H*W, C] without a copy.  Storage f32 or bf16 (one type per call, layer norm's parameters may be f32 next
+ * to bf16 rows); every sum, statistic and activation is f32.  `ld*` are row strides in elements (>= the row, 0 = operand not
+ * given); rows need no alignment beyond their element, 16-byte aligned ones (pointer and stride) run wider accesses.
+ * Outputs are dense.  Deterministic: no atomics, the same call gives the same bits.  These calls were added after version
+ * 119 without changing anything that version declares; a caller that may meet an older library looks the symbols up. */
+#define SRMI_ROWS_MAX 0x7fffffffff /* rows per call */
+#define SRMI_PASS_FWD 0
+#define SRMI_PASS_BWD 1
+
+typedef struct srmi_linear_desc {
+    int64_t M;                     /* rows */
+    int32_t N, K;                  /* output and input features */
+    int32_t dtype;                 /* of every tensor of the call */
+    int32_t act;                   /* NONE, LRELU, RELU, TANH, SIGMOID, GELU, GELU_TANH, SILU (PReLU: the convs' epilogue) */
+    float act_param;               /* LeakyReLU slope */
+    int32_t reserved;              /* must be 0 */
+    int64_t ldx, ldw, ldr, lddy;   /* row strides of x, w, residual, dy */
+} srmi_linear_desc;
+
+/* y = act(x w^T + bias) + residual:  x [M, K], w [N, K] (nn.Linear's layout), bias [N] or NULL, residual [M, N] or NULL,
+ * y [M, N].  z (NULL, or dense [M, N]) also receives x w^T + bias, which the backward of a smooth activation needs.
+ * K == 0 is a product of nothing: y = act(bias) + residual.
+ * ws: srmi_linear_workspace_bytes(d, pass) bytes, 256-byte aligned, written and read by this call alone. */
+int srmi_linear_workspace_bytes(const srmi_linear_desc* d, int32_t pass, size_t* bytes);
+int srmi_linear_fwd(const srmi_linear_desc* d, const void* x, const void* w, const void* bias, const void* residual, void* y, void* z,
+                    void* ws, size_t ws_bytes, void* stream);
+/* dz = dy act'(saved);  dx = dz w [M, K],  dw = dz^T x [N, K],  db = sum of dz over rows [N]; each may be NULL (not wanted).
+ * `saved` (dense [M, N]; NULL for NONE): z, or - RELU, or LRELU with a positive slope, called without a residual - y, whose
+ * sign is z's.  The residual's gradient is dy itself. */
+int srmi_linear_bwd(const srmi_linear_desc* d, const void* x, const void* w, const void* saved, const void* dy, void* dx, void* dw, void* db,
+                    void* ws, size_t ws_bytes, void* stream);
+
+typedef struct srmi_norm_desc {
+    int64_t rows;
+    int32_t C;                     /* normalised features, >= 1 */
+    int32_t dtype, param_dtype;    /* of x, y, dy, dx / of weight, bias and their gradients */
+    float eps;
+    int64_t ldx, lddy;
+} srmi_norm_desc;
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis (biased variance); weight, bias [C] may be NULL (1, 0).
+ * mean, rstd [rows] f32 (both or neither): kept for the backward. */
+int srmi_layer_norm_fwd(const srmi_norm_desc* d, const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                        void* stream);
+/* dx [rows, C], dweight, dbias [C]; each may be NULL.  ws is needed with dweight or dbias (16-byte aligned). */
+int srmi_layer_norm_workspace_bytes(const srmi_norm_desc* d, size_t* bytes);
+int srmi_layer_norm_bwd(const srmi_norm_desc* d, const void* x, const void* weight, const float* mean, const float* rstd, const void* dy,
+                        void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes, void* stream);
+
+/* y = residual + keep * x / (1 - p) over n dense elements, residual may be NULL; y may be x.  keep of element i: word i % 4 of
+ * the Philox4x32-10 block with counter (i / 4, offset) and key seed is >= floor(p 2^32).  A dropped x contributes exactly 0
+ * (also when it is infinite or NaN); p = 1 drops everything.  The backward is the same call on dy without a residual: nothing
+ * is stored.  rng != NULL: {seed, offset} are read from device memory instead, so that a captured graph can draw a new mask at
+ * every replay. */
+int srmi_dropout(const void* x, const void* residual, void* y, size_t n, int32_t dtype, double p, uint64_t seed, uint64_t offset,
+                 const uint64_t* rng, void* stream);
 
 #ifdef __cplusplus
 }

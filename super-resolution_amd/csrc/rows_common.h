@@ -1,0 +1,134 @@
+// Shared pieces of the row operators (linear, layer norm, dropout): storage conversion, activations and their slopes.
+#pragma once
+#include "common.h"
+
+namespace srmi {
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16_t v) { return bf2f(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) { return f2bf(v); }
+
+// V consecutive elements as f32.  The caller guarantees alignment to V elements.
+template <int V>
+__device__ __forceinline__ void load_vec(const float* p, float* o) {
+    if constexpr (V == 1) {
+        o[0] = p[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const f32x4 q = *(const f32x4*)(p + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i + j] = q[j];
+        }
+    }
+}
+template <int V>
+__device__ __forceinline__ void load_vec(const bf16_t* p, float* o) {
+    if constexpr (V == 1) {
+        o[0] = bf2f(p[0]);
+    } else if constexpr (V == 4) {
+        const u32x2 q = *(const u32x2*)p;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            o[2 * j] = __builtin_bit_cast(float, q[j] << 16);
+            o[2 * j + 1] = __builtin_bit_cast(float, q[j] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 8) {
+            const u32x4 q = *(const u32x4*)(p + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[i + 2 * j] = __builtin_bit_cast(float, q[j] << 16);
+                o[i + 2 * j + 1] = __builtin_bit_cast(float, q[j] & 0xffff0000u);
+            }
+        }
+    }
+}
+template <int V>
+__device__ __forceinline__ void store_vec(float* p, const float* v) {
+    if constexpr (V == 1) {
+        p[0] = v[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) *(f32x4*)(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+    }
+}
+template <int V>
+__device__ __forceinline__ void store_vec(bf16_t* p, const float* v) {
+    if constexpr (V == 1) {
+        p[0] = f2bf(v[0]);
+    } else if constexpr (V == 4) {
+        *(u32x2*)p = u32x2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 8)
+            *(u32x4*)(p + i) = u32x4{pack_bf2(v[i], v[i + 1]), pack_bf2(v[i + 2], v[i + 3]), pack_bf2(v[i + 4], v[i + 5]),
+                                     pack_bf2(v[i + 6], v[i + 7])};
+    }
+}
+
+// exp and division of the epilogues.  Where the result is stored in bf16 (half a step = 2^-9 of the value) the hardware's
+// 2^x and reciprocal, a few 2^-23 off, are enough; f32 results take the library's functions.
+template <bool FAST> __device__ __forceinline__ float exp_(float v) {
+    if constexpr (FAST) return __builtin_amdgcn_exp2f(v * 1.442695040888963f);
+    else return expf(v);
+}
+template <bool FAST> __device__ __forceinline__ float div_(float a, float b) {
+    if constexpr (FAST) return a * __builtin_amdgcn_rcpf(b);
+    else return a / b;
+}
+template <bool FAST> __device__ __forceinline__ float logistic(float v) { return div_<FAST>(1.f, 1.f + exp_<FAST>(-v)); }
+
+constexpr float GELU_2C = 1.5957691216057308f;      // 2 sqrt(2 / pi)
+constexpr float GELU_K = 0.044715f;
+
+// act(z).  gelu = z Phi(z); its tanh form is z * logistic(2 sqrt(2/pi) (z + 0.044715 z^3)) since (1 + tanh u)/2 = logistic(2u):
+// no cancellation for negative z.
+template <bool FAST>
+__device__ __forceinline__ float row_act(float z, int act, float param) {
+    switch (act) {
+        case SRMI_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
+        case SRMI_ACT_LRELU: return z >= 0.f ? z : z * param;
+        case SRMI_ACT_TANH: return tanhf(z);
+        case SRMI_ACT_SIGMOID: return logistic<FAST>(z);
+        case SRMI_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+        case SRMI_ACT_GELU_TANH: return z * logistic<FAST>(GELU_2C * (z + GELU_K * z * z * z));
+        case SRMI_ACT_SILU: return z * logistic<FAST>(z);
+        default: return z;
+    }
+}
+
+// d act / d z at z.  tanh and sigmoid from e = exp(-k|z|): 1 - t^2 and s (1 - s) would cancel for large |z|.
+template <bool FAST>
+__device__ __forceinline__ float row_act_slope(float z, int act, float param) {
+    switch (act) {
+        case SRMI_ACT_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
+        case SRMI_ACT_LRELU: return z >= 0.f ? 1.f : (z != z ? z : param);
+        case SRMI_ACT_TANH: {
+            const float e = exp_<FAST>(-2.f * fabsf(z)), d = 1.f + e;
+            return div_<FAST>(4.f * e, d * d);
+        }
+        case SRMI_ACT_SIGMOID: {
+            const float e = exp_<FAST>(-fabsf(z)), d = 1.f + e;
+            return div_<FAST>(e, d * d);
+        }
+        case SRMI_ACT_GELU:
+            return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.3989422804014327f * exp_<FAST>(-0.5f * z * z);
+        case SRMI_ACT_GELU_TANH: {
+            const float s = logistic<FAST>(GELU_2C * (z + GELU_K * z * z * z));
+            return s + z * s * (1.f - s) * GELU_2C * (1.f + 3.f * GELU_K * z * z);
+        }
+        case SRMI_ACT_SILU: {
+            const float s = logistic<FAST>(z);
+            return s + z * s * (1.f - s);
+        }
+        default: return 1.f;
+    }
+}
+
+}  // namespace srmi

@@ -16,6 +16,9 @@ F32, BF16 = 0, 1
 NHWC, NCHW = 0, 1
 COMPUTE_F32, COMPUTE_BF16 = 0, 1
 ACT_NONE, ACT_PRELU, ACT_LRELU, ACT_RELU, ACT_TANH, ACT_SIGMOID, ACT_ADD_RELU = 0, 1, 2, 3, 4, 5, 6
+ACT_GELU, ACT_GELU_TANH, ACT_SILU = 7, 8, 9        # row operators only
+PASS_FWD, PASS_BWD = 0, 1
+ROWS_MAX = 0x7fffffffff
 SHUFFLE_CRD, SHUFFLE_DCR = 0, 1
 
 
@@ -76,6 +79,21 @@ class CropItem(C.Structure):
         ("lr_offset", C.c_int64), ("gt_offset", C.c_int64),
         ("lr_h", C.c_int32), ("lr_w", C.c_int32), ("iy", C.c_int32), ("ix", C.c_int32),
         ("flags", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class LinearDesc(C.Structure):
+    _fields_ = [
+        ("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32),
+        ("dtype", C.c_int32), ("act", C.c_int32), ("act_param", C.c_float), ("reserved", C.c_int32),
+        ("ldx", C.c_int64), ("ldw", C.c_int64), ("ldr", C.c_int64), ("lddy", C.c_int64),
+    ]
+
+
+class NormDesc(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("C", C.c_int32), ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("eps", C.c_float),
+        ("ldx", C.c_int64), ("lddy", C.c_int64),
     ]
 
 
@@ -145,6 +163,14 @@ SYMBOLS = {
                                    C.c_void_p, C.c_void_p]),
     "srmi_adam_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_double, C.c_double,
                                  C.c_double, C.c_double, C.c_int32, C.c_void_p]),
+    "srmi_linear_workspace_bytes": (C.c_int, [C.POINTER(LinearDesc), C.c_int32, C.POINTER(C.c_size_t)]),
+    "srmi_linear_fwd": (C.c_int, [C.POINTER(LinearDesc)] + [C.c_void_p] * 7 + [C.c_size_t, C.c_void_p]),
+    "srmi_linear_bwd": (C.c_int, [C.POINTER(LinearDesc)] + [C.c_void_p] * 8 + [C.c_size_t, C.c_void_p]),
+    "srmi_layer_norm_fwd": (C.c_int, [C.POINTER(NormDesc)] + [C.c_void_p] * 7),
+    "srmi_layer_norm_workspace_bytes": (C.c_int, [C.POINTER(NormDesc), C.POINTER(C.c_size_t)]),
+    "srmi_layer_norm_bwd": (C.c_int, [C.POINTER(NormDesc)] + [C.c_void_p] * 9 + [C.c_size_t, C.c_void_p]),
+    "srmi_dropout": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int32, C.c_double, C.c_uint64, C.c_uint64,
+                               C.c_void_p, C.c_void_p]),
 }
 REDUCE_WS_BYTES = 16384
 METRICS_MAX_BATCH = 256

@@ -1,0 +1,148 @@
+"""CPU: refusals of the row operators - Python checks and the C ABI's validation, which comes before any launch."""
+import ctypes as C
+
+import pytest
+import torch
+import torch.nn as nn
+
+from srmi import _lib as L
+from srmi import rows
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.randn(3, 8), torch.randn(5, 8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        rows.linear(x, w)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        rows.layer_norm(x)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        rows.dropout(x, 0.5, 1)
+
+
+def test_non_tensors_are_refused():
+    with pytest.raises(TypeError):
+        rows.linear([1.0], torch.randn(1, 1))
+    with pytest.raises(TypeError):
+        rows.layer_norm(3.0)
+
+
+def test_modules_refuse_what_they_cannot_run():
+    with pytest.raises(NotImplementedError):
+        rows.Linear(4, 4, act=nn.PReLU())
+    with pytest.raises(NotImplementedError):
+        rows.Linear(4, 4, act=nn.Hardtanh())
+    with pytest.raises(NotImplementedError):
+        rows.LayerNorm((4, 4))
+    with pytest.raises(ValueError):
+        rows.Dropout(1.5)
+    lin, ref = rows.Linear(4, 3, act=nn.GELU()), nn.Linear(4, 3)
+    assert list(lin.state_dict()) == list(ref.state_dict())
+    assert list(rows.LayerNorm(8).state_dict()) == list(nn.LayerNorm(8).state_dict())
+
+
+def test_struct_layout():
+    assert C.sizeof(L.LinearDesc) == 8 + 6 * 4 + 4 * 8
+    assert L.LinearDesc.ldx.offset == 32
+    assert C.sizeof(L.NormDesc) == 8 + 4 * 4 + 2 * 8
+
+
+def _lin(**kw):
+    d = L.LinearDesc(4, 8, 16, L.F32, L.ACT_NONE, 0.0, 0, 16, 16, 8, 8)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("field,value", [("M", -1), ("N", -1), ("K", -2), ("M", L.ROWS_MAX + 1), ("dtype", 2), ("act", L.ACT_PRELU),
+                                         ("act", L.ACT_ADD_RELU), ("act", 10), ("act", -1), ("ldx", 15), ("ldw", 0), ("ldr", 7), ("lddy", 3),
+                                         ("ldr", -8)])
+def test_linear_descriptor_refusals(field, value):
+    lib, n = L.load(), C.c_size_t(0)
+    d = _lin(**{field: value})
+    assert lib.srmi_linear_workspace_bytes(C.byref(d), L.PASS_FWD, C.byref(n)) < 0
+    assert lib.srmi_last_error() != b""
+    big = 1 << 40
+    assert lib.srmi_linear_fwd(C.byref(d), big, big, None, None, big, None, big, big, None) < 0
+    assert lib.srmi_linear_bwd(C.byref(d), big, big, big, big, big, big, big, big, big, None) < 0
+
+
+def test_linear_argument_refusals():
+    lib, n = L.load(), C.c_size_t(0)
+    d = _lin()
+    assert lib.srmi_linear_workspace_bytes(None, 0, C.byref(n)) == -1
+    assert lib.srmi_linear_workspace_bytes(C.byref(d), 2, C.byref(n)) == -1
+    assert lib.srmi_linear_workspace_bytes(C.byref(d), 0, None) == -1
+    big = 1 << 40
+    for hole in range(3):                                                       # x, w, y
+        a = [big, big, big]
+        a[hole] = None
+        assert lib.srmi_linear_fwd(C.byref(d), a[0], a[1], None, None, a[2], None, None, 0, None) == -1
+    assert lib.srmi_linear_fwd(C.byref(d), big + 2, big, None, None, big, None, None, 0, None) == -1     # not on an element
+    assert lib.srmi_linear_fwd(C.byref(_lin(ldr=0)), big, big, None, big, big, None, None, 0, None) == -1
+    assert lib.srmi_linear_bwd(C.byref(d), big, big, None, None, big, big, big, None, 0, None) == -1     # no dy
+    assert lib.srmi_linear_bwd(C.byref(_lin(act=L.ACT_GELU)), big, big, None, big, big, big, big, None, 0, None) == -1   # no z
+    assert lib.srmi_linear_bwd(C.byref(d), None, big, None, big, None, big, None, big, 1 << 30, None) == -1     # dw without x
+    assert lib.srmi_linear_bwd(C.byref(d), big, None, None, big, big, None, None, big, 1 << 30, None) == -1     # dx without w
+    L.check(lib.srmi_linear_workspace_bytes(C.byref(_lin(act=L.ACT_GELU)), L.PASS_BWD, C.byref(n)))
+    assert n.value > 0
+    assert lib.srmi_linear_bwd(C.byref(_lin(act=L.ACT_GELU)), big, big, big, big, big, big, big, big, n.value - 1, None) == -1
+    assert lib.srmi_linear_bwd(C.byref(_lin(act=L.ACT_GELU)), big, big, big, big, big, big, big, None, n.value, None) == -1
+    assert lib.srmi_linear_bwd(C.byref(_lin(act=L.ACT_GELU)), big, big, big, big, big, big, big, big + 16, n.value, None) == -1
+    assert lib.srmi_linear_fwd(C.byref(_lin(M=0)), None, None, None, None, None, None, None, 0, None) == 0     # nothing to do
+    assert lib.srmi_linear_fwd(C.byref(_lin(N=0)), None, None, None, None, None, None, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(rows=-1), dict(C=0), dict(C=-4), dict(dtype=5), dict(param_dtype=5), dict(eps=-1.0), dict(eps=float("nan")),
+                                dict(ldx=7), dict(lddy=7), dict(rows=L.ROWS_MAX + 1)])
+def test_norm_descriptor_refusals(kw):
+    lib, n = L.load(), C.c_size_t(0)
+    d = L.NormDesc(4, 8, L.F32, L.F32, 1e-5, 8, 8)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    big = 1 << 40
+    assert lib.srmi_layer_norm_workspace_bytes(C.byref(d), C.byref(n)) < 0
+    assert lib.srmi_layer_norm_fwd(C.byref(d), big, None, None, big, None, None, None) < 0
+    assert lib.srmi_layer_norm_bwd(C.byref(d), big, None, big, big, big, big, big, big, big, big, None) < 0
+
+
+def test_norm_argument_refusals():
+    lib, n = L.load(), C.c_size_t(0)
+    d = L.NormDesc(4, 8, L.F32, L.F32, 1e-5, 8, 8)
+    big = 1 << 40
+    assert lib.srmi_layer_norm_fwd(None, big, None, None, big, None, None, None) == -1
+    assert lib.srmi_layer_norm_fwd(C.byref(d), None, None, None, big, None, None, None) == -1
+    assert lib.srmi_layer_norm_fwd(C.byref(d), big, None, None, None, None, None, None) == -1
+    assert lib.srmi_layer_norm_fwd(C.byref(d), big, None, None, big, big, None, None) == -1              # mean without rstd
+    assert lib.srmi_layer_norm_fwd(C.byref(d), big + 1, None, None, big, None, None, None) == -1
+    assert lib.srmi_layer_norm_bwd(C.byref(d), big, None, big, big, None, big, None, None, None, 0, None) == -1
+    L.check(lib.srmi_layer_norm_workspace_bytes(C.byref(d), C.byref(n)))
+    assert lib.srmi_layer_norm_bwd(C.byref(d), big, None, big, big, big, None, big, None, big, n.value - 1, None) == -1
+    assert lib.srmi_layer_norm_bwd(C.byref(d), big, None, big, big, big, None, None, None, None, 0, None) == 0     # nothing wanted
+
+
+def test_dropout_argument_refusals():
+    lib, big = L.load(), 1 << 40
+    for p in (-0.1, 1.1, float("nan")):
+        assert lib.srmi_dropout(big, None, big, 8, L.F32, p, 0, 0, None, None) == -1
+    assert lib.srmi_dropout(big, None, big, 8, 7, 0.5, 0, 0, None, None) == -1
+    assert lib.srmi_dropout(None, None, big, 8, L.F32, 0.5, 0, 0, None, None) == -1
+    assert lib.srmi_dropout(big, None, None, 8, L.F32, 0.5, 0, 0, None, None) == -1
+    assert lib.srmi_dropout(big + 1, None, big, 8, L.BF16, 0.5, 0, 0, None, None) == -1
+    assert lib.srmi_dropout(big, None, big, 8, L.F32, 0.5, 0, 0, big + 4, None) == -1
+    assert lib.srmi_dropout(None, None, None, 0, L.F32, 0.5, 0, 0, None, None) == 0
+
+
+def test_strided_rows_finds_uniform_strides():
+    buf = torch.arange(2 * 3 * 40.).reshape(2, 3, 40)
+    t, ld = rows._strided_rows(buf[..., 5:13])
+    assert t.data_ptr() == buf[..., 5:13].data_ptr() and ld == 40
+    t, ld = rows._strided_rows(buf[:, 1:2, 5:13])
+    assert ld == 120 and t.data_ptr() == buf[:, 1:2, 5:13].data_ptr()
+    for bad in (buf[:, :2, 5:13], buf.transpose(1, 2), buf[0, :1].expand(4, 40), buf[..., :1].expand(2, 3, 8), buf[0].t()):
+        t, ld = rows._strided_rows(bad)
+        assert t.is_contiguous() and ld == bad.shape[-1] and torch.equal(t, bad)
+    one, ld = rows._strided_rows(buf[:1, :1, 5:13])
+    assert ld == 8
+    maps = torch.randn(2, 6, 4, 5).to(memory_format=torch.channels_last).permute(0, 2, 3, 1)
+    t, ld = rows._strided_rows(maps)
+    assert t is maps and ld == 6

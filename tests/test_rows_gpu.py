@@ -1,0 +1,624 @@
+"""GPU: the row operators against plain 64-bit implementations, forward and backward.
+
+Bounds are derived, not fitted.  u = 2^-24 is half a step of f32, s = finfo(dtype).eps / 2 half a step of the storage type.
+A sum of n products accumulated in f32 in any order is off by at most about n u sum|terms|; every stored value by s of itself.
+In bf16 the backward pass rounds the pre-activation it keeps and dz = dy act'(z) once each: both appear as per-term errors.
+"""
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+from srmi import autograd as AG
+from srmi import rows
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+TINY = 2.0 ** -120
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+ACTS = {"none": None, "relu": nn.ReLU(), "lrelu": nn.LeakyReLU(0.2), "tanh": nn.Tanh(), "sigmoid": nn.Sigmoid(), "gelu": nn.GELU(),
+        "gelu_tanh": nn.GELU(approximate="tanh"), "silu": nn.SiLU()}
+# largest |act'| and |act''| (0 away from the kink of the piecewise linear ones)
+LIP = {"none": 1, "relu": 1, "lrelu": 1, "tanh": 1, "sigmoid": 0.25, "gelu": 1.13, "gelu_tanh": 1.13, "silu": 1.1}
+CURV = {"none": 0, "relu": 0, "lrelu": 0, "tanh": 0.77, "sigmoid": 0.097, "gelu": 0.8, "gelu_tanh": 0.8, "silu": 0.5}
+# own error of the act / slope evaluation relative to max(|value|, |z|-scaled terms): bf16 uses the hardware's 2^x and reciprocal
+FN = {"f32": 64 * U, "bf16": 2.0 ** -14}
+
+
+def half_step(dt):
+    return torch.finfo(DT[dt]).eps / 2
+
+
+def act64(z, name):
+    if name == "none":
+        return z, torch.ones_like(z)
+    zz = z.clone().requires_grad_()
+    y = ACTS[name](zz) if name not in ("relu", "lrelu") else torch.where(zz > 0, zz, zz * (0.2 if name == "lrelu" else 0.0))
+    (g,) = torch.autograd.grad(y.sum(), zz)
+    return y.detach(), g
+
+
+def assert_within(got, want, bound, what):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    if not got.numel():
+        return
+    excess = (got - want).abs() - bound
+    k = int(excess.argmax())
+    assert torch.isfinite(got).all() and float(excess.max()) <= 0, \
+        f"{what}: |{float(got.flatten()[k])} - {float(want.flatten()[k])}| over its bound {float(bound.flatten()[k]):.3g}"
+
+
+def make(shape, dt, gen, scale=1.0, pitch=0):
+    wide = list(shape)
+    if pitch:
+        wide[-1] += pitch
+    t = (torch.randn(wide, generator=gen) * scale).to(DT[dt]).to(DEV)
+    return t[..., pitch:] if pitch else t
+
+
+def linear_case(M, K, N, dt, act, bias, res, pitch, seed, lead=None):
+    gen = torch.Generator().manual_seed(seed)
+    x = make((lead or (M,)) + (K,) if not isinstance(lead, tuple) else lead + (K,), dt, gen, pitch=pitch)
+    w = make((N, K), dt, gen, 1 / math.sqrt(max(K, 1)), pitch=pitch)
+    b = make((N,), dt, gen, 0.1) if bias else None
+    r = make(tuple(x.shape[:-1]) + (N,), dt, gen, pitch=pitch) if res else None
+    dy = make(tuple(x.shape[:-1]) + (N,), dt, gen, pitch=pitch)
+    leaves = [t.requires_grad_() if t is not None else None for t in (x, w, b, r)]
+    return leaves, dy
+
+
+def check_linear(leaves, dy, dt, act, run=None):
+    x, w, b, r = leaves
+    N, K = w.shape
+    M = math.prod(x.shape[:-1])
+    y = (run or (lambda: rows.linear(x, w, b, act=ACTS[act], residual=r)))()
+    assert y.dtype == DT[dt] and y.is_contiguous() and y.shape == x.shape[:-1] + (N,)
+    wanted = [t for t in leaves if t is not None]
+    grads = dict(zip([k for k, t in zip("xwbr", leaves) if t is not None], torch.autograd.grad(y, wanted, dy)))
+
+    x64, w64 = x.detach().double().cpu().reshape(M, K), w.detach().double().cpu()
+    b64 = b.detach().double().cpu() if b is not None else torch.zeros(N, dtype=torch.float64)
+    dy64 = dy.double().cpu().reshape(M, N)
+    z = x64 @ w64.t() + b64
+    f, g = act64(z, act)
+    s, fn = half_step(dt), FN[dt]
+    # z: K products + bias; the f32 path splits operands into three bf16 parts and drops products below 2^-24 (4 u)
+    ez = (K + 8) * U * (x64.abs() @ w64.abs().t() + b64.abs())
+    out = f + (r.detach().double().cpu().reshape(M, N) if r is not None else 0)
+    ey = LIP[act] * ez + fn * (f.abs() + 0.01 * z.abs()) + 2 * U * out.abs() + s * out.abs() + TINY
+    assert_within(y.reshape(M, N), out, ey + s * ey, f"y {act}")
+
+    dz = dy64 * g
+    zq = (s if dt == "bf16" else 0) * z.abs() + ez                      # the kept pre-activation
+    edz = dy64.abs() * (CURV[act] * zq + fn * (g.abs() + 0.01) * (act != "none"))
+    if act in ("relu", "lrelu"):
+        edz = edz + dy64.abs() * (z.abs() <= ez)                        # either slope within a rounding of the kink
+    edz_q = edz + (s if act != "none" else 0) * (dz.abs() + edz)        # dz as the products read it (act none: dy itself)
+    if "b" in grads:
+        e = edz.sum(0) + (M + 8) * U * dz.abs().sum(0)
+        want = dz.sum(0)
+        assert_within(grads["b"], want, e * (1 + s) + s * want.abs() + TINY, f"db {act}")
+    want = dz @ w64
+    e = edz_q @ w64.abs() + (N + 8) * U * ((dz.abs() + edz_q) @ w64.abs())
+    assert_within(grads["x"].reshape(M, K), want, e * (1 + s) + s * want.abs() + TINY, f"dx {act}")
+    want = dz.t() @ x64
+    e = edz_q.t() @ x64.abs() + (M + 8) * U * ((dz.abs() + edz_q).t() @ x64.abs())
+    assert_within(grads["w"], want, e * (1 + s) + s * want.abs() + TINY, f"dw {act}")
+    if r is not None:
+        assert torch.equal(grads["r"], dy)
+
+
+SIZES = [(1, 1, 1), (1, 16, 1), (2, 3, 5), (1, 1024, 264), (7, 64, 64), (16, 520, 72), (17, 1030, 33), (33, 2048, 16), (64, 96, 130),
+         (65, 64, 256), (129, 257, 129), (256, 128, 256), (300, 512, 200), (1000, 40, 24), (515, 1152, 384)]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_linear_sizes(M, K, N, dt):
+    leaves, dy = linear_case(M, K, N, dt, "gelu", True, True, 0, 1000 * M + K + N)
+    check_linear(leaves, dy, dt, "gelu")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("act", sorted(ACTS))
+@pytest.mark.parametrize("bias,res", [(True, False), (False, True)])
+def test_linear_activations(act, bias, res, dt):
+    leaves, dy = linear_case(70, 96, 136, dt, act, bias, res, 0, 5)
+    check_linear(leaves, dy, dt, act)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("pitch", [1, 8, 13])
+def test_linear_strided_rows(pitch, dt):
+    for M, K, N in ((5, 72, 40), (200, 136, 144)):
+        leaves, dy = linear_case(M, K, N, dt, "silu", True, True, pitch, 6)
+        check_linear(leaves, dy, dt, "silu")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("lead", [(), (3, 1, 5), (2, 7)])
+def test_linear_leading_axes(lead, dt):
+    leaves, dy = linear_case(None, 48, 24, dt, "none", True, False, 0, 7, lead=lead)
+    check_linear(leaves, dy, dt, "none")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("M,K,N", [(0, 8, 5), (4, 0, 6), (4, 8, 0), (0, 0, 0)])
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_linear_empty(M, K, N, dt, act):
+    leaves, dy = linear_case(M, K, N, dt, act, True, True, 0, 8)
+    check_linear(leaves, dy, dt, act)
+
+
+def test_linear_transposed_and_broadcast_operands_are_copied():
+    gen = torch.Generator().manual_seed(9)
+    x = make((40, 9), "f32", gen).t().requires_grad_()                       # [9, 40], last axis strided
+    w = make((40, 6), "f32", gen).t().requires_grad_()
+    b = make((1,), "f32", gen).expand(6)
+    y = rows.linear(x, w, b)
+    torch.testing.assert_close(y, x @ w.t() + b, rtol=1e-5, atol=1e-5)
+    gx, gw = torch.autograd.grad(y.sum(), (x, w))                            # dy is an expanded scalar
+    torch.testing.assert_close(gx, torch.ones_like(y) @ w, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(gw, torch.ones_like(y).t() @ x, rtol=1e-5, atol=1e-5)
+
+
+def test_linear_broadcast_bias_gradient():
+    gen = torch.Generator().manual_seed(10)
+    x, w = make((50, 16), "f32", gen), make((6, 16), "f32", gen)
+    b = make((1,), "f32", gen).requires_grad_()
+    y = rows.linear(x, w, b.expand(6), act=nn.Tanh())
+    (g,) = torch.autograd.grad(y, b, torch.ones_like(y))
+    want = (1 - torch.tanh(x.double() @ w.double().t() + b.double()) ** 2).sum()
+    assert abs(float(g) - float(want)) <= 300 * 40 * U * float(want)
+
+
+def test_linear_gradients_by_differences():
+    # central differences of f(h) = sum(dy * y(theta + h v)) in f32: step h = 2^-8, truncation ~ h^2, noise ~ 2^-24 * |f| / h
+    gen = torch.Generator().manual_seed(11)
+    leaves, dy = linear_case(33, 24, 20, "f32", "gelu", True, False, 0, 11)
+    x, w, b, _ = leaves
+    y = rows.linear(x, w, b, act=nn.GELU())
+    grads = torch.autograd.grad(y, (x, w, b), dy)
+    h = 2.0 ** -8
+    for k, t in enumerate((x, w, b)):
+        v = torch.randn(t.shape, generator=gen).to(DEV)
+        v /= v.norm()
+        args = [a.detach() for a in (x, w, b)]
+        f = []
+        for sign in (1, -1):
+            moved = list(args)
+            moved[k] = args[k] + sign * h * v
+            f.append(float((rows.linear(*moved, act=nn.GELU()).double() * dy.double()).sum()))
+        slope = float((grads[k].double() * v.double()).sum())
+        terms = float(dy.double().abs().sum())
+        assert abs((f[0] - f[1]) / (2 * h) - slope) <= 2 * h * h * terms + 64 * U * terms / h
+
+
+def test_linear_partial_gradients():
+    leaves, dy = linear_case(40, 32, 24, "bf16", "silu", True, False, 0, 12)
+    full = torch.autograd.grad(rows.linear(leaves[0], leaves[1], leaves[2], act=nn.SiLU()), leaves[:3], dy)
+    for k in range(3):
+        args = [t.detach().requires_grad_(j == k) for j, t in enumerate(leaves[:3])]
+        (g,) = torch.autograd.grad(rows.linear(*args, act=nn.SiLU()), args[k], dy)
+        assert torch.equal(g, full[k])
+
+
+def test_linear_same_call_same_bits():
+    for dt in ("bf16", "f32"):
+        leaves, dy = linear_case(700, 320, 192, dt, "gelu", True, True, 0, 13)
+        runs = []
+        for _ in range(2):
+            y = rows.linear(leaves[0], leaves[1], leaves[2], act=nn.GELU(), residual=leaves[3])
+            runs.append([y] + list(torch.autograd.grad(y, leaves, dy)))
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_linear_leaves_neighbours_alone():
+    # outputs are dense, but operands are slices of wider buffers: nothing outside them is written
+    gen = torch.Generator().manual_seed(14)
+    wide = make((30, 64), "bf16", gen)
+    before = wide.clone()
+    x = wide[:, 8:40].requires_grad_()
+    w = make((24, 32), "bf16", gen).requires_grad_()
+    y = rows.linear(x, w, act=nn.ReLU())
+    torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    assert torch.equal(wide, before)
+
+
+def test_linear_nonfinite_rows_stay_in_their_rows():
+    gen = torch.Generator().manual_seed(15)
+    for dt in ("bf16", "f32"):
+        x, w = make((130, 72), dt, gen), make((70, 72), dt, gen)
+        ref = rows.linear(x, w)
+        bad = x.clone()
+        bad[3, 5], bad[77, 0] = float("nan"), float("inf")
+        got = rows.linear(bad, w)
+        keep = torch.ones(130, dtype=torch.bool, device=DEV)
+        keep[[3, 77]] = False
+        assert torch.equal(got[keep], ref[keep]) and not torch.isfinite(got[~keep]).any()
+
+
+# ---- layer norm ----------------------------------------------------------------------------------------------------------
+def check_norm(x, w, b, dy, dt, pdt):
+    c = x.shape[-1]
+    y = rows.layer_norm(x, w, b, eps=1e-5)
+    leaves = [t for t in (x, w, b) if t is not None and t.requires_grad]
+    names = [k for k, t in zip("xwb", (x, w, b)) if t is not None and t.requires_grad]
+    grads = dict(zip(names, torch.autograd.grad(y, leaves, dy)))
+    x64, dy64 = x.detach().double().cpu().reshape(-1, c), dy.double().cpu().reshape(-1, c)
+    w64 = w.detach().double().cpu() if w is not None else torch.ones(c, dtype=torch.float64)
+    b64 = b.detach().double().cpu() if b is not None else torch.zeros(c, dtype=torch.float64)
+    n = x64.shape[0]
+    mean = x64.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(x64.var(1, unbiased=False, keepdim=True) + 1e-5)
+    xh = (x64 - mean) * rstd
+    s, sp, k = half_step(dt), half_step(pdt), c + 16
+    big = x64.abs().amax(1, keepdim=True) * rstd                         # |x| in units of the deviation: what subtracting the mean loses
+    exh = k * U * (big + xh.abs() * (1 + big) + xh.abs())                # mean, variance (through the mean) and rstd
+    want = xh * w64 + b64
+    e = w64.abs() * exh + 4 * U * (w64 * xh).abs() + 2 * U * want.abs()
+    assert y.dtype == DT[dt] and y.is_contiguous()
+    assert_within(y.reshape(-1, c), want, e * (1 + s) + s * want.abs() + TINY, "y")
+    g = dy64 * w64
+    G = g.abs().mean(1, keepdim=True)
+    c2 = (g * xh).mean(1, keepdim=True)
+    GA = (g * xh).abs().mean(1, keepdim=True)
+    ec2 = k * U * GA + (g.abs() * exh).mean(1, keepdim=True)
+    want = rstd * (g - g.mean(1, keepdim=True) - xh * c2)
+    e = rstd * (k * U * (g.abs() + G + xh.abs() * c2.abs()) * (1 + big) + exh * c2.abs() + (xh.abs() + exh) * ec2)
+    if "x" in grads:
+        assert_within(grads["x"].reshape(-1, c), want, e * (1 + s) + s * want.abs() + TINY, "dx")
+    if "w" in grads:
+        want = (dy64 * xh).sum(0)
+        e = (dy64.abs() * exh).sum(0) + (n + 16) * U * (dy64 * xh).abs().sum(0)
+        assert_within(grads["w"], want, e * (1 + sp) + sp * want.abs() + TINY, "dw")
+    if "b" in grads:
+        want = dy64.sum(0)
+        assert_within(grads["b"], want, (n + 16) * U * dy64.abs().sum(0) * (1 + sp) + sp * want.abs() + TINY, "db")
+
+
+def norm_case(n, c, dt, pdt, affine, pitch, seed, lead=None):
+    gen = torch.Generator().manual_seed(seed)
+    shape = (lead or (n,)) + (c,)
+    x = make(shape, dt, gen, 1.5, pitch=pitch)
+    x = (x + 0.75).detach() if not pitch else x
+    w = (1 + make((c,), pdt, gen, 0.2)).requires_grad_() if affine else None
+    b = make((c,), pdt, gen, 0.2).requires_grad_() if affine else None
+    return x.requires_grad_(), w, b, make(shape, dt, gen, pitch=pitch)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("c", [1, 2, 5, 8, 16, 24, 64, 65, 128, 136, 256, 300, 512, 771, 1024, 1025, 1032, 2048, 2052, 2056, 4099, 8192, 20000])
+def test_norm_widths(c, dt):
+    for n in (1, 37):
+        check_norm(*norm_case(n, c, dt, dt, True, 0, c + n), dt, dt)
+
+
+@pytest.mark.parametrize("dt,pdt", [("bf16", "f32"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("affine", [True, False])
+@pytest.mark.parametrize("pitch", [0, 3, 8])
+def test_norm_forms(dt, pdt, affine, pitch):
+    for n, c in ((5, 96), (1111, 64), (3000, 33)):
+        check_norm(*norm_case(n, c, dt, pdt, affine, pitch, n + pitch), dt, pdt)
+
+
+def test_norm_empty_rows_and_leading_axes():
+    for dt in ("bf16", "f32"):
+        check_norm(*norm_case(0, 32, dt, dt, True, 0, 1), dt, dt)
+        check_norm(*norm_case(None, 40, dt, dt, True, 0, 2, lead=(2, 3, 5)), dt, dt)
+        x = torch.randn(40, device=DEV).to(DT[dt])                          # a single row without leading axes
+        torch.testing.assert_close(rows.layer_norm(x), rows.layer_norm(x[None])[0], rtol=0, atol=0)
+
+
+def test_norm_weight_or_bias_alone():
+    gen = torch.Generator().manual_seed(3)
+    x, w = make((9, 48), "f32", gen), make((48,), "f32", gen)
+    y0 = rows.layer_norm(x)
+    torch.testing.assert_close(rows.layer_norm(x, weight=w), y0 * w, rtol=1e-6, atol=1e-6)
+    torch.testing.assert_close(rows.layer_norm(x, bias=w), y0 + w, rtol=1e-6, atol=1e-6)
+    b = w.clone().requires_grad_()
+    y = rows.layer_norm(x, bias=b)
+    (g,) = torch.autograd.grad(y, b, torch.ones_like(y))
+    assert torch.equal(g, torch.full_like(g, 9.0))
+
+
+def test_norm_constant_and_offset_rows():
+    # a constant row has variance 0: xh = 0 exactly; a large common offset must not eat the deviations (two-pass variance)
+    x = torch.full((4, 256), 3.0, device=DEV)
+    assert torch.equal(rows.layer_norm(x), torch.zeros_like(x))
+    gen = torch.Generator().manual_seed(4)
+    d = torch.randint(-8, 9, (5, 256), generator=gen).double()
+    x = (d + 2.0 ** 14).float().to(DEV)                                     # exact in f32
+    want = (d - d.mean(1, keepdim=True)) / torch.sqrt(d.var(1, unbiased=False, keepdim=True) + 1e-5)
+    assert float((rows.layer_norm(x).double().cpu() - want).abs().max()) <= 256 * U * 2.0 ** 14 * 2
+
+
+def test_norm_same_call_same_bits_and_eps():
+    x, w, b, dy = norm_case(5000, 192, "bf16", "bf16", True, 0, 5)
+    runs = []
+    for _ in range(2):
+        y = rows.layer_norm(x, w, b, eps=0.5)
+        runs.append([y] + list(torch.autograd.grad(y, (x, w, b), dy)))
+    assert all(torch.equal(p, q) for p, q in zip(*runs))
+    x64 = x.detach().double()
+    want = (x64 - x64.mean(1, keepdim=True)) / torch.sqrt(x64.var(1, unbiased=False, keepdim=True) + 0.5) * w.double() + b.double()
+    assert float((runs[0][0].double() - want).abs().max()) <= 2.0 ** -8 * float(want.abs().max())
+
+
+# ---- dropout -------------------------------------------------------------------------------------------------------------
+def philox(n, seed, offset):
+    """word i % 4 of the Philox4x32-10 block with counter (i // 4, offset) and key seed, in Python integers"""
+    out, m = [], 0xFFFFFFFF
+    for block in range((n + 3) // 4):
+        c = [block & m, block >> 32, offset & m, offset >> 32]
+        k0, k1 = seed & m, seed >> 32
+        for _ in range(10):
+            a, b = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+            c = [(b >> 32) ^ c[1] ^ k0, b & m, (a >> 32) ^ c[3] ^ k1, a & m]
+            k0, k1 = (k0 + 0x9E3779B9) & m, (k1 + 0xBB67AE85) & m
+        out += c
+    return torch.tensor(out[:n], dtype=torch.float64)
+
+
+def test_philox_known_answers():
+    # published test vectors of Philox4x32-10: counter and key of all zeros and of all ones
+    assert [int(v) for v in philox(4, 0, 0)] == [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [1, 3, 4, 7, 8, 255, 2049])
+@pytest.mark.parametrize("p", [0.0, 0.1, 0.5, 1.0])
+def test_dropout_mask_and_values(n, p, dt):
+    gen = torch.Generator().manual_seed(n)
+    seed, offset = 0xDEADBEEF12345678, (1 << 40) + 17
+    keep = philox(n, seed, offset) >= math.floor(p * 2 ** 32)
+    s = half_step(dt)
+    for res in (False, True):
+        for shift in (0, 1):                                                # shift 1: off the 16-byte boundary
+            x = make((n + shift,), dt, gen)[shift:].requires_grad_()
+            r = make((n + shift,), dt, gen)[shift:].requires_grad_() if res else None
+            y = rows.dropout(x, p, seed, offset, residual=r)
+            scaled = torch.where(keep, x.detach().double().cpu() * (1 / (1 - p) if p < 1 else 0.0), torch.zeros(n, dtype=torch.float64))
+            want = scaled + (r.detach().double().cpu() if res else 0)
+            assert_within(y, want, 4 * U * (scaled.abs() + want.abs()) + s * want.abs() + TINY, "y")
+            dy = make((n,), dt, gen)
+            g = torch.autograd.grad(y, [x] + ([r] if res else []), dy)
+            want = torch.where(keep, dy.double().cpu() * (1 / (1 - p) if p < 1 else 0.0), torch.zeros(n, dtype=torch.float64))
+            assert_within(g[0], want, 4 * U * want.abs() + s * want.abs() + TINY, "dx")
+            assert not res or torch.equal(g[1], dy)
+
+
+def test_dropout_drops_what_is_not_finite():
+    x = torch.full((4096,), float("nan"), device=DEV)
+    x[::2] = float("inf")
+    y = rows.dropout(x, 0.5, 7)
+    keep = philox(4096, 7, 0) >= 2 ** 31
+    assert torch.equal(y.cpu()[~keep], torch.zeros(int((~keep).sum()))) and not torch.isfinite(y.cpu()[keep]).any()
+    assert torch.equal(rows.dropout(x, 1.0, 7), torch.zeros_like(x))
+
+
+def test_dropout_rate_and_streams_differ():
+    x = torch.ones(1 << 20, device=DEV)
+    a, b, c = (rows.dropout(x, 0.25, s, o) for s, o in ((1, 0), (1, 1), (2, 0)))
+    # kept counts are binomial: 6 standard deviations of sqrt(n p q)
+    assert abs(int((a != 0).sum()) - 0.75 * 2 ** 20) <= 6 * math.sqrt(2 ** 20 * 0.1875)
+    for u, v in ((a, b), (a, c), (b, c)):
+        agree = int(((u != 0) == (v != 0)).sum())
+        assert abs(agree - 0.625 * 2 ** 20) <= 6 * math.sqrt(2 ** 20 * 0.625 * 0.375)
+
+
+def test_dropout_device_counter_and_its_guard():
+    x = torch.randn(1000, device=DEV, requires_grad=True)
+    rng = torch.tensor([11, 5], dtype=torch.int64, device=DEV)
+    y = rows.dropout(x, 0.3, rng)
+    assert torch.equal(y, rows.dropout(x, 0.3, 11, 5))
+    rng[1] += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    assert torch.equal(rows.dropout(x.detach(), 0.3, rng), rows.dropout(x.detach(), 0.3, 11, 6))
+
+
+def test_dropout_module():
+    m = rows.Dropout(0.5, seed=3)
+    x = torch.randn(64, 32, device=DEV)
+    a, b = m(x), m(x)
+    assert m.calls == 2 and torch.equal(a, rows.dropout(x, 0.5, 3, 1)) and torch.equal(b, rows.dropout(x, 0.5, 3, 2))
+    assert torch.equal(m(x, residual=x), rows.dropout(x, 0.5, 3, 3, residual=x))
+    m.eval()
+    assert m(x) is x and torch.equal(m(x, residual=x), x + x)
+
+
+# ---- refusals on device tensors ------------------------------------------------------------------------------------------
+def test_refusals():
+    x, w = torch.randn(4, 8, device=DEV), torch.randn(6, 8, device=DEV)
+    for bad in (lambda: rows.linear(x, w.bfloat16()), lambda: rows.linear(x.double(), w.double()), lambda: rows.linear(x.half(), w.half()),
+                lambda: rows.layer_norm(x, torch.ones(8, device=DEV, dtype=torch.bfloat16)), lambda: rows.dropout(x.long(), 0.1, 0),
+                lambda: rows.layer_norm(x.bfloat16(), torch.ones(8, device=DEV), torch.ones(8, device=DEV, dtype=torch.bfloat16)),
+                lambda: rows.dropout(x, 0.1, torch.zeros(2, device=DEV))):
+        with pytest.raises(TypeError):
+            bad()
+    for bad in (lambda: rows.linear(x, w[:, :4]), lambda: rows.linear(x, w[0]), lambda: rows.linear(x, w, torch.zeros(8, device=DEV)),
+                lambda: rows.linear(x, w, residual=torch.zeros(1, 6, device=DEV)), lambda: rows.layer_norm(x, torch.ones(4, device=DEV)),
+                lambda: rows.layer_norm(x, eps=-1.0), lambda: rows.layer_norm(x, eps=float("nan")), lambda: rows.layer_norm(x[:, :0]),
+                lambda: rows.dropout(x, 1.5, 0), lambda: rows.dropout(x, 0.1, -1), lambda: rows.dropout(x, 0.1, 1 << 64),
+                lambda: rows.dropout(x, 0.1, 0, 1.5), lambda: rows.dropout(x, 0.1, 0, residual=x[:2]), lambda: rows.dropout(x, float("nan"), 0),
+                lambda: rows.dropout(x, 0.1, torch.zeros(2, device=DEV, dtype=torch.int64), 3),
+                lambda: rows.layer_norm(torch.tensor(1.0, device=DEV))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        rows.linear(x, w.cpu())
+    with pytest.raises(NotImplementedError):
+        rows.linear(x, w, act=nn.PReLU().to(DEV))
+
+
+# ---- a run of them together ----------------------------------------------------------------------------------------------
+def _mixer(t, p, conv_in=None):
+    h = rows.layer_norm(t, p["g"], p["b"])
+    h = rows.linear(h, p["w1"], p["b1"], act=nn.GELU())
+    h = rows.linear(h, p["w2"], p["b2"])
+    return rows.dropout(h, 0.2, 99, 4, residual=t)
+
+
+def _mixer64(t, p):
+    c = t.shape[-1]
+    m = t.mean(-1, keepdim=True)
+    h = (t - m) / torch.sqrt(((t - m) ** 2).mean(-1, keepdim=True) + 1e-5) * p["g"] + p["b"]
+    h = nn.functional.gelu(h @ p["w1"].t() + p["b1"]) @ p["w2"].t() + p["b2"]
+    keep = (philox(t.numel(), 99, 4) >= math.floor(0.2 * 2 ** 32)).double().reshape(t.shape)
+    return t + h * keep / 0.8
+
+
+def _mixer_params(c, hid, dt, gen):
+    p = {"g": 1 + make((c,), dt, gen, 0.1), "b": make((c,), dt, gen, 0.1), "w1": make((hid, c), dt, gen, c ** -0.5), "b1": make((hid,), dt, gen, 0.1),
+         "w2": make((c, hid), dt, gen, hid ** -0.5), "b2": make((c,), dt, gen, 0.1)}
+    return {k: v.requires_grad_() for k, v in p.items()}
+
+
+@pytest.mark.parametrize("dt,tol", [("f32", 2e-5), ("bf16", 0.04)])
+def test_channel_mixer(dt, tol):
+    # chained roundings: about a dozen of half a step each, over sums of O(1) terms - relative to the largest value
+    gen = torch.Generator().manual_seed(21)
+    t = make((2, 5, 7, 64), dt, gen).requires_grad_()
+    p = _mixer_params(64, 160, dt, gen)
+    y = _mixer(t, p)
+    dy = make(tuple(t.shape), dt, gen)
+    got = [y] + list(torch.autograd.grad(y, [t] + list(p.values()), dy))
+    t64 = t.detach().double().cpu().requires_grad_()
+    p64 = {k: v.detach().double().cpu().requires_grad_() for k, v in p.items()}
+    y64 = _mixer64(t64, p64)
+    want = [y64.detach()] + list(torch.autograd.grad(y64, [t64] + list(p64.values()), dy.double().cpu()))
+    for a, b in zip(got, want):
+        assert float((a.double().cpu() - b).abs().max()) <= tol * float(b.abs().max())
+
+
+def test_mixer_between_convolutions():
+    # the operators on a channels-last map between two fused convs of this package: no copies, gradients reach the first conv
+    torch.manual_seed(22)
+    gen = torch.Generator().manual_seed(22)
+    c1, c2 = nn.Conv2d(3, 32, 3, padding=1).to(DEV), nn.Conv2d(32, 3, 3, padding=1).to(DEV)
+    p = _mixer_params(32, 96, "f32", gen)
+    img = torch.randn(2, 3, 9, 11, generator=gen).to(DEV)
+    feat = AG.fused_conv(img, c1, None, nn.ReLU())
+    t = feat.permute(0, 2, 3, 1)
+    assert t.is_contiguous()
+    out = AG.fused_conv(_mixer(t, p).permute(0, 3, 1, 2), c2, None, None)
+    params = [c1.weight, c2.weight] + list(p.values())
+    got = [out] + list(torch.autograd.grad(out.square().mean(), params))
+    d1, d2 = nn.Conv2d(3, 32, 3, padding=1).double(), nn.Conv2d(32, 3, 3, padding=1).double()
+    d1.load_state_dict({k: v.double().cpu() for k, v in c1.state_dict().items()})
+    d2.load_state_dict({k: v.double().cpu() for k, v in c2.state_dict().items()})
+    p64 = {k: v.detach().double().cpu().requires_grad_() for k, v in p.items()}
+    f64 = torch.relu(d1(img.double().cpu())).permute(0, 2, 3, 1)
+    o64 = d2(_mixer64(f64, p64).permute(0, 3, 1, 2))
+    want = [o64.detach()] + list(torch.autograd.grad(o64.square().mean(), [d1.weight, d2.weight] + list(p64.values())))
+    for a, b in zip(got, want):
+        assert float((a.double().cpu() - b).abs().max()) <= 1e-4 * float(b.abs().max())
+
+
+def test_modules_train_together():
+    torch.manual_seed(23)
+    net = nn.Sequential(rows.LayerNorm(48), rows.Linear(48, 96, act=nn.SiLU()), rows.Linear(96, 48), rows.Dropout(0.1, seed=1)).to(DEV)
+    x = torch.randn(6, 10, 48, device=DEV)
+    net(x).square().mean().backward()
+    assert all(q.grad is not None and torch.isfinite(q.grad).all() and float(q.grad.abs().max()) > 0 for q in net.parameters())
+
+
+# ---- streams and graphs --------------------------------------------------------------------------------------------------
+def _step(t, p, rng):
+    h = rows.layer_norm(t, p["g"], p["b"])
+    h = rows.linear(h, p["w1"], p["b1"], act=nn.GELU())
+    h = rows.linear(h, p["w2"], p["b2"])
+    return rows.dropout(h, 0.2, rng, residual=t)
+
+
+def test_two_streams_at_once():
+    gen = torch.Generator().manual_seed(31)
+    p = {k: v.detach() for k, v in _mixer_params(256, 512, "bf16", gen).items()}
+    ts = [make((4096, 256), "bf16", gen) for _ in range(2)]
+    want = [_mixer(t, p) for t in ts]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = [None, None]
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = _mixer(ts[i], p)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_two_captured_graphs_replayed_in_turn():
+    # forward and backward in one capture (fresh leaves, autograd.grad); two graphs replayed back to back on two streams must not
+    # share scratch memory; the device counter moves between replays, so every replay draws another mask
+    gen = torch.Generator().manual_seed(32)
+    graphs = []
+    for i in range(2):
+        p = _mixer_params(64, 160, "bf16", gen)
+        t = make((300 + i, 64), "bf16", gen).requires_grad_()
+        dy = make((300 + i, 64), "bf16", gen)
+        rng = torch.tensor([5 + i, 0], dtype=torch.int64, device=DEV)
+        warm = torch.cuda.Stream()
+        warm.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(warm):
+            y = _step(t, p, rng)
+            torch.autograd.grad(y, [t] + list(p.values()), dy)
+            del y
+        torch.cuda.current_stream().wait_stream(warm)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = _step(t, p, rng)
+            outs = [y] + list(torch.autograd.grad(y, [t] + list(p.values()), dy))
+        graphs.append((graph, outs, t, p, dy, rng))
+    side = torch.cuda.Stream()
+    for it in range(4):
+        for graph, outs, t, p, dy, rng in graphs:
+            rng[1] = it
+            with torch.no_grad():
+                t.mul_(0.9).add_(0.01)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graphs[1][0].replay()
+        graphs[0][0].replay()
+        torch.cuda.synchronize()
+        for graph, outs, t, p, dy, rng in graphs:
+            q = {k: v.detach().requires_grad_() for k, v in p.items()}
+            tt = t.detach().clone().requires_grad_()
+            y = _step(tt, q, rng)
+            want = [y] + list(torch.autograd.grad(y, [tt] + list(q.values()), dy))
+            assert all(torch.equal(a, b) for a, b in zip(outs, want)), it
+
+
+def test_offsets_past_32_bits():
+    # 2^31 + elements in x and y: rows at the far end are computed from their own data
+    c, n = 512, (1 << 22) + 3000                                            # 2.15e9 elements, 4.3 GB in bf16
+    x = torch.empty((n, c), dtype=torch.bfloat16, device=DEV)
+    x[: n // 2] = 0
+    x[n // 2:] = 1
+    gen = torch.Generator().manual_seed(41)
+    tail = make((3000, c), "bf16", gen)
+    x[-3000:] = tail
+    w, b = make((8, c), "bf16", gen, c ** -0.5), make((c,), "bf16", gen)
+    assert torch.equal(rows.linear(x, w)[-3000:], rows.linear(tail, w))
+    y = rows.layer_norm(x, b, b)
+    assert torch.equal(y[-3000:], rows.layer_norm(tail, b, b))
+    del y
+    y = rows.dropout(x, 0.5, 3)
+    first = (n - 3000) * c
+    bits = []
+    for i in (first, first + 4 * 1000, n * c - 4):                           # blocks past 2^29 counters, elements past 2^31
+        m, blk = 0xFFFFFFFF, i // 4
+        cc, k0, k1 = [blk & m, blk >> 32, 0, 0], 3, 0
+        for _ in range(10):
+            a_, b_ = 0xD2511F53 * cc[0], 0xCD9E8D57 * cc[2]
+            cc = [(b_ >> 32) ^ cc[1] ^ k0, b_ & m, (a_ >> 32) ^ cc[3] ^ k1, a_ & m]
+            k0, k1 = (k0 + 0x9E3779B9) & m, (k1 + 0xBB67AE85) & m
+        bits.append((i, cc))
+    flat, src = y.view(-1), x.view(-1)
+    for i, cc in bits:
+        keep = torch.tensor([v >= 2 ** 31 for v in cc])
+        assert torch.equal(flat[i:i + 4].float().cpu(), torch.where(keep, 2 * src[i:i + 4].float().cpu(), torch.zeros(4)))
