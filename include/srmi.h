@@ -495,7 +495,7 @@ int srmi_adam_step(float* param, const float* grad, float* exp_avg, float* exp_a
  * given); rows need no alignment beyond their element, 16-byte aligned ones (pointer and stride) run wider accesses.
  * Outputs are dense.  Deterministic: no atomics, the same call gives the same bits.  These calls were added after version
  * 119 without changing anything that version declares; a caller that may meet an older library looks the symbols up. */
-#define SRMI_ROWS_MAX 0x7fffffffff /* rows per call */
+#define SRMI_ROWS_MAX 0xfffffffff /* rows per call */
 #define SRMI_PASS_FWD 0
 #define SRMI_PASS_BWD 1
 
@@ -505,13 +505,14 @@ typedef struct srmi_linear_desc {
     int32_t dtype;                 /* of every tensor of the call */
     int32_t act;                   /* NONE, LRELU, RELU, TANH, SIGMOID, GELU, GELU_TANH, SILU (PReLU: the convs' epilogue) */
     float act_param;               /* LeakyReLU slope */
-    int32_t reserved;              /* must be 0 */
+    int32_t align;                 /* 16: x, w and dy are multiples of 16 bytes, and those in bf16 whose row stride and width are
+                                      multiples of 8 are read in place.  0: element aligned, operands are laid out in ws */
     int64_t ldx, ldw, ldr, lddy;   /* row strides of x, w, residual, dy */
 } srmi_linear_desc;
 
 /* y = act(x w^T + bias) + residual:  x [M, K], w [N, K] (nn.Linear's layout), bias [N] or NULL, residual [M, N] or NULL,
  * y [M, N].  z (NULL, or dense [M, N]) also receives x w^T + bias, which the backward of a smooth activation needs.
- * K == 0 is a product of nothing: y = act(bias) + residual.
+ * K == 0 is a product of nothing: y = act(bias) + residual.  N, K <= 2^22.
  * ws: srmi_linear_workspace_bytes(d, pass) bytes, 256-byte aligned, written and read by this call alone. */
 int srmi_linear_workspace_bytes(const srmi_linear_desc* d, int32_t pass, size_t* bytes);
 int srmi_linear_fwd(const srmi_linear_desc* d, const void* x, const void* w, const void* bias, const void* residual, void* y, void* z,

@@ -8,6 +8,7 @@ int linear_fwd(const srmi_linear_desc& d, const void* x, const void* w, const vo
 int linear_bwd(const srmi_linear_desc& d, const void* x, const void* w, const void* saved, const void* dy, void* dx, void* dw, void* db,
                void* ws, hipStream_t s);
 size_t linear_workspace_bytes(const srmi_linear_desc& d, int pass);
+bool linear_too_wide(const srmi_linear_desc& d);
 int norm_fwd(const srmi_norm_desc& d, const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, hipStream_t s);
 int norm_bwd(const srmi_norm_desc& d, const void* x, const void* w, const float* mean, const float* rstd, const void* dy, void* dx,
              void* dw, void* db, float* ws, hipStream_t s);
@@ -18,8 +19,9 @@ int dropout(const void* x, const void* residual, void* y, long long n, double p,
 static bool is_dtype(int v) { return v == SRMI_F32 || v == SRMI_BF16; }
 static size_t dsize(int dtype) { return dtype == SRMI_BF16 ? 2 : 4; }
 
-// pointers are aligned to their element and to nothing more
+// pointers are aligned to their element; a linear call may promise 16 bytes for the products' operands
 static bool element_aligned(const void* p, int dtype) { return ((uintptr_t)p & (dsize(dtype) - 1)) == 0; }
+static bool linear_aligned(const srmi_linear_desc* d, const void* p) { return d->align >= 16 ? ((uintptr_t)p & 15) == 0 : element_aligned(p, d->dtype); }
 
 static int check_linear(const srmi_linear_desc* d, const char* who) {
     if (!d) { set_error("%s: NULL descriptor", who); return SRMI_EINVAL; }
@@ -28,6 +30,7 @@ static int check_linear(const srmi_linear_desc* d, const char* who) {
         return SRMI_EINVAL;
     }
     if (!is_dtype(d->dtype)) { set_error("%s: bad dtype %d", who, d->dtype); return SRMI_EINVAL; }
+    if (linear_too_wide(*d)) { set_error("%s: N=%d or K=%d over 2^22", who, d->N, d->K); return SRMI_EUNSUPPORTED; }
     switch (d->act) {
         case SRMI_ACT_NONE: case SRMI_ACT_LRELU: case SRMI_ACT_RELU: case SRMI_ACT_TANH: case SRMI_ACT_SIGMOID:
         case SRMI_ACT_GELU: case SRMI_ACT_GELU_TANH: case SRMI_ACT_SILU: break;
@@ -77,9 +80,9 @@ int srmi_linear_fwd(const srmi_linear_desc* d, const void* x, const void* w, con
     if (d->M == 0 || d->N == 0) return SRMI_OK;
     if (!y || (d->K > 0 && (!x || !w))) { set_error("linear_fwd: NULL argument"); return SRMI_EINVAL; }
     if (residual && d->ldr < d->N) { set_error("linear_fwd: residual without its row stride"); return SRMI_EINVAL; }
-    if (!element_aligned(x, d->dtype) || !element_aligned(w, d->dtype) || !element_aligned(bias, d->dtype) ||
+    if (!linear_aligned(d, x) || !linear_aligned(d, w) || !element_aligned(bias, d->dtype) ||
         !element_aligned(residual, d->dtype) || !element_aligned(y, d->dtype) || !element_aligned(z, d->dtype)) {
-        set_error("linear_fwd: an operand is not aligned to its element");
+        set_error("linear_fwd: an operand is not aligned to its element, or not as d->align says");
         return SRMI_EINVAL;
     }
     const size_t need = linear_workspace_bytes(*d, SRMI_PASS_FWD);
@@ -99,9 +102,9 @@ int srmi_linear_bwd(const srmi_linear_desc* d, const void* x, const void* w, con
         return SRMI_EINVAL;
     }
     if ((dw && d->M > 0 && d->K > 0 && !x) || (dx && d->N > 0 && d->K > 0 && !w)) { set_error("linear_bwd: NULL x or w"); return SRMI_EINVAL; }
-    if (!element_aligned(x, d->dtype) || !element_aligned(w, d->dtype) || !element_aligned(saved, d->dtype) || !element_aligned(dy, d->dtype) ||
+    if (!linear_aligned(d, x) || !linear_aligned(d, w) || !element_aligned(saved, d->dtype) || !linear_aligned(d, dy) ||
         !element_aligned(dx, d->dtype) || !element_aligned(dw, d->dtype) || !element_aligned(db, d->dtype)) {
-        set_error("linear_bwd: an operand is not aligned to its element");
+        set_error("linear_bwd: an operand is not aligned to its element, or not as d->align says");
         return SRMI_EINVAL;
     }
     const size_t need = linear_workspace_bytes(*d, SRMI_PASS_BWD);

@@ -12,7 +12,11 @@ template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) { return f2bf(v); }
 
-// V consecutive elements as f32.  The caller guarantees alignment to V elements.
+// V consecutive elements as f32, at any element's address: global memory takes unaligned 16-byte accesses on this target
+// (aligned ones are faster where rows allow them, nothing else changes).
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
 template <int V>
 __device__ __forceinline__ void load_vec(const float* p, float* o) {
     if constexpr (V == 1) {
@@ -20,7 +24,7 @@ __device__ __forceinline__ void load_vec(const float* p, float* o) {
     } else {
 #pragma unroll
         for (int i = 0; i < V; i += 4) {
-            const f32x4 q = *(const f32x4*)(p + i);
+            const f32x4 q = *(const f32x4_any*)(p + i);
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i + j] = q[j];
         }
@@ -31,7 +35,7 @@ __device__ __forceinline__ void load_vec(const bf16_t* p, float* o) {
     if constexpr (V == 1) {
         o[0] = bf2f(p[0]);
     } else if constexpr (V == 4) {
-        const u32x2 q = *(const u32x2*)p;
+        const u32x2 q = *(const u32x2_any*)p;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             o[2 * j] = __builtin_bit_cast(float, q[j] << 16);
@@ -40,7 +44,7 @@ __device__ __forceinline__ void load_vec(const bf16_t* p, float* o) {
     } else {
 #pragma unroll
         for (int i = 0; i < V; i += 8) {
-            const u32x4 q = *(const u32x4*)(p + i);
+            const u32x4 q = *(const u32x4_any*)(p + i);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 o[i + 2 * j] = __builtin_bit_cast(float, q[j] << 16);
@@ -55,7 +59,7 @@ __device__ __forceinline__ void store_vec(float* p, const float* v) {
         p[0] = v[0];
     } else {
 #pragma unroll
-        for (int i = 0; i < V; i += 4) *(f32x4*)(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+        for (int i = 0; i < V; i += 4) *(f32x4_any*)(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
     }
 }
 template <int V>
@@ -63,11 +67,11 @@ __device__ __forceinline__ void store_vec(bf16_t* p, const float* v) {
     if constexpr (V == 1) {
         p[0] = f2bf(v[0]);
     } else if constexpr (V == 4) {
-        *(u32x2*)p = u32x2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
+        *(u32x2_any*)p = u32x2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
     } else {
 #pragma unroll
         for (int i = 0; i < V; i += 8)
-            *(u32x4*)(p + i) = u32x4{pack_bf2(v[i], v[i + 1]), pack_bf2(v[i + 2], v[i + 3]), pack_bf2(v[i + 4], v[i + 5]),
+            *(u32x4_any*)(p + i) = u32x4{pack_bf2(v[i], v[i + 1]), pack_bf2(v[i + 2], v[i + 3]), pack_bf2(v[i + 4], v[i + 5]),
                                      pack_bf2(v[i + 6], v[i + 7])};
     }
 }
@@ -84,6 +88,16 @@ template <bool FAST> __device__ __forceinline__ float div_(float a, float b) {
 }
 template <bool FAST> __device__ __forceinline__ float logistic(float v) { return div_<FAST>(1.f, 1.f + exp_<FAST>(-v)); }
 
+// E = exp(-z^2 / 2) and q = Phi(-|z|) for bf16 results: q = E u P(u), u = 1 / (1 + 0.38 |z|), P of degree 4 fitted to
+// Phi(-t) exp(t^2 / 2) on t in [0, 14] for the least relative error, 3.5e-5 (the storage rounds by up to 3.9e-3); the same
+// relative error holds far out, where 1 + erf(z / sqrt 2) would cancel, at a third of an erf's instructions.
+__device__ __forceinline__ void normal_tail(float z, float& E, float& q) {
+    const float t = fminf(fabsf(z), 15.f);                 // q underflows beyond; keeps 0 * inf out
+    E = __builtin_amdgcn_exp2f(-0.72134752044448170f * t * t);
+    const float u = __builtin_amdgcn_rcpf(1.f + 0.38f * t);
+    q = E * u * (0.15122523f + u * (0.157829f + u * (0.09198039f + u * (0.18887625f - u * 0.0899284f))));
+}
+
 constexpr float GELU_2C = 1.5957691216057308f;      // 2 sqrt(2 / pi)
 constexpr float GELU_K = 0.044715f;
 
@@ -94,9 +108,23 @@ __device__ __forceinline__ float row_act(float z, int act, float param) {
     switch (act) {
         case SRMI_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
         case SRMI_ACT_LRELU: return z >= 0.f ? z : z * param;
-        case SRMI_ACT_TANH: return tanhf(z);
+        case SRMI_ACT_TANH:
+            if constexpr (FAST) {                              // (1 - e) / (1 + e) cancels near 0: three terms of the series there
+                const float t = fabsf(z), e = exp_<true>(-2.f * t), s = z * z;
+                const float far = (1.f - e) * __builtin_amdgcn_rcpf(1.f + e);
+                return t < 0.06f ? z * (1.f - s * (0.33333333f - s * 0.13333333f)) : copysignf(far, z);
+            } else {
+                return tanhf(z);
+            }
         case SRMI_ACT_SIGMOID: return logistic<FAST>(z);
-        case SRMI_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+        case SRMI_ACT_GELU:
+            if constexpr (FAST) {
+                float E, q;
+                normal_tail(z, E, q);
+                return (z < 0.f ? 0.f : z) - fminf(fabsf(z), 15.f) * q;
+            } else {
+                return 0.5f * z * erfcf(-0.70710678118654752f * z);
+            }
         case SRMI_ACT_GELU_TANH: return z * logistic<FAST>(GELU_2C * (z + GELU_K * z * z * z));
         case SRMI_ACT_SILU: return z * logistic<FAST>(z);
         default: return z;
@@ -118,7 +146,13 @@ __device__ __forceinline__ float row_act_slope(float z, int act, float param) {
             return div_<FAST>(e, d * d);
         }
         case SRMI_ACT_GELU:
-            return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.3989422804014327f * exp_<FAST>(-0.5f * z * z);
+            if constexpr (FAST) {
+                float E, q;
+                normal_tail(z, E, q);
+                return (z < 0.f ? q : 1.f - q) + z * 0.3989422804014327f * E;
+            } else {
+                return 0.5f * erfcf(-0.70710678118654752f * z) + z * 0.3989422804014327f * expf(-0.5f * z * z);
+            }
         case SRMI_ACT_GELU_TANH: {
             const float s = logistic<FAST>(GELU_2C * (z + GELU_K * z * z * z));
             return s + z * s * (1.f - s) * GELU_2C * (1.f + 3.f * GELU_K * z * z);

@@ -33,16 +33,17 @@ __device__ __forceinline__ void philox4(unsigned long long ctr, unsigned long lo
     o[0] = c0; o[1] = c1; o[2] = c2; o[3] = c3;
 }
 
-// V elements per lane and step (4 or 8, whole Philox blocks); VEC: 16-byte accesses where the step is whole
-template <typename T, int V, bool VEC>
+// 16 bytes per lane and step: 4 or 8 elements, whole Philox blocks
+template <typename T>
 __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
+    constexpr int V = 16 / (int)sizeof(T);
     const unsigned long long seed = a.rng ? a.rng[0] : a.seed, offset = a.rng ? a.rng[1] : a.offset;
     const T* x = (const T*)a.x;
     const T* res = (const T*)a.residual;
     T* y = (T*)a.y;
     for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * V; i < a.n; i += (long long)gridDim.x * 256 * V) {
         float v[V], r[V];
-        const bool whole = VEC && i + V <= a.n;
+        const bool whole = i + V <= a.n;
         if (whole) {
             load_vec<V>(x + i, v);
             if (res) load_vec<V>(res + i, r);
@@ -76,11 +77,9 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
 template <typename T>
 static void dropout_go(const DropArgs& a, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T);
-    const bool vec = (((uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.y) & 15) == 0;
     long long grid = (a.n + 256 * V - 1) / (256 * V);
     if (grid > 8192) grid = 8192;
-    if (vec) hipLaunchKernelGGL((dropout_kernel<T, V, true>), dim3((unsigned)grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((dropout_kernel<T, V, false>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((dropout_kernel<T>), dim3((unsigned)grid), dim3(256), 0, s, a);
 }
 
 int dropout(const void* x, const void* residual, void* y, long long n, double p, unsigned long long seed, unsigned long long offset,

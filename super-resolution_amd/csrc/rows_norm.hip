@@ -32,14 +32,33 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
-template <int V>
-__device__ __forceinline__ void load_param(const void* p, int p_bf16, int c, float* o) {
-    if (p_bf16) load_vec<V>((const bf16_t*)p + c, o);
-    else load_vec<V>((const float*)p + c, o);
+// V columns from c on; TAIL: those past C read as `fill` (rows need no alignment: rows_common.h)
+template <int V, bool TAIL, typename T>
+__device__ __forceinline__ void load_cols(const T* p, int c, int C, float fill, float* o) {
+    if (!TAIL || c + V <= C) load_vec<V>(p + c, o);
+    else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = c + j < C ? to_f32(p[c + j]) : fill;
+    }
+}
+template <int V, bool TAIL, typename T>
+__device__ __forceinline__ void store_cols(T* p, int c, int C, const float* o) {
+    if (!TAIL || c + V <= C) store_vec<V>(p + c, o);
+    else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (c + j < C) p[c + j] = from_f32<T>(o[j]);
+    }
+}
+template <int V, bool TAIL>
+__device__ __forceinline__ void load_param(const void* p, int p_bf16, int c, int C, float* o) {
+    if (p_bf16) load_cols<V, TAIL>((const bf16_t*)p, c, C, 0.f, o);
+    else load_cols<V, TAIL>((const float*)p, c, C, 0.f, o);
 }
 
-template <typename T, int LANES, int V, int ITER>
+template <typename T, int LANES, int ITER, bool TAIL>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
+    constexpr int V = 16 / (int)sizeof(T);
     const int l = threadIdx.x % LANES;
     const long long ngroups = (long long)gridDim.x * (256 / LANES);
     float w[ITER * V], b[ITER * V];
@@ -49,8 +68,8 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
 #pragma unroll
         for (int j = 0; j < V; ++j) { w[i * V + j] = 1.f; b[i * V + j] = 0.f; }
         if (c < a.C) {
-            if (a.w) load_param<V>(a.w, a.p_bf16, c, w + i * V);
-            if (a.b) load_param<V>(a.b, a.p_bf16, c, b + i * V);
+            if (a.w) load_param<V, TAIL>(a.w, a.p_bf16, c, a.C, w + i * V);
+            if (a.b) load_param<V, TAIL>(a.b, a.p_bf16, c, a.C, b + i * V);
         }
     }
     const float inv = 1.f / (float)a.C;
@@ -60,7 +79,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int c = (i * LANES + l) * V;
-            if (c < a.C) load_vec<V>(x + c, v + i * V);
+            if (c < a.C) load_cols<V, TAIL>(x, c, a.C, 0.f, v + i * V);
             else {
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[i * V + j] = 0.f;
@@ -74,7 +93,10 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
         for (int i = 0; i < ITER; ++i) {
             if ((i * LANES + l) * V < a.C) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) { v[i * V + j] -= mean; q += v[i * V + j] * v[i * V + j]; }
+                for (int j = 0; j < V; ++j) {
+                    v[i * V + j] -= mean;
+                    if (!TAIL || (i * LANES + l) * V + j < a.C) q += v[i * V + j] * v[i * V + j];
+                }
             }
         }
         const float rstd = 1.f / sqrtf(group_sum<LANES>(q) * inv + a.eps);
@@ -86,15 +108,16 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
                 float o[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) o[j] = v[i * V + j] * rstd * w[i * V + j] + b[i * V + j];
-                store_vec<V>(y + c, o);
+                store_cols<V, TAIL>(y, c, a.C, o);
             }
         }
         if (a.mean && l == 0) { a.mean[r] = mean; a.rstd[r] = rstd; }
     }
 }
 
-template <typename T, int LANES, int V, int ITER>
+template <typename T, int LANES, int ITER, bool TAIL>
 __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
+    constexpr int V = 16 / (int)sizeof(T);
     constexpr int G = 256 / LANES;
     __shared__ float red[G > 1 ? G : 1][LANES * V];
     const int l = threadIdx.x % LANES, gr = threadIdx.x / LANES;
@@ -105,7 +128,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
         const int c = (i * LANES + l) * V;
 #pragma unroll
         for (int j = 0; j < V; ++j) { w[i * V + j] = 1.f; dw[i * V + j] = 0.f; db[i * V + j] = 0.f; }
-        if (c < a.C && a.w) load_param<V>(a.w, a.p_bf16, c, w + i * V);
+        if (c < a.C && a.w) load_param<V, TAIL>(a.w, a.p_bf16, c, a.C, w + i * V);
     }
     const float inv = 1.f / (float)a.C;
     for (long long r = (long long)blockIdx.x * G + gr; r < a.rows; r += ngroups) {
@@ -117,8 +140,8 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
         for (int i = 0; i < ITER; ++i) {
             const int c = (i * LANES + l) * V;
             if (c < a.C) {
-                load_vec<V>(x + c, xh + i * V);
-                load_vec<V>(dy + c, g + i * V);
+                load_cols<V, TAIL>(x, c, a.C, 0.f, xh + i * V);
+                load_cols<V, TAIL>(dy, c, a.C, 0.f, g + i * V);         // 0 past the end: adds nothing below
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const int k = i * V + j;
@@ -141,7 +164,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
                     float o[V];
 #pragma unroll
                     for (int j = 0; j < V; ++j) o[j] = rstd * (g[i * V + j] - c1 - xh[i * V + j] * c2);
-                    store_vec<V>(dx + c, o);
+                    store_cols<V, TAIL>(dx, c, a.C, o);
                 }
             }
         }
@@ -178,8 +201,9 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
     return red[0] + red[1] + red[2] + red[3];
 }
 
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
+    constexpr int V = 16 / (int)sizeof(T);
     __shared__ float red[4];
     const float inv = 1.f / (float)a.C;
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -188,7 +212,7 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
         float s = 0.f;
         for (int c = threadIdx.x * V; c < a.C; c += 256 * V) {
             float v[V];
-            load_vec<V>(x + c, v);
+            load_cols<V, true>(x, c, a.C, 0.f, v);
 #pragma unroll
             for (int j = 0; j < V; ++j) s += v[j];
         }
@@ -196,28 +220,30 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
         float q = 0.f;
         for (int c = threadIdx.x * V; c < a.C; c += 256 * V) {
             float v[V];
-            load_vec<V>(x + c, v);
+            load_cols<V, true>(x, c, a.C, 0.f, v);
 #pragma unroll
-            for (int j = 0; j < V; ++j) { v[j] -= mean; q += v[j] * v[j]; }
+            for (int j = 0; j < V; ++j)
+                if (c + j < a.C) { v[j] -= mean; q += v[j] * v[j]; }
         }
         const float rstd = 1.f / sqrtf(block_sum(q, red) * inv + a.eps);
         for (int c = threadIdx.x * V; c < a.C; c += 256 * V) {
             float v[V], w[V], b[V];
-            load_vec<V>(x + c, v);
+            load_cols<V, true>(x, c, a.C, 0.f, v);
 #pragma unroll
             for (int j = 0; j < V; ++j) { w[j] = 1.f; b[j] = 0.f; }
-            if (a.w) load_param<V>(a.w, a.p_bf16, c, w);
-            if (a.b) load_param<V>(a.b, a.p_bf16, c, b);
+            if (a.w) load_param<V, true>(a.w, a.p_bf16, c, a.C, w);
+            if (a.b) load_param<V, true>(a.b, a.p_bf16, c, a.C, b);
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = (v[j] - mean) * rstd * w[j] + b[j];
-            store_vec<V>(y + c, v);
+            store_cols<V, true>(y, c, a.C, v);
         }
         if (a.mean && threadIdx.x == 0) { a.mean[r] = mean; a.rstd[r] = rstd; }
     }
 }
 
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
+    constexpr int V = 16 / (int)sizeof(T);
     __shared__ float red[4];
     const float inv = 1.f / (float)a.C;
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -231,11 +257,11 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
             if (pass) { c1 = block_sum(s1, red) * inv; c2 = block_sum(s2, red) * inv; }
             for (int c = threadIdx.x * V; c < a.C; c += 256 * V) {
                 float xh[V], g[V], w[V];
-                load_vec<V>(x + c, xh);
-                load_vec<V>(dy + c, g);
+                load_cols<V, true>(x, c, a.C, 0.f, xh);
+                load_cols<V, true>(dy, c, a.C, 0.f, g);
 #pragma unroll
                 for (int j = 0; j < V; ++j) w[j] = 1.f;
-                if (a.w) load_param<V>(a.w, a.p_bf16, c, w);
+                if (a.w) load_param<V, true>(a.w, a.p_bf16, c, a.C, w);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     xh[j] = (xh[j] - mean) * rstd;
@@ -243,15 +269,16 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
                     if (!pass) { s1 += g[j]; s2 += g[j] * xh[j]; }
                     else g[j] = rstd * (g[j] - c1 - xh[j] * c2);
                 }
-                if (pass) store_vec<V>(dx + c, g);
+                if (pass) store_cols<V, true>(dx, c, a.C, g);
             }
         }
     }
 }
 
 // dw / db of wide rows: workgroup (strip of 256 V columns, slot of rows); a lane owns V columns of the strip
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(256) void norm_wide_dw_kernel(NormArgs a) {
+    constexpr int V = 16 / (int)sizeof(T);
     const int c = ((int)blockIdx.y * 256 + threadIdx.x) * V;
     if (c >= a.C) return;
     float dw[V], db[V];
@@ -259,16 +286,15 @@ __global__ __launch_bounds__(256) void norm_wide_dw_kernel(NormArgs a) {
     for (int j = 0; j < V; ++j) dw[j] = db[j] = 0.f;
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         float x[V], dy[V];
-        load_vec<V>((const T*)a.x + r * a.ldx + c, x);
-        load_vec<V>((const T*)a.dy + r * a.lddy + c, dy);
+        load_cols<V, true>((const T*)a.x + r * a.ldx, c, a.C, 0.f, x);
+        load_cols<V, true>((const T*)a.dy + r * a.lddy, c, a.C, 0.f, dy);
         const float mean = a.mean[r], rstd = a.rstd[r];
 #pragma unroll
         for (int j = 0; j < V; ++j) { dw[j] += dy[j] * ((x[j] - mean) * rstd); db[j] += dy[j]; }
     }
     float* slot = a.part + (size_t)blockIdx.x * 2 * a.C;
-    store_vec<V>(slot + c, dw);
-    if constexpr (V == 1) slot[a.C + c] = db[0];
-    else store_vec<V>(slot + a.C + c, db);
+    store_cols<V, true>(slot, c, a.C, dw);
+    store_cols<V, true>(slot + a.C, c, a.C, db);
 }
 
 // out[c] = sum over slots of part[slot][c], n columns; 32 columns x 8 slot lanes per workgroup, slots added in index order
@@ -302,73 +328,57 @@ int slot_sum_launch(const float* part, int slots, int n, int n0, void* o0, void*
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-// 16-byte accesses need every row of every operand on a 16-byte boundary and whole vectors per row
-static bool norm_aligned(const NormArgs& a, int esz) {
-    const int v = 16 / esz;
-    uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.dy | (uintptr_t)a.w | (uintptr_t)a.b | (uintptr_t)a.part;
-    return (bits & 15) == 0 && a.C % v == 0 && a.ldx % v == 0 && a.lddy % v == 0;
-}
+static constexpr int NORM_WIDE = 2048;      // widest row kept in registers: 32 values a lane; the re-reading kernels take what is wider
 
-static constexpr int NORM_WIDE_V = 2048, NORM_WIDE_1 = 1024;      // widest row of the register kernels: vector / scalar accesses
-
-int norm_slots(long long rows, int C) {
-    (void)C;
+// partial rows of dw / db: enough workgroups to fill the chip, each with several rows
+int norm_slots(long long rows) {
     const long long want = (rows + 7) / 8;
     return (int)(want < 1 ? 1 : want > 512 ? 512 : want);
 }
 
-template <bool BWD, typename T, int LANES, int V, int ITER>
+template <bool BWD, typename T, int LANES, int ITER, bool TAIL>
 static void norm_go(const NormArgs& a, int slots, hipStream_t s) {
     const long long rpb = 256 / LANES;
     long long grid = (a.rows + rpb - 1) / rpb;
     if constexpr (BWD) {
         if (a.part || grid > slots) grid = slots;
-        hipLaunchKernelGGL((norm_bwd_kernel<T, LANES, V, ITER>), dim3((unsigned)grid), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((norm_bwd_kernel<T, LANES, ITER, TAIL>), dim3((unsigned)grid), dim3(256), 0, s, a);
     } else {
         if (grid > 2048) grid = 2048;
-        hipLaunchKernelGGL((norm_fwd_kernel<T, LANES, V, ITER>), dim3((unsigned)grid), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((norm_fwd_kernel<T, LANES, ITER, TAIL>), dim3((unsigned)grid), dim3(256), 0, s, a);
     }
 }
 
-template <bool BWD, typename T>
-static void norm_dispatch(const NormArgs& a, bool vec, int slots, hipStream_t s) {
-    const int C = a.C;
+template <bool BWD, typename T, bool TAIL>
+static void norm_rows(const NormArgs& a, int slots, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T);
-    if (vec) {
-        if (C <= 8 * V) norm_go<BWD, T, 8, V, 1>(a, slots, s);
-        else if (C <= 16 * V) norm_go<BWD, T, 16, V, 1>(a, slots, s);
-        else if (C <= 32 * V) norm_go<BWD, T, 32, V, 1>(a, slots, s);
-        else if (C <= 64 * V) norm_go<BWD, T, 64, V, 1>(a, slots, s);
-        else if (C <= 128 * V) norm_go<BWD, T, 64, V, 2>(a, slots, s);
-        else if (C <= 256 * V) norm_go<BWD, T, 64, V, 4>(a, slots, s);
-        else if constexpr (V == 4) norm_go<BWD, T, 64, V, 8>(a, slots, s);
-    } else {
-        if (C <= 16) norm_go<BWD, T, 16, 1, 1>(a, slots, s);
-        else if (C <= 64) norm_go<BWD, T, 64, 1, 1>(a, slots, s);
-        else if (C <= 128) norm_go<BWD, T, 64, 1, 2>(a, slots, s);
-        else if (C <= 256) norm_go<BWD, T, 64, 1, 4>(a, slots, s);
-        else if (C <= 512) norm_go<BWD, T, 64, 1, 8>(a, slots, s);
-        else norm_go<BWD, T, 64, 1, 16>(a, slots, s);
-    }
+    const int C = a.C;
+    if (C <= 8 * V) norm_go<BWD, T, 8, 1, TAIL>(a, slots, s);
+    else if (C <= 16 * V) norm_go<BWD, T, 16, 1, TAIL>(a, slots, s);
+    else if (C <= 32 * V) norm_go<BWD, T, 32, 1, TAIL>(a, slots, s);
+    else if (C <= 64 * V) norm_go<BWD, T, 64, 1, TAIL>(a, slots, s);
+    else if (C <= 128 * V) norm_go<BWD, T, 64, 2, TAIL>(a, slots, s);
+    else if (C <= 256 * V) norm_go<BWD, T, 64, 4, TAIL>(a, slots, s);
+    else if constexpr (V == 4) norm_go<BWD, T, 64, 8, TAIL>(a, slots, s);
 }
 
 template <bool BWD, typename T>
-static void norm_wide(const NormArgs& a, bool vec, int slots, hipStream_t s) {
+static void norm_wide(const NormArgs& a, int slots, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T);
     const unsigned grid = (unsigned)(a.rows > 4096 ? 4096 : a.rows);
     if constexpr (BWD) {
-        if (a.y) {
-            if (vec) hipLaunchKernelGGL((norm_wide_dx_kernel<T, V>), dim3(grid), dim3(256), 0, s, a);
-            else hipLaunchKernelGGL((norm_wide_dx_kernel<T, 1>), dim3(grid), dim3(256), 0, s, a);
-        }
-        if (a.part) {
-            if (vec) hipLaunchKernelGGL((norm_wide_dw_kernel<T, V>), dim3(slots, (a.C + 256 * V - 1) / (256 * V)), dim3(256), 0, s, a);
-            else hipLaunchKernelGGL((norm_wide_dw_kernel<T, 1>), dim3(slots, (a.C + 255) / 256), dim3(256), 0, s, a);
-        }
+        if (a.y && grid) hipLaunchKernelGGL((norm_wide_dx_kernel<T>), dim3(grid), dim3(256), 0, s, a);
+        if (a.part) hipLaunchKernelGGL((norm_wide_dw_kernel<T>), dim3(slots, (a.C + 256 * V - 1) / (256 * V)), dim3(256), 0, s, a);
     } else {
-        if (vec) hipLaunchKernelGGL((norm_wide_fwd_kernel<T, V>), dim3(grid), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((norm_wide_fwd_kernel<T, 1>), dim3(grid), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((norm_wide_fwd_kernel<T>), dim3(grid), dim3(256), 0, s, a);
     }
+}
+
+template <bool BWD, typename T>
+static void norm_dispatch(const NormArgs& a, int slots, hipStream_t s) {
+    if (a.C > NORM_WIDE) norm_wide<BWD, T>(a, slots, s);
+    else if (a.C % (16 / (int)sizeof(T))) norm_rows<BWD, T, true>(a, slots, s);
+    else norm_rows<BWD, T, false>(a, slots, s);
 }
 
 static void fill_args(NormArgs* a, const srmi_norm_desc& d, const void* x, const void* w, const void* b) {
@@ -380,14 +390,12 @@ int norm_fwd(const srmi_norm_desc& d, const void* x, const void* w, const void* 
     NormArgs a;
     fill_args(&a, d, x, w, b);
     a.y = y; a.mean = mean; a.rstd = rstd;
-    const bool vec = norm_aligned(a, d.dtype == SRMI_BF16 ? 2 : 4);
-    const bool wide = d.C > (vec ? NORM_WIDE_V : NORM_WIDE_1);
-    if (d.dtype == SRMI_BF16) { if (wide) norm_wide<false, bf16_t>(a, vec, 0, s); else norm_dispatch<false, bf16_t>(a, vec, 0, s); }
-    else { if (wide) norm_wide<false, float>(a, vec, 0, s); else norm_dispatch<false, float>(a, vec, 0, s); }
+    if (d.dtype == SRMI_BF16) norm_dispatch<false, bf16_t>(a, 0, s);
+    else norm_dispatch<false, float>(a, 0, s);
     return hip_check(hipGetLastError(), "layer_norm_fwd");
 }
 
-size_t norm_workspace_bytes(const srmi_norm_desc& d) { return (size_t)norm_slots(d.rows, d.C) * 2 * d.C * sizeof(float); }
+size_t norm_workspace_bytes(const srmi_norm_desc& d) { return (size_t)norm_slots(d.rows) * 2 * d.C * sizeof(float); }
 
 int norm_bwd(const srmi_norm_desc& d, const void* x, const void* w, const float* mean, const float* rstd, const void* dy, void* dx,
              void* dw, void* db, float* ws, hipStream_t s) {
@@ -395,11 +403,9 @@ int norm_bwd(const srmi_norm_desc& d, const void* x, const void* w, const float*
     fill_args(&a, d, x, w, nullptr);
     a.y = dx; a.mean = (float*)mean; a.rstd = (float*)rstd; a.dy = dy; a.lddy = d.lddy;
     a.part = dw || db ? ws : nullptr;
-    const int slots = norm_slots(d.rows, d.C);
-    const bool vec = norm_aligned(a, d.dtype == SRMI_BF16 ? 2 : 4);
-    const bool wide = d.C > (vec ? NORM_WIDE_V : NORM_WIDE_1);
-    if (d.dtype == SRMI_BF16) { if (wide) norm_wide<true, bf16_t>(a, vec, slots, s); else norm_dispatch<true, bf16_t>(a, vec, slots, s); }
-    else { if (wide) norm_wide<true, float>(a, vec, slots, s); else norm_dispatch<true, float>(a, vec, slots, s); }
+    const int slots = norm_slots(d.rows);
+    if (d.dtype == SRMI_BF16) norm_dispatch<true, bf16_t>(a, slots, s);
+    else norm_dispatch<true, float>(a, slots, s);
     const int rc = hip_check(hipGetLastError(), "layer_norm_bwd");
     if (rc || !a.part) return rc;
     return slot_sum_launch(ws, slots, 2 * d.C, d.C, dw, db, d.param_dtype == SRMI_BF16, s);

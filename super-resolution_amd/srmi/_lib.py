@@ -18,7 +18,7 @@ COMPUTE_F32, COMPUTE_BF16 = 0, 1
 ACT_NONE, ACT_PRELU, ACT_LRELU, ACT_RELU, ACT_TANH, ACT_SIGMOID, ACT_ADD_RELU = 0, 1, 2, 3, 4, 5, 6
 ACT_GELU, ACT_GELU_TANH, ACT_SILU = 7, 8, 9        # row operators only
 PASS_FWD, PASS_BWD = 0, 1
-ROWS_MAX = 0x7fffffffff
+ROWS_MAX = 0xfffffffff
 SHUFFLE_CRD, SHUFFLE_DCR = 0, 1
 
 
@@ -85,7 +85,7 @@ class CropItem(C.Structure):
 class LinearDesc(C.Structure):
     _fields_ = [
         ("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32),
-        ("dtype", C.c_int32), ("act", C.c_int32), ("act_param", C.c_float), ("reserved", C.c_int32),
+        ("dtype", C.c_int32), ("act", C.c_int32), ("act_param", C.c_float), ("align", C.c_int32),
         ("ldx", C.c_int64), ("ldw", C.c_int64), ("ldr", C.c_int64), ("lddy", C.c_int64),
     ]
 

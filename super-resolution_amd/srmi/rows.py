@@ -105,8 +105,7 @@ def _linear_desc(*key):
     """(descriptor, forward / backward workspace bytes) of one shape, kept: building them costs more than a small launch"""
     hit = _DESCS.get(key)
     if hit is None:
-        M, N, K, dtype, act, param, ldx, ldw, ldr, lddy = key
-        d = L.LinearDesc(M, N, K, dtype, act, param, 0, ldx, ldw, ldr, lddy)
+        d = L.LinearDesc(*key)
         sizes = []
         for which in (L.PASS_FWD, L.PASS_BWD):
             n = C.c_size_t(0)
@@ -116,6 +115,15 @@ def _linear_desc(*key):
             _DESCS.clear()
         hit = _DESCS[key] = (d, C.byref(d), sizes[0], sizes[1])
     return hit
+
+
+def _align(*tensors):
+    """what the library may assume of the pointers: 16 bytes, or just their element"""
+    bits = 0
+    for t in tensors:
+        if t is not None:
+            bits |= t.data_ptr()
+    return 0 if bits & 15 else 16
 
 
 def _workspace(nbytes, device):
@@ -134,7 +142,7 @@ def _linear_fwd(x, weight, bias, residual, act, param, want_z):
     if M and N:
         b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
         with _on(x.device):
-            _, ref, ws_fwd, _ = _linear_desc(M, N, K, Fn.dtype_code(x.dtype), act, param, ldx, ldw, ldr, 0)
+            _, ref, ws_fwd, _ = _linear_desc(M, N, K, Fn.dtype_code(x.dtype), act, param, _align(xr, wr), ldx, ldw, ldr, 0)
             ws = _workspace(ws_fwd, x.device)
             L.check(L.load().srmi_linear_fwd(ref, xr.data_ptr(), wr.data_ptr(), _ptr(b), _ptr(rr), y.data_ptr(), _ptr(z), _ptr(ws),
                                              ws_fwd, Fn.stream_ptr(x.device)))
@@ -173,7 +181,7 @@ class _LinearFn(torch.autograd.Function):
             if need[2] and has_bias:
                 db = torch.empty((N,), dtype=dt, device=dev)
             with _on(dev):
-                _, ref, _, ws_bwd = _linear_desc(M, N, K, Fn.dtype_code(dt), act, param, ldx, ldw, 0, lddy)
+                _, ref, _, ws_bwd = _linear_desc(M, N, K, Fn.dtype_code(dt), act, param, _align(x, w, dyr), ldx, ldw, 0, lddy)
                 ws = _workspace(ws_bwd, dev)
                 L.check(L.load().srmi_linear_bwd(ref, _ptr(x), _ptr(w), _ptr(saved), dyr.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
                                                  ws_bwd, Fn.stream_ptr(dev)))
