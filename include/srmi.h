@@ -505,8 +505,8 @@ typedef struct srmi_linear_desc {
     int32_t dtype;                 /* of every tensor of the call */
     int32_t act;                   /* NONE, LRELU, RELU, TANH, SIGMOID, GELU, GELU_TANH, SILU (PReLU: the convs' epilogue) */
     float act_param;               /* LeakyReLU slope */
-    int32_t align;                 /* 16: x, w and dy are multiples of 16 bytes, and those in bf16 whose row stride and width are
-                                      multiples of 8 are read in place.  0: element aligned, operands are laid out in ws */
+    int32_t align;                 /* 16: x, w and dy are multiples of 16 bytes, which lets bf16 products whose row strides and widths
+                                      are multiples of 8 take the faster loads.  0: aligned to their element */
     int64_t ldx, ldw, ldr, lddy;   /* row strides of x, w, residual, dy */
 } srmi_linear_desc;
 

@@ -13,9 +13,11 @@
 // The DMA writes LDS linearly, so the permutation is applied to the global address of each lane.
 // Rows and k past the operand's end are lanes whose buffer offset is out of range: the hardware returns zeros.
 //
-// f32 operands arrive as three bf16 planes (x = hi + mid + lo exactly, to 24 bits); the six products hi hi, hi mid, mid hi, hi lo,
-// mid mid, lo hi are six passes over K with the plane pointers exchanged, smallest first, which leaves the rounding of an
-// f32 sum over K (the dropped products are below 2^-24 of the largest).
+// Operands this kernel cannot take - f32, or bf16 rows off 16-byte boundaries - go through gemm_staged_kernel: the same tiles and fragments,
+// loaded through registers at any alignment.  f32 values are split there into three bf16 (x = hi + mid + lo to 24 bits) and
+// multiplied as six products hi hi, hi mid, mid hi, hi lo, mid mid, lo hi: the matrix cores run bf16 sixteen times as fast as f32, the
+// dropped products are below 2^-22 of the largest and of either sign.  hi hi has an accumulator of its own, so that a sum over K is
+// rounded once per 32 k as an f32 sum would be, not six times.
 #pragma once
 #include "rows_common.h"
 
@@ -31,11 +33,9 @@ constexpr unsigned OUT_OF_RANGE = 0x80000000u;       // buffer offset = the reso
 constexpr long long GEMM_MAX_LD = 1 << 22;           // a tile's offsets stay below 2^31 bytes
 
 struct TileArgs {
-    const bf16_t* a; const bf16_t* b;
-    long long lda, ldb;                              // row strides in elements, multiples of 8
-    long long pa, pb;                                // distance of the planes (f32)
+    const void* a; const void* b;                    // rows operand [M, K] and column operand [N, K], stored along or across k
+    long long lda, ldb;                              // row strides in elements
     long long M, K; int N;
-    int terms;                                       // 1, or 6 for f32 planes
     int tiles_m, tiles_n, splits;
     float* part; int part_ld;                        // split sums: [splits][M][part_ld]
     // epilogue
@@ -153,10 +153,8 @@ struct TileLoader {
             }
         }
     }
-    // address of step `step` (64 k each) in the plane at element offset `plane`, and the distance to the next step
-    __device__ __forceinline__ unsigned long long at(long long step, long long plane) const {
-        return (unsigned long long)(uintptr_t)base + 2 * (plane + step * GK * (T ? ld : 1));
-    }
+    // address of step `step` (64 k each), and the distance to the next step
+    __device__ __forceinline__ unsigned long long at(long long step) const { return (unsigned long long)(uintptr_t)base + 2 * step * GK * (T ? ld : 1); }
     __device__ __forceinline__ unsigned long long stride() const { return 2 * GK * (unsigned long long)(T ? ld : 1); }
     // request the wave's i-th KiB; klim: k of the step that exist, lds: byte address of the tile
     __device__ __forceinline__ void issue(int i, const u32x4& rsrc, int klim, unsigned lds, int wave) const {
@@ -208,14 +206,68 @@ __device__ __forceinline__ void tile_of_block(const TileArgs& p, int& tm, int& t
     tn = in / rows;
 }
 
+constexpr int ER = 32;                                // rows of a wave's tile per epilogue pass
+constexpr int epilogue_bytes(int waves, int wtn) { return waves * ER * (wtn + 4) * 4; }
+
+// The wave's accumulators (tile at row m0, column n0): split sums as they are, or the finished output
+template <int WTM, int WTN, typename T, bool PART>
+__device__ __forceinline__ void tile_store(const TileArgs& p, const f32x4 (&acc)[WTM / 16][WTN / 16], unsigned char* lds, int split, int wave,
+                                           int lane, long long m0, int n0) {
+    constexpr int MT = WTM / 16, NT = WTN / 16, EP = WTN + 4;
+    // a lane holds columns 4 q .. 4 q + 3 (q = lane / 16) of row lane % 16 of every 16 x 16 tile
+    const int r = lane & 15, q = lane >> 4;
+    if constexpr (PART) {
+        float* part = p.part + (size_t)split * p.M * p.part_ld;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const long long m = m0 + 16 * i + r;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int n = n0 + 16 * j + 4 * q;
+                if (m < p.M && n < p.part_ld) *(f32x4*)(part + m * p.part_ld + n) = acc[i][j];
+            }
+        }
+    } else {
+        // through LDS, 32 rows of the wave at a time, to whole rows: each lane then has 8 columns of one row, and 8 neighbouring
+        // lanes of a 64-column wave tile write whole 128-byte lines
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        float* st = (float*)lds + wave * (ER * EP);
+        constexpr int LPR = WTN / 8, RPI = 64 / LPR;          // lanes per row, rows per step
+        const int c = (lane % LPR) * 8, n = n0 + c;
+        float bias[8];
+        load_bias<T, 8>(p, n, bias);
+#pragma unroll 1
+        for (int pass = 0; pass < WTM / ER; ++pass) {
+#pragma unroll
+            for (int w = 0; w < WTM / ER; ++w) {
+                if (w != pass) continue;
+#pragma unroll
+                for (int i = 0; i < ER / 16; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) *(f32x4*)(st + (16 * i + r) * EP + 16 * j + 4 * q) = acc[w * (ER / 16) + i][j];
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1
+            for (int it = 0; it < ER / RPI; ++it) {
+                const int row = it * RPI + lane / LPR;
+                const long long m = m0 + pass * ER + row;
+                float v[8];
+                const f32x4 v0 = *(const f32x4*)(st + row * EP + c), v1 = *(const f32x4*)(st + row * EP + c + 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { v[j] = v0[j]; v[4 + j] = v1[j]; }
+                if (m < p.M && n < p.N) row_epilogue<T, 8>(p, v, bias, m, n);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    }
+}
+
 template <int BM, int BN, int WM, int WN, bool AT, bool BT, int NSTAGE, bool PIPE, typename T, bool PART>
 __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(TileArgs p) {
     constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, MT = WTM / 16, NT = WTN / 16;
     constexpr int STAGE = (BM + BN) * GK * 2;
     constexpr int U = (BM + BN) / 8 / NW;                     // DMA instructions per wave and step
-    constexpr int ER = 32;                                    // rows per epilogue pass
-    constexpr int EP = WTN + 4;                               // floats per staged row
-    static_assert(NW * ER * EP * 4 <= NSTAGE * STAGE, "the epilogue reuses the operand stages");
+    static_assert(epilogue_bytes(NW, WTN) <= NSTAGE * STAGE, "the epilogue reuses the operand stages");
     extern __shared__ __align__(1024) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int tm, tn, split;
@@ -226,45 +278,30 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(TileArgs p) {
 
     TileLoader<BM, NW, AT> la;
     TileLoader<BN, NW, BT> lb;
-    la.init(p.a, p.lda, m0, p.M, wave, lane);
-    lb.init(p.b, p.ldb, n0, p.N, wave, lane);
+    la.init((const bf16_t*)p.a, p.lda, m0, p.M, wave, lane);
+    lb.init((const bf16_t*)p.b, p.ldb, n0, p.N, wave, lane);
     TileReader<BM, MT, AT> ra;
     TileReader<BN, NT, BT> rb;
     ra.init(wm, lane);
     rb.init(wn, lane);
 
-    const int ksteps = (int)((p.K + GK - 1) / GK);
-    const long long total = (long long)p.terms * ksteps;
-    const long long s_begin = total * split / p.splits, s_end = total * (split + 1) / p.splits;
+    const int ksteps = (int)((p.K + GK - 1) / GK), klast = (int)(p.K - (long long)(ksteps - 1) * GK);
+    int kstep = (int)((long long)ksteps * split / p.splits);                    // the next step to request
+    const int nsteps = (int)((long long)ksteps * (split + 1) / p.splits) - kstep, kend = kstep + nsteps;
     const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr)lds;
-
-    // the next step to request: its place in the pass over k (f32: which pass over the planes, 5 = hi hi), and what its requests need
-    constexpr bool PLANES = sizeof(T) == 4;
-    int term = PLANES ? (int)(s_begin / (ksteps > 0 ? ksteps : 1)) : 5;
-    int kstep = PLANES ? (int)(s_begin - (long long)term * ksteps) : (int)s_begin;
-    const int klast = (int)(p.K - (long long)(ksteps - 1) * GK), nsteps = (int)(s_end - s_begin);
-    auto plane_a = [&] { return PLANES ? (0x001012 >> (4 * term) & 3) * p.pa : 0; };      // planes of (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
-    auto plane_b = [&] { return PLANES ? (0x010210 >> (4 * term) & 3) * p.pb : 0; };
-    unsigned long long at_a = la.at(kstep, plane_a()), at_b = lb.at(kstep, plane_b());
+    unsigned long long at_a = la.at(kstep), at_b = lb.at(kstep);
     const unsigned long long inc_a = la.stride(), inc_b = lb.stride();
     u32x4 rsa, rsb;
-    int klim, left = nsteps;
+    int klim;
     unsigned dst;
     auto step_setup = [&](int buf) {
         rsa = tile_rsrc(at_a);
         rsb = tile_rsrc(at_b);
-        klim = left <= 0 ? 0 : kstep + 1 == ksteps ? klast : GK;      // past the end: every lane out of range, zeros nobody multiplies
-        --left;
+        klim = kstep >= kend ? 0 : kstep + 1 == ksteps ? klast : GK;          // past the end: every lane out of range, zeros nobody multiplies
         dst = lds0 + (unsigned)(buf * STAGE);
         ++kstep;
         at_a += inc_a;
         at_b += inc_b;
-        if (PLANES && kstep == ksteps) {
-            kstep = 0;
-            ++term;
-            at_a = la.at(0, plane_a());
-            at_b = lb.at(0, plane_b());
-        }
     };
     auto request = [&](int i) {
         if (i < TileLoader<BM, NW, AT>::UNITS) la.issue(i, rsa, klim, dst, wave);
@@ -345,52 +382,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(TileArgs p) {
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // the requests past the end, before LDS is used again or given back
 
-    // a lane holds columns 4 q .. 4 q + 3 (q = lane / 16) of row lane % 16 of every 16 x 16 tile
-    const int r = lane & 15, q = lane >> 4;
-    if constexpr (PART) {
-        float* part = p.part + (size_t)split * p.M * p.part_ld;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const long long m = m0 + wm + 16 * i + r;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int n = n0 + wn + 16 * j + 4 * q;
-                if (m < p.M && n < p.part_ld) *(f32x4*)(part + m * p.part_ld + n) = acc[i][j];
-            }
-        }
-    } else {
-        // through LDS, 32 rows of the wave at a time, to whole rows: each lane then has 8 columns of one row, and 8 neighbouring
-        // lanes of a 64-column wave tile write whole 128-byte lines
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        float* st = (float*)lds + wave * (ER * EP);
-        constexpr int LPR = WTN / 8, RPI = 64 / LPR;          // lanes per row, rows per step
-        const int c = (lane % LPR) * 8, n = n0 + wn + c;
-        float bias[8];
-        load_bias<T, 8>(p, n, bias);
-#pragma unroll 1
-        for (int pass = 0; pass < WTM / ER; ++pass) {
-#pragma unroll
-            for (int w = 0; w < WTM / ER; ++w) {
-                if (w != pass) continue;
-#pragma unroll
-                for (int i = 0; i < ER / 16; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) *(f32x4*)(st + (16 * i + r) * EP + 16 * j + 4 * q) = acc[w * (ER / 16) + i][j];
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll 1
-            for (int it = 0; it < ER / RPI; ++it) {
-                const int row = it * RPI + lane / LPR;
-                const long long m = m0 + wm + pass * ER + row;
-                float v[8];
-                const f32x4 v0 = *(const f32x4*)(st + row * EP + c), v1 = *(const f32x4*)(st + row * EP + c + 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { v[j] = v0[j]; v[4 + j] = v1[j]; }
-                if (m < p.M && n < p.N) row_epilogue<T, 8>(p, v, bias, m, n);
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
-    }
+    tile_store<WTM, WTN, T, PART>(p, acc, lds, split, wave, lane, m0 + wm, n0 + wn);
 }
 
 // Adds the split sums and applies the epilogue; 8 columns of a row belong to SL lanes, lane k of which adds splits k, k + SL, ... in
@@ -437,57 +429,190 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(TileArgs p) {
     }
 }
 
-// ---- operands in the kernel's form -------------------------------------------------------------------------------------
-// x as three bf16 values whose sum is x to 24 bits (rounded, not cut: the dropped products of two operands then have either sign).
-// Values that would round to infinity are cut; an infinity or NaN stays in the first value.
-__device__ __forceinline__ void split3(float x, bf16_t* o) {
-    bf16_t h = f2bf(x);
-    const bool finite = (__builtin_bit_cast(unsigned, x) & 0x7f800000u) != 0x7f800000u;
-    if (finite && (h & 0x7f80) == 0x7f80) h = (bf16_t)(__builtin_bit_cast(unsigned, x) >> 16);
-    const float r1 = finite ? x - bf2f(h) : 0.f;
-    const bf16_t m = f2bf(r1);
-    o[0] = h;
-    o[1] = m;
-    o[2] = f2bf(r1 - bf2f(m));
+// ---- operands through registers ------------------------------------------------------------------------------------------
+constexpr int SK = 32;                                // k per step
+
+// two f32 -> the high, middle and low bf16 pairs.  hi is cut, not rounded (no overflow at the largest values, and an infinity or NaN
+// leaves a NaN in the rest), mid and lo are rounded: what is dropped has either sign.
+__device__ __forceinline__ void split3(float x0, float x1, unsigned& hi, unsigned& mid, unsigned& lo) {
+    const unsigned b0 = __builtin_bit_cast(unsigned, x0), b1 = __builtin_bit_cast(unsigned, x1);
+    hi = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+    const float r0 = x0 - __builtin_bit_cast(float, b0 & 0xffff0000u), r1 = x1 - __builtin_bit_cast(float, b1 & 0xffff0000u);
+    mid = pack_bf2(r0, r1);
+    lo = pack_bf2(r0 - __builtin_bit_cast(float, mid << 16), r1 - __builtin_bit_cast(float, mid & 0xffff0000u));
 }
 
-// 8 values -> `planes` bf16 planes at dst, dst + plane, ...
-template <typename T>
-__device__ __forceinline__ void store_planes8(bf16_t* dst, long long plane, const float* v) {
-    if constexpr (sizeof(T) == 2) {
-        store_vec<8>(dst, v);
-    } else {
-        bf16_t o[8][3];
+// R x 32 of an operand: 256 threads, chunks of 8 values.  LDS planes of bf16: along k 64-byte rows of four 16-byte chunks, chunk c
+// of row r at c ^ g(r / 4 % 4) with g = 0, 2, 3, 1 (the four lane groups of a ds_read_b128 each hit sixteen different chunks); across k
+// as in TileLoader.
+template <typename E, int R, bool T>
+struct StagedOperand {
+    static constexpr int P = sizeof(E) == 4 ? 3 : 1, CH = R / 64, CPR = R / 8, PLANE = R * SK * 2;
+    u32x4 v[CH][sizeof(E) == 4 ? 2 : 1];
+    const E* base; long long ld, row0, rows;
+    static_assert(R % 64 == 0, "whole chunks per thread");
+
+    __device__ __forceinline__ void load(long long k0, long long K, int tid) {
+        const bool inside = row0 + R <= rows && k0 + SK <= K;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) split3(v[j], o[j]);
+        for (int i = 0; i < CH; ++i) {
+            const int e = tid + 256 * i;
+            const long long row = T ? k0 + e / CPR : row0 + e / 4, col = T ? row0 + 8 * (e % CPR) : k0 + 8 * (e % 4);
+            const E* p = base + row * ld + col;
+            if (inside) {
 #pragma unroll
-        for (int t = 0; t < 3; ++t) {
-            u16x8 q;
+                for (int h = 0; h < (sizeof(E) == 4 ? 2 : 1); ++h) v[i][h] = *(const u32x4_any*)(p + 4 * h);
+            } else {
+                const long long left = row < (T ? K : rows) ? (T ? rows : K) - col : 0;          // elements of the chunk that exist
+                if constexpr (sizeof(E) == 4) {
+                    unsigned o[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = o[j][t];
-            *(u16x8*)(dst + t * plane) = q;
+                    for (int j = 0; j < 8; ++j) o[j] = j < left ? ((const unsigned*)p)[j] : 0u;
+                    v[i][0] = u32x4{o[0], o[1], o[2], o[3]};
+                    v[i][1] = u32x4{o[4], o[5], o[6], o[7]};
+                } else {
+                    u16x8 o;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) o[j] = j < left ? p[j] : (bf16_t)0;
+                    v[i][0] = __builtin_bit_cast(u32x4, o);
+                }
+            }
         }
     }
+    __device__ __forceinline__ void store(unsigned char* tile, int tid) const {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int e = tid + 256 * i;
+            int at;
+            if constexpr (T) {
+                const int k = e / CPR, c = e % CPR;
+                at = k * 2 * R + ((((c >> 1) ^ (((k & 3) | ((k >> 3 & 1) << 2)) & (R / 16 - 1))) * 2 + (c & 1)) * 16);
+            } else {
+                const int r = e / 4, g = r >> 2 & 3;
+                at = r * 64 + (((e % 4) ^ ((g ^ (g >> 1)) & 1) << 1 ^ (g >> 1)) * 16);
+            }
+            if constexpr (sizeof(E) == 4) {
+                u32x4 o[3];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned q0 = v[i][j >> 1][2 * (j & 1)], q1 = v[i][j >> 1][2 * (j & 1) + 1];
+                    unsigned hi, mid, lo;
+                    split3(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1), hi, mid, lo);
+                    o[0][j] = hi; o[1][j] = mid; o[2][j] = lo;
+                }
+#pragma unroll
+                for (int t = 0; t < 3; ++t) *(u32x4*)(tile + t * PLANE + at) = o[t];
+            } else {
+                *(u32x4*)(tile + at) = v[i][0];
+            }
+        }
+    }
+};
+
+template <int R, int NT, bool T>
+struct StagedReader {
+    unsigned addr[T ? NT : 1];
+    __device__ __forceinline__ void init(int w0, int lane) {
+        const int r = lane & 15, q = lane >> 4;
+        if constexpr (T) {
+            const int f = ((r >> 2) | ((q & 1) << 2)) & (R / 16 - 1);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) addr[t] = (unsigned)((8 * q + (r >> 2)) * 2 * R + (((w0 / 16 + t) ^ f) * 32) + 8 * (r & 3));
+        } else {
+            const int g = r >> 2;
+            addr[0] = (unsigned)((w0 + r) * 64 + ((q ^ ((g ^ (g >> 1)) & 1) << 1 ^ (g >> 1)) * 16));
+        }
+    }
+    __device__ __forceinline__ bf16x8 get(const unsigned char* plane, int t) const {
+        if constexpr (T) {
+            const unsigned char* p = plane + addr[t];
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(lds_ptr)p);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(lds_ptr)(p + 4 * 2 * R));
+            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            return *(const bf16x8*)(plane + addr[0] + t * 1024);
+        }
+    }
+};
+
+template <int B, typename T>
+constexpr int staged_lds() {
+    constexpr int tiles = (sizeof(T) == 4 ? 3 : 1) * 2 * B * SK * 2, ep = epilogue_bytes(4, B / 2);
+    return tiles > ep ? tiles : ep;
 }
 
-// [rows, cols] of T with any row stride -> bf16 plane(s) [rows, ld], ld = cols rounded up to 8, zeros behind the columns
-template <typename T>
-__global__ __launch_bounds__(256) void pack_rows_kernel(const T* src, long long src_ld, long long rows, int cols, bf16_t* dst, int ld,
-                                                        long long plane) {
-    const int c8 = ld / 8;
-    const long long n = rows * c8;
-    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long long)gridDim.x * 256) {
-        const long long r = e / c8;
-        const int c = (int)(e - r * c8) * 8;
-        const T* s = src + r * src_ld + c;
-        float v[8];
-        if (c + 8 <= cols) load_vec<8>(s, v);
-        else {
+// B x B tile, four waves of B/2 x B/2; the next step's operands wait in registers while this step's are multiplied
+template <int B, bool AT, bool BT, typename T, bool PART>
+__global__ __launch_bounds__(256, 2) void gemm_staged_kernel(TileArgs p) {
+    constexpr int WT = B / 2, MT = WT / 16, P = sizeof(T) == 4 ? 3 : 1, PLANE = B * SK * 2;
+    __shared__ __align__(1024) unsigned char lds[staged_lds<B, T>()];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tm, tn, split;
+    tile_of_block(p, tm, tn, split);
+    const long long m0 = (long long)tm * B;
+    const int n0 = tn * B, wm = (wave >> 1) * WT, wn = (wave & 1) * WT;
+    StagedOperand<T, B, AT> sa;
+    StagedOperand<T, B, BT> sb;
+    sa.base = (const T*)p.a; sa.ld = p.lda; sa.row0 = m0; sa.rows = p.M;
+    sb.base = (const T*)p.b; sb.ld = p.ldb; sb.row0 = n0; sb.rows = p.N;
+    StagedReader<B, MT, AT> ra;
+    StagedReader<B, MT, BT> rb;
+    ra.init(wm, lane);
+    rb.init(wn, lane);
+    const long long ksteps = (p.K + SK - 1) / SK;
+    const long long s0 = ksteps * split / p.splits, s1 = ksteps * (split + 1) / p.splits;
+    f32x4 acc[MT][MT], low[P == 3 ? MT : 1][P == 3 ? MT : 1];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f32(s[j]) : 0.f;
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (P == 3) low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        store_planes8<T>(dst + r * ld + c, plane, v);
+    if (s0 < s1) {
+        sa.load(s0 * SK, p.K, tid);
+        sb.load(s0 * SK, p.K, tid);
     }
+    unsigned char* const ta = lds;
+    unsigned char* const tb = lds + P * PLANE;
+    for (long long s = s0; s < s1; ++s) {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        sa.store(ta, tid);
+        sb.store(tb, tid);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (s + 1 < s1) {
+            sa.load((s + 1) * SK, p.K, tid);
+            sb.load((s + 1) * SK, p.K, tid);
+        }
+        bf16x8 fb[P][MT];
+#pragma unroll
+        for (int t = 0; t < P; ++t)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) fb[t][j] = rb.get(tb + t * PLANE, j);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            bf16x8 fa[P];
+#pragma unroll
+            for (int t = 0; t < P; ++t) fa[t] = ra.get(ta + t * PLANE, i);
+            if constexpr (P == 3) {
+#pragma unroll
+                for (int u = 0; u < 5; ++u) {                  // mid mid, lo hi, hi lo, mid hi, hi mid
+                    constexpr int UA[5] = {1, 2, 0, 1, 0}, UB[5] = {1, 0, 2, 0, 1};
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) low[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[UB[u]][j], fa[UA[u]], low[i][j], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[0][j], fa[0], acc[i][j], 0, 0, 0);
+        }
+    }
+    if constexpr (P == 3) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[i][j] += low[i][j];
+    }
+    tile_store<WT, WT, T, PART>(p, acc, lds, split, wave, lane, m0 + wm, n0 + wn);
 }
 
 }  // namespace srmi

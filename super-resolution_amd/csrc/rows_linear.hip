@@ -5,9 +5,8 @@
 //   dx = dz w              [M, K] = [M, N] [N, K]
 //   dw = dz^T x            [N, K] = [M, N]^T [M, K]
 //
-// All three are the tile product of rows_gemm.h.  bf16 operands whose rows lie on 16-byte boundaries are read in place; others, and f32
-// operands (as three bf16 planes), are first laid out in the workspace: one pass over M K + N K elements in front of M N K
-// multiplications.  Few rows take the products of rows_thin.h, which read every operand once, in place, whatever its alignment.
+// All three are tile products: bf16 operands whose rows lie on 16-byte boundaries take gemm_tile_kernel, f32 ones and others
+// gemm_staged_kernel (rows_gemm.h).  Few rows take the products of rows_thin.h.  Nothing is re-laid out in memory.
 #include "rows_thin.h"
 
 namespace srmi {
@@ -17,28 +16,27 @@ int slot_sum_launch(const float* part, int slots, int n, int n0, void* o0, void*
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static int up8(int n) { return (n + 7) & ~7; }
 
-// ---- the tile product: shape -> tile, split ------------------------------------------------------------------------------
-enum { TILE_256 = 0, TILE_128 = 1, TILE_32 = 2 };
-struct TilePlan { int kind, bm, bn, tiles_m, tiles_n, splits; size_t part_bytes; };
+// ---- the tile product: shape -> kernel, tile, split --------------------------------------------------------------------------
+enum TileKind { TILE_256, TILE_128, TILE_32, STAGED_128, STAGED_64 };
+struct TilePlan { TileKind kind; long long tiles_m; int tiles_n, splits; size_t part_bytes; };
 
-static TilePlan tile_plan(long long M, int N, long long K, int terms) {
+// direct: both operands can be read by the DMA
+static TilePlan tile_plan(bool direct, long long M, int N, long long K) {
     TilePlan t;
-    const long long steps = terms * ((K + GK - 1) / GK);
-    const long long tiles256 = ((M + 255) / 256) * ((N + 255) / 256);
-    t.kind = M <= 32 ? TILE_32 : tiles256 >= 200 && steps >= 8 ? TILE_256 : TILE_128;
-#ifdef FORCE_KIND
-    if (M > 32) t.kind = FORCE_KIND;
-#endif
-    t.bm = t.kind == TILE_256 ? 256 : t.kind == TILE_128 ? 128 : 32;
-    t.bn = t.kind == TILE_256 ? 256 : 128;
-    const long long tm = (M + t.bm - 1) / t.bm, tn = (N + t.bn - 1) / t.bn, tiles = tm * tn;
-    t.tiles_m = (int)(tm > 0x7fffffff ? 0x7fffffff : tm);
-    t.tiles_n = (int)tn;
+    auto tiles = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+    const long long steps = (K + (direct ? GK : SK) - 1) / (direct ? GK : SK);
+    if (direct) t.kind = M <= 32 ? TILE_32 : tiles(256, 256) >= 200 && steps >= 8 ? TILE_256 : TILE_128;
+    else t.kind = tiles(128, 128) >= 384 ? STAGED_128 : STAGED_64;
+    const int bm = t.kind == TILE_256 ? 256 : t.kind == TILE_32 ? 32 : t.kind == STAGED_64 ? 64 : 128;
+    const int bn = t.kind == TILE_256 ? 256 : t.kind == STAGED_64 ? 64 : 128;
+    t.tiles_m = (M + bm - 1) / bm;
+    t.tiles_n = (N + bn - 1) / bn;
     t.splits = 1;
-    if (tiles < 256) {
-        long long s = 512 / (tiles ? tiles : 1);
-        if (s > steps / 4) s = steps / 4;
-        t.splits = (int)(s < 1 ? 1 : s > 128 ? 128 : s);
+    const long long n = t.tiles_m * t.tiles_n;
+    if (n < 256 && n > 0) {
+        const long long s = 512 / n, most = steps / 4;
+        t.splits = (int)(s < most ? (s < 128 ? s : 128) : most);
+        if (t.splits < 1) t.splits = 1;
     }
     t.part_bytes = t.splits > 1 ? up256((size_t)t.splits * M * up8(N) * sizeof(float)) : 0;
     return t;
@@ -56,30 +54,38 @@ static int join(const TileArgs& p, hipStream_t s) {
 }
 
 template <int BM, int BN, int WM, int WN, int NSTAGE, bool PIPE, bool AT, bool BT, typename T>
-static int tile_go(const TileArgs& p, hipStream_t s) {
-    const dim3 grid((unsigned)((long long)p.tiles_m * p.tiles_n * p.splits)), block(64 * WM * WN);
+static void tile_go(const TileArgs& p, unsigned grid, hipStream_t s) {
     constexpr size_t lds = (size_t)NSTAGE * (BM + BN) * GK * 2;
-    if (p.splits > 1) {
-        hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, NSTAGE, PIPE, T, true>), grid, block, lds, s, p);
-        return join<T>(p, s);
-    } else {
-        hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, NSTAGE, PIPE, T, false>), grid, block, lds, s, p);
-    }
-    return hip_check(hipGetLastError(), "linear product");
+    if (p.splits > 1) hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, NSTAGE, PIPE, T, true>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
+    else hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, NSTAGE, PIPE, T, false>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
+}
+template <int B, bool AT, bool BT, typename T>
+static void staged_go(const TileArgs& p, unsigned grid, hipStream_t s) {
+    if (p.splits > 1) hipLaunchKernelGGL((gemm_staged_kernel<B, AT, BT, T, true>), dim3(grid), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((gemm_staged_kernel<B, AT, BT, T, false>), dim3(grid), dim3(256), 0, s, p);
 }
 
 template <bool AT, bool BT, typename T>
-static int tile_gemm(TileArgs& p, float* part, hipStream_t s) {
+static int tile_gemm(bool direct, TileArgs& p, float* part, hipStream_t s) {
     if (p.M == 0 || p.N == 0) return SRMI_OK;
-    const TilePlan t = tile_plan(p.M, p.N, p.K, p.terms);
-    if ((long long)t.tiles_m * t.tiles_n * t.splits > 0x7fffffff) { set_error("linear: more than 2^31 tiles"); return SRMI_EUNSUPPORTED; }
-    p.tiles_m = t.tiles_m; p.tiles_n = t.tiles_n; p.splits = t.splits;
+    const TilePlan t = tile_plan(direct, p.M, p.N, p.K);
+    const long long grid = t.tiles_m * t.tiles_n * t.splits;
+    if (grid > 0x7fffffff) { set_error("linear: more than 2^31 tiles"); return SRMI_EUNSUPPORTED; }
+    p.tiles_m = (int)t.tiles_m; p.tiles_n = t.tiles_n; p.splits = t.splits;
     p.part = part; p.part_ld = up8(p.N);
-    switch (t.kind) {
-        case TILE_256: return tile_go<256, 256, 2, 4, 2, true, AT, BT, T>(p, s);
-        case TILE_128: return tile_go<128, 128, 2, 2, 2, false, AT, BT, T>(p, s);
-        default: return tile_go<32, 128, 1, 4, 3, true, AT, BT, T>(p, s);
+    const unsigned g = (unsigned)grid;
+    if constexpr (sizeof(T) == 2) {
+        switch (t.kind) {
+            case TILE_256: tile_go<256, 256, 2, 4, 2, true, AT, BT, T>(p, g, s); break;
+            case TILE_128: tile_go<128, 128, 2, 2, 2, false, AT, BT, T>(p, g, s); break;
+            case TILE_32: tile_go<32, 128, 1, 4, 3, true, AT, BT, T>(p, g, s); break;
+            default: break;
+        }
     }
+    if (t.kind == STAGED_128) staged_go<128, AT, BT, T>(p, g, s);
+    else if (t.kind == STAGED_64) staged_go<64, AT, BT, T>(p, g, s);
+    const int rc = hip_check(hipGetLastError(), "linear product");
+    return rc || t.splits == 1 ? rc : join<T>(p, s);
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------------
@@ -134,38 +140,19 @@ static int thin_bwd_go(const srmi_linear_desc& d, const float* dz, long long ldd
     return hip_check(hipGetLastError(), "linear bwd");
 }
 
-// ---- operands -------------------------------------------------------------------------------------------------------------
-struct Operand { const bf16_t* p; long long ld, plane; };
-
-static bool in_place(const srmi_linear_desc& d, int cols, long long ld) {
+// rows the DMA can read: 16-byte aligned, whole chunks (zeros behind the last column count as columns)
+static bool dma_rows(const srmi_linear_desc& d, int cols, long long ld) {
     return d.dtype == SRMI_BF16 && d.align >= 16 && cols % 8 == 0 && ld % 8 == 0 && ld <= GEMM_MAX_LD;
 }
-static size_t packed_bytes(const srmi_linear_desc& d, long long rows, int cols) {
-    return up256((size_t)rows * up8(cols) * (d.dtype == SRMI_BF16 ? 2 : 6));
-}
 
-template <typename T>
-static int operand(const srmi_linear_desc& d, const void* src, long long ld, long long rows, int cols, char*& ws, Operand* o, hipStream_t s) {
-    if (in_place(d, cols, ld)) { *o = Operand{(const bf16_t*)src, ld, 0}; return SRMI_OK; }
-    *o = Operand{(const bf16_t*)ws, up8(cols), rows * up8(cols)};
-    ws += packed_bytes(d, rows, cols);
-    const long long n = rows * (up8(cols) / 8);
-    if (n == 0) return SRMI_OK;
-    const long long g = (n + 255) / 256;
-    hipLaunchKernelGGL((pack_rows_kernel<T>), dim3((unsigned)(g > 8192 ? 8192 : g)), dim3(256), 0, s, (const T*)src, ld, rows, cols,
-                       (bf16_t*)o->p, up8(cols), o->plane);
-    return hip_check(hipGetLastError(), "linear operand layout");
-}
-
-// ---- dz = dy * act'(saved) in the products' form, and the partial column sums of dz --------------------------------------------
+// ---- dz = dy * act'(saved) and the partial column sums of dz -----------------------------------------------------------------
 // Workgroup (slot of rows, strip of columns): tx lanes of 8 columns, 256 / tx rows at a time; the sums of a workgroup's rows
 // are added in LDS and stored as one partial row, a second launch adds the partial rows in index order.  db sums the f32
 // products, before dz is rounded to bf16 (the matrix cores' operand type: half a step of 2^-8 per term of dx and dw, as in y itself).
 struct DzArgs {
     const void* dy; long long lddy;
     const void* saved;                // dense [M, N]: z, or y where its sign says the same; NULL: act'(z) = 1
-    bf16_t* dz; int ldz; long long plane;      // [M, ldz] planes, zeros behind column N; NULL: only the sums are wanted
-    float* dzf;                       // f32 with few rows: dense [M, N] instead
+    void* dz; int ldz;                // [M, ldz], zeros behind column N; NULL: only the sums are wanted
     float* part;                      // [gridDim.x][N] or NULL
     long long M; int N;
     int act; float act_param;
@@ -201,18 +188,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) g[j] *= row_act_slope<sizeof(T) == 2>(z[j], p.act, p.act_param);
             }
-            if constexpr (sizeof(T) == 4) {
-                if (p.dzf) {
-                    float* o = p.dzf + m * p.N + c;
-                    if (whole) store_vec<8>(o, g);
-                    else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (c + j < p.N) o[j] = g[j];
-                    }
-                }
-            }
-            if (p.dz) store_planes8<T>(p.dz + m * p.ldz + c, p.plane, g);
+            if (p.dz) store_vec<8>((T*)p.dz + m * p.ldz + c, g);
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] += g[j];
         }
@@ -231,57 +207,63 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
     }
 }
 
-static int dz_slots(long long M) { return (int)(M < 8 ? 1 : M / 8 > 256 ? 256 : M / 8); }
+// lanes of 8 columns per row: a power of two; rows of a pass; workgroups of rows = partial rows of db: one per pass up to eight
+// workgroups per CU (36864 x 1024 gelu: 148 us with 256 workgroups, 52 with 1024)
+static int dz_tx(int N) {
+    int tx = 1;
+    while (tx < 256 && tx * 8 < N) tx *= 2;
+    return tx;
+}
+static int dz_slots(long long M, int N) {
+    const int tx = dz_tx(N), strips = N / (tx * 8) + 1;
+    const long long want = (M + 256 / tx - 1) / (256 / tx), most = 2048 / strips < 64 ? 64 : 2048 / strips;
+    return (int)(want < 1 ? 1 : want > most ? most : want);
+}
 
 template <typename T>
 static int dz_launch(DzArgs& p, hipStream_t s) {
     if (p.N == 0) return SRMI_OK;
-    p.tx = 1;
-    while (p.tx < 256 && p.tx * 8 < p.N) p.tx *= 2;
-    const dim3 grid(dz_slots(p.M), (p.N + p.tx * 8 - 1) / (p.tx * 8));
+    p.tx = dz_tx(p.N);
+    const dim3 grid(dz_slots(p.M, p.N), (p.N + p.tx * 8 - 1) / (p.tx * 8));
     hipLaunchKernelGGL((linear_dz_kernel<T>), grid, dim3(256), 0, s, p);
     return hip_check(hipGetLastError(), "linear dz");
 }
 
 // ---- entry points' bodies ---------------------------------------------------------------------------------------------------
-static int terms_of(const srmi_linear_desc& d) { return d.dtype == SRMI_BF16 ? 1 : 6; }
-static bool own_dz(const srmi_linear_desc& d) { return d.act != SRMI_ACT_NONE || !in_place(d, d.N, d.lddy); }
+static bool own_dz(const srmi_linear_desc& d) { return d.act != SRMI_ACT_NONE; }
+static bool dma_fwd(const srmi_linear_desc& d) { return dma_rows(d, d.K, d.ldx) && dma_rows(d, d.K, d.ldw); }
+static bool dma_dz(const srmi_linear_desc& d) { return own_dz(d) ? d.dtype == SRMI_BF16 : dma_rows(d, d.N, d.lddy); }
+static bool dma_dx(const srmi_linear_desc& d) { return dma_dz(d) && dma_rows(d, d.K, d.ldw); }
+static bool dma_dw(const srmi_linear_desc& d) { return dma_dz(d) && dma_rows(d, d.K, d.ldx); }
+static size_t db_bytes(const srmi_linear_desc& d) { return up256((size_t)dz_slots(d.M, d.N) * d.N * sizeof(float)); }
+static size_t dz_bytes(const srmi_linear_desc& d) { return own_dz(d) ? up256((size_t)d.M * up8(d.N) * (d.dtype == SRMI_BF16 ? 2 : 4)) : 0; }
 
+// backward: [partial db][dz][split sums of dx, then of dw]
 size_t linear_workspace_bytes(const srmi_linear_desc& d, int pass) {
-    size_t n = 0;
-    if (pass == SRMI_PASS_FWD && thin_fwd(d)) return thin_part_bytes(d);
-    if (pass == SRMI_PASS_BWD && thin_bwd(d))
-        return up256((size_t)dz_slots(d.M) * d.N * sizeof(float)) + (d.act != SRMI_ACT_NONE ? up256((size_t)d.M * d.N * sizeof(float)) : 0);
-    if (!in_place(d, d.K, d.ldx)) n += packed_bytes(d, d.M, d.K);
-    if (!in_place(d, d.K, d.ldw)) n += packed_bytes(d, d.N, d.K);
-    if (pass == SRMI_PASS_FWD) return n + tile_plan(d.M, d.N, d.K, terms_of(d)).part_bytes;
-    n += up256((size_t)dz_slots(d.M) * d.N * sizeof(float));
-    if (own_dz(d)) n += packed_bytes(d, d.M, d.N);
-    const size_t pd = tile_plan(d.M, d.K, d.N, terms_of(d)).part_bytes, pw = tile_plan(d.N, d.K, d.M, terms_of(d)).part_bytes;
-    return n + (pd > pw ? pd : pw);
+    if (pass == SRMI_PASS_FWD) return thin_fwd(d) ? thin_part_bytes(d) : tile_plan(dma_fwd(d), d.M, d.N, d.K).part_bytes;
+    const size_t n = db_bytes(d) + dz_bytes(d);
+    if (thin_bwd(d)) return n;
+    const size_t px = tile_plan(dma_dx(d), d.M, d.K, d.N).part_bytes, pw = tile_plan(dma_dw(d), d.N, d.K, d.M).part_bytes;
+    return n + (px > pw ? px : pw);
 }
 
 template <typename T>
 static int linear_fwd_t(const srmi_linear_desc& d, const void* x, const void* w, const void* bias, const void* residual, void* y, void* z,
-                        char* ws, hipStream_t s) {
+                        float* ws, hipStream_t s) {
     TileArgs p = {};
-    p.M = d.M; p.N = d.N; p.K = d.K; p.terms = terms_of(d);
+    p.M = d.M; p.N = d.N; p.K = d.K;
     p.bias = bias; p.residual = residual; p.ldr = d.ldr; p.y = y; p.ldy = d.N; p.z = z;
     p.act = d.act; p.act_param = d.act_param;
-    if (thin_fwd(d)) return thin_fwd_go<T>(d, x, w, p, (float*)ws, s);
-    Operand a, b;
-    int rc;
-    if ((rc = operand<T>(d, x, d.ldx, d.M, d.K, ws, &a, s))) return rc;
-    if ((rc = operand<T>(d, w, d.ldw, d.N, d.K, ws, &b, s))) return rc;
-    p.a = a.p; p.lda = a.ld; p.pa = a.plane;
-    p.b = b.p; p.ldb = b.ld; p.pb = b.plane;
-    return tile_gemm<false, false, T>(p, (float*)ws, s);
+    if (thin_fwd(d)) return thin_fwd_go<T>(d, x, w, p, ws, s);
+    p.a = x; p.lda = d.ldx;
+    p.b = w; p.ldb = d.ldw;
+    return tile_gemm<false, false, T>(dma_fwd(d), p, ws, s);
 }
 
 int linear_fwd(const srmi_linear_desc& d, const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, void* ws,
                hipStream_t s) {
-    return d.dtype == SRMI_BF16 ? linear_fwd_t<bf16_t>(d, x, w, bias, residual, y, z, (char*)ws, s)
-                                : linear_fwd_t<float>(d, x, w, bias, residual, y, z, (char*)ws, s);
+    return d.dtype == SRMI_BF16 ? linear_fwd_t<bf16_t>(d, x, w, bias, residual, y, z, (float*)ws, s)
+                                : linear_fwd_t<float>(d, x, w, bias, residual, y, z, (float*)ws, s);
 }
 
 template <typename T>
@@ -289,41 +271,36 @@ static int linear_bwd_t(const srmi_linear_desc& d, const void* x, const void* w,
                         void* db, char* ws, hipStream_t s) {
     int rc;
     float* part = (float*)ws;
-    ws += up256((size_t)dz_slots(d.M) * d.N * sizeof(float));
-    Operand dz = {(const bf16_t*)dy, d.lddy, 0}, o;
-    const bool thin = thin_bwd(d), own = !thin && own_dz(d) && (dx || dw);
-    float* dzf = thin && d.act != SRMI_ACT_NONE && (dx || dw) ? (float*)ws : nullptr;
-    if (own) {
-        dz = Operand{(const bf16_t*)ws, up8(d.N), d.M * up8(d.N)};
-        ws += packed_bytes(d, d.M, d.N);
+    const void* dz = dy;
+    long long lddz = d.lddy;
+    DzArgs q = {};
+    if (own_dz(d) && (dx || dw)) {
+        dz = q.dz = ws + db_bytes(d);
+        lddz = q.ldz = up8(d.N);
     }
-    if (db || ((own || dzf) && d.M > 0)) {
-        DzArgs q = {};
-        q.dy = dy; q.lddy = d.lddy; q.saved = d.act != SRMI_ACT_NONE ? saved : nullptr;
-        q.dz = own ? (bf16_t*)dz.p : nullptr; q.ldz = up8(d.N); q.plane = dz.plane; q.dzf = dzf;
+    if (db || (q.dz && d.M > 0)) {
+        q.dy = dy; q.lddy = d.lddy; q.saved = own_dz(d) ? saved : nullptr;
         q.part = db ? part : nullptr;
         q.M = d.M; q.N = d.N; q.act = d.act; q.act_param = d.act_param;
         if ((rc = dz_launch<T>(q, s))) return rc;
-        if (db && (rc = slot_sum_launch(part, dz_slots(d.M), d.N, d.N, db, nullptr, sizeof(T) == 2, s))) return rc;
+        if (db && (rc = slot_sum_launch(part, dz_slots(d.M, d.N), d.N, d.N, db, nullptr, sizeof(T) == 2, s))) return rc;
     }
-    if (thin) return thin_bwd_go(d, dzf ? dzf : (const float*)dy, dzf ? d.N : d.lddy, x, w, dx, dw, s);
+    if (thin_bwd(d)) return thin_bwd_go(d, (const float*)dz, lddz, x, w, dx, dw, s);
+    part = (float*)(ws + db_bytes(d) + dz_bytes(d));
     TileArgs p = {};
     p.act = SRMI_ACT_NONE;
-    p.terms = terms_of(d);
-    p.a = dz.p; p.lda = dz.ld; p.pa = dz.plane;
+    p.a = dz; p.lda = lddz;
     if (dx) {
-        if ((rc = operand<T>(d, w, d.ldw, d.N, d.K, ws, &o, s))) return rc;
-        p.b = o.p; p.ldb = o.ld; p.pb = o.plane;
+        p.b = w; p.ldb = d.ldw;
         p.M = d.M; p.N = d.K; p.K = d.N;
         p.y = dx; p.ldy = d.K;
-        if ((rc = tile_gemm<false, true, T>(p, (float*)ws, s))) return rc;
+        if ((rc = tile_gemm<false, true, T>(dma_dx(d), p, part, s))) return rc;
     }
     if (dw) {
-        if ((rc = operand<T>(d, x, d.ldx, d.M, d.K, ws, &o, s))) return rc;
-        p.b = o.p; p.ldb = o.ld; p.pb = o.plane;
+        p.b = x; p.ldb = d.ldx;
         p.M = d.N; p.N = d.K; p.K = d.M;
         p.y = dw; p.ldy = d.K;
-        if ((rc = tile_gemm<true, true, T>(p, (float*)ws, s))) return rc;
+        if ((rc = tile_gemm<true, true, T>(dma_dw(d), p, part, s))) return rc;
     }
     return SRMI_OK;
 }

@@ -297,21 +297,27 @@ __global__ __launch_bounds__(256) void norm_wide_dw_kernel(NormArgs a) {
     store_cols<V, true>(slot + a.C, c, a.C, db);
 }
 
-// out[c] = sum over slots of part[slot][c], n columns; 32 columns x 8 slot lanes per workgroup, slots added in index order
-// within a lane and the 8 lanes in index order.  Two outputs: columns [0, n0) to o0, [n0, n) to o1.
-__global__ __launch_bounds__(256) void slot_sum_kernel(const float* part, int slots, int n, int n0, void* o0, void* o1, int out_bf16) {
-    __shared__ float red[8][32];
-    const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + cl;
+// out[c] = sum over slots of part[slot][c], n columns.  16 columns x 64 lanes per workgroup: lane k adds slots k, k + 64, ... in order, then
+// four lanes at a time and the sixteen sums are added in order.  (Many lanes per column because the launch waits on memory, not on
+// bandwidth: 512 slots of 512 columns took 20 us with 8 lanes.)  Two outputs: columns [0, n0) to o0, [n0, n) to o1.
+__global__ __launch_bounds__(1024) void slot_sum_kernel(const float* part, int slots, int n, int n0, void* o0, void* o1, int out_bf16) {
+    __shared__ float red[64][17];
+    const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4;
+    const int c = blockIdx.x * 16 + cl;
     float s = 0.f;
     if (c < n) {
-        for (int k = sl; k < slots; k += 8) s += part[(size_t)k * n + c];
+#pragma unroll 4
+        for (int k = sl; k < slots; k += 64) s += part[(size_t)k * n + c];
     }
     red[sl][cl] = s;
     __syncthreads();
+    if (sl < 16) s = red[4 * sl][cl] + red[4 * sl + 1][cl] + red[4 * sl + 2][cl] + red[4 * sl + 3][cl];
+    __syncthreads();
+    if (sl < 16) red[sl][cl] = s;
+    __syncthreads();
     if (sl == 0 && c < n) {
 #pragma unroll
-        for (int k = 1; k < 8; ++k) s += red[k][cl];
+        for (int k = 1; k < 16; ++k) s += red[k][cl];
         void* o = c < n0 ? o0 : o1;
         const int i = c < n0 ? c : c - n0;
         if (o) {
@@ -323,17 +329,26 @@ __global__ __launch_bounds__(256) void slot_sum_kernel(const float* part, int sl
 
 int slot_sum_launch(const float* part, int slots, int n, int n0, void* o0, void* o1, int out_bf16, hipStream_t s) {
     if (n == 0) return SRMI_OK;
-    hipLaunchKernelGGL(slot_sum_kernel, dim3((n + 31) / 32), dim3(256), 0, s, part, slots, n, n0, o0, o1, out_bf16);
+    hipLaunchKernelGGL(slot_sum_kernel, dim3((n + 15) / 16), dim3(1024), 0, s, part, slots, n, n0, o0, o1, out_bf16);
     return hip_check(hipGetLastError(), "slot_sum");
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 static constexpr int NORM_WIDE = 2048;      // widest row kept in registers: 32 values a lane; the re-reading kernels take what is wider
 
-// partial rows of dw / db: enough workgroups to fill the chip, each with several rows
-int norm_slots(long long rows) {
-    const long long want = (rows + 7) / 8;
-    return (int)(want < 1 ? 1 : want > 512 ? 512 : want);
+static int norm_lanes(int C, int dtype) {
+    const int v = dtype == SRMI_BF16 ? 8 : 4;
+    return C <= 8 * v ? 8 : C <= 16 * v ? 16 : C <= 32 * v ? 32 : 64;
+}
+
+// Workgroups of the backward = partial rows of dw / db: eight per CU where there are rows for them (147456 x 256 bf16: 58 us with 512
+// workgroups, 47 with 2048) and the partial rows stay below an eighth of x's bytes.
+int norm_slots(const srmi_norm_desc& d) {
+    const long long esz = d.dtype == SRMI_BF16 ? 2 : 4, per = 256 / norm_lanes(d.C, d.dtype);
+    long long most = d.rows * esz / 64;
+    most = most < 64 ? 64 : most > 2048 ? 2048 : most;
+    const long long want = (d.rows + per - 1) / per;
+    return (int)(want < 1 ? 1 : want > most ? most : want);
 }
 
 template <bool BWD, typename T, int LANES, int ITER, bool TAIL>
@@ -353,10 +368,13 @@ template <bool BWD, typename T, bool TAIL>
 static void norm_rows(const NormArgs& a, int slots, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T);
     const int C = a.C;
-    if (C <= 8 * V) norm_go<BWD, T, 8, 1, TAIL>(a, slots, s);
-    else if (C <= 16 * V) norm_go<BWD, T, 16, 1, TAIL>(a, slots, s);
-    else if (C <= 32 * V) norm_go<BWD, T, 32, 1, TAIL>(a, slots, s);
-    else if (C <= 64 * V) norm_go<BWD, T, 64, 1, TAIL>(a, slots, s);
+    switch (norm_lanes(C, V == 8 ? SRMI_BF16 : SRMI_F32)) {
+        case 8: norm_go<BWD, T, 8, 1, TAIL>(a, slots, s); return;
+        case 16: norm_go<BWD, T, 16, 1, TAIL>(a, slots, s); return;
+        case 32: norm_go<BWD, T, 32, 1, TAIL>(a, slots, s); return;
+        default: break;
+    }
+    if (C <= 64 * V) norm_go<BWD, T, 64, 1, TAIL>(a, slots, s);
     else if (C <= 128 * V) norm_go<BWD, T, 64, 2, TAIL>(a, slots, s);
     else if (C <= 256 * V) norm_go<BWD, T, 64, 4, TAIL>(a, slots, s);
     else if constexpr (V == 4) norm_go<BWD, T, 64, 8, TAIL>(a, slots, s);
@@ -395,7 +413,7 @@ int norm_fwd(const srmi_norm_desc& d, const void* x, const void* w, const void* 
     return hip_check(hipGetLastError(), "layer_norm_fwd");
 }
 
-size_t norm_workspace_bytes(const srmi_norm_desc& d) { return (size_t)norm_slots(d.rows) * 2 * d.C * sizeof(float); }
+size_t norm_workspace_bytes(const srmi_norm_desc& d) { return (size_t)norm_slots(d) * 2 * d.C * sizeof(float); }
 
 int norm_bwd(const srmi_norm_desc& d, const void* x, const void* w, const float* mean, const float* rstd, const void* dy, void* dx,
              void* dw, void* db, float* ws, hipStream_t s) {
@@ -403,7 +421,7 @@ int norm_bwd(const srmi_norm_desc& d, const void* x, const void* w, const float*
     fill_args(&a, d, x, w, nullptr);
     a.y = dx; a.mean = (float*)mean; a.rstd = (float*)rstd; a.dy = dy; a.lddy = d.lddy;
     a.part = dw || db ? ws : nullptr;
-    const int slots = norm_slots(d.rows);
+    const int slots = norm_slots(d);
     if (d.dtype == SRMI_BF16) norm_dispatch<true, bf16_t>(a, slots, s);
     else norm_dispatch<true, float>(a, slots, s);
     const int rc = hip_check(hipGetLastError(), "layer_norm_bwd");
