@@ -28,7 +28,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
-constexpr int GK = 64;                               // k per step
 constexpr unsigned OUT_OF_RANGE = 0x80000000u;       // buffer offset = the resource's size: reads zeros
 constexpr long long GEMM_MAX_LD = 1 << 22;           // a tile's offsets stay below 2^31 bytes
 
@@ -123,15 +122,24 @@ __device__ __forceinline__ u32x4 tile_rsrc(unsigned long long base) {
                  OUT_OF_RANGE, 0x00020000u};
 }
 
+// along k: the permutation of a row's 16-byte chunks.  The 16 lanes that a ds_read_b128 serves at a time then hit sixteen different
+// chunks of the 256 bytes of banks: rows of 128 bytes (64 k) take r mod 8, rows of 64 bytes 0, 2, 3, 1 by r / 4 mod 4.
+template <int GK>
+__device__ __forceinline__ int chunk_key(int r) {
+    if constexpr (GK == 64) return r & 7;
+    const int g = r >> 2 & 3;
+    return (((g ^ (g >> 1)) & 1) << 1) | (g >> 1);
+}
+
 // Staging of one operand: R rows, NW waves, T: stored across k
-template <int R, int NW, bool T>
+template <int R, int NW, bool T, int GK>
 struct TileLoader {
-    static constexpr int UNITS = R / 8 / NW;          // KiB per wave and step
+    static constexpr int UNITS = R * GK / 512 / NW;   // KiB per wave and step
     static constexpr int CPR = R / 8;                 // chunks per k row (T)
     unsigned voff[UNITS];
     int kk[T ? UNITS : 1];                            // k of the lane's chunk inside the step
     const bf16_t* base; long long ld;
-    static_assert(R % (8 * NW) == 0, "whole KiB per wave");
+    static_assert(R * GK % (512 * NW) == 0, "whole KiB per wave");
 
     // row0: the tile's first row; rows: rows of the operand
     __device__ __forceinline__ void init(const bf16_t* p, long long ld_, long long row0, long long rows, int wave, int lane) {
@@ -147,8 +155,8 @@ struct TileLoader {
                 kk[i] = k;
                 voff[i] = row0 + 8 * c < rows ? (unsigned)(k * ld_ * 2 + 16 * c) : OUT_OF_RANGE;
             } else {
-                const int r = 8 * u + (lane >> 3), c = (lane & 7) ^ (lane >> 3);
-                kk[0] = 8 * c;
+                const int r = u * (512 / GK) + lane / (GK / 8), c = (lane % (GK / 8)) ^ chunk_key<GK>(r);
+                kk[0] = 8 * c;                       // (the key repeats every unit: one chunk per lane)
                 voff[i] = row0 + r < rows ? (unsigned)(r * ld_ * 2 + 16 * c) : OUT_OF_RANGE;
             }
         }
@@ -163,9 +171,9 @@ struct TileLoader {
 };
 
 // Fragments of one operand for the wave: NT tiles of 16 rows starting at row w0 (a multiple of 16 NT) of the LDS tile
-template <int R, int NT, bool T>
+template <int R, int NT, bool T, int GK>
 struct TileReader {
-    unsigned addr[T ? NT : 2];
+    unsigned addr[T ? NT : GK / 32];
     __device__ __forceinline__ void init(int w0, int lane) {
         const int r = lane & 15, q = lane >> 4;
         if constexpr (T) {
@@ -175,7 +183,7 @@ struct TileReader {
             for (int t = 0; t < NT; ++t) addr[t] = (unsigned)((8 * q + (r >> 2)) * 2 * R + (((w0 / 16 + t) ^ f) * 32) + 8 * (r & 3));
         } else {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) addr[h] = (unsigned)((w0 + r) * 128 + (((4 * h + q) ^ (r & 7)) * 16));
+            for (int h = 0; h < GK / 32; ++h) addr[h] = (unsigned)((w0 + r) * 2 * GK + (((4 * h + q) ^ chunk_key<GK>(r)) * 16));
         }
     }
     // fragment of tile t, k half h (32 k)
@@ -186,7 +194,7 @@ struct TileReader {
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(lds_ptr)(p + 4 * 2 * R));
             return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
-            return *(const bf16x8*)(tile + addr[h] + t * 2048);
+            return *(const bf16x8*)(tile + addr[h] + t * (32 * GK));
         }
     }
 };
@@ -262,11 +270,11 @@ __device__ __forceinline__ void tile_store(const TileArgs& p, const f32x4 (&acc)
     }
 }
 
-template <int BM, int BN, int WM, int WN, bool AT, bool BT, int NSTAGE, bool PIPE, typename T, bool PART>
+template <int BM, int BN, int WM, int WN, bool AT, bool BT, int GK, int NSTAGE, bool PIPE, typename T, bool PART>
 __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(TileArgs p) {
     constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, MT = WTM / 16, NT = WTN / 16;
     constexpr int STAGE = (BM + BN) * GK * 2;
-    constexpr int U = (BM + BN) / 8 / NW;                     // DMA instructions per wave and step
+    constexpr int U = (BM + BN) * GK / 512 / NW;              // DMA instructions per wave and step
     static_assert(epilogue_bytes(NW, WTN) <= NSTAGE * STAGE, "the epilogue reuses the operand stages");
     extern __shared__ __align__(1024) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -276,12 +284,12 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(TileArgs p) {
     const int n0 = tn * BN;
     const int wm = (wave / WN) * WTM, wn = (wave % WN) * WTN;
 
-    TileLoader<BM, NW, AT> la;
-    TileLoader<BN, NW, BT> lb;
+    TileLoader<BM, NW, AT, GK> la;
+    TileLoader<BN, NW, BT, GK> lb;
     la.init((const bf16_t*)p.a, p.lda, m0, p.M, wave, lane);
     lb.init((const bf16_t*)p.b, p.ldb, n0, p.N, wave, lane);
-    TileReader<BM, MT, AT> ra;
-    TileReader<BN, NT, BT> rb;
+    TileReader<BM, MT, AT, GK> ra;
+    TileReader<BN, NT, BT, GK> rb;
     ra.init(wm, lane);
     rb.init(wn, lane);
 
@@ -304,8 +312,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(TileArgs p) {
         at_b += inc_b;
     };
     auto request = [&](int i) {
-        if (i < TileLoader<BM, NW, AT>::UNITS) la.issue(i, rsa, klim, dst, wave);
-        else lb.issue(i - TileLoader<BM, NW, AT>::UNITS, rsb, klim, dst + BM * GK * 2, wave);
+        if (i < TileLoader<BM, NW, AT, GK>::UNITS) la.issue(i, rsa, klim, dst, wave);
+        else lb.issue(i - TileLoader<BM, NW, AT, GK>::UNITS, rsb, klim, dst + BM * GK * 2, wave);
     };
     auto issue = [&](int buf) {
         step_setup(buf);
@@ -371,11 +379,15 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(TileArgs p) {
             issue(wbuf);
             wbuf = wbuf + 1 == NSTAGE ? 0 : wbuf + 1;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < GK / 32; ++h) {
+                const unsigned char* ta = lds + buf * STAGE;
+                const unsigned char* tb = ta + BM * GK * 2;
 #pragma unroll
-                for (int i = 0; i < MT; ++i) read(h, buf, i);
+                for (int i = 0; i < MT; ++i) fa[0][i] = ra.get(ta, i, h);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) multiply(h, i);
+                for (int j = 0; j < NT; ++j) fb[0][j] = rb.get(tb, j, h);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) multiply(0, i);
             }
             buf = buf + 1 == NSTAGE ? 0 : buf + 1;
         }
@@ -442,9 +454,7 @@ __device__ __forceinline__ void split3(float x0, float x1, unsigned& hi, unsigne
     lo = pack_bf2(r0 - __builtin_bit_cast(float, mid << 16), r1 - __builtin_bit_cast(float, mid & 0xffff0000u));
 }
 
-// R x 32 of an operand: 256 threads, chunks of 8 values.  LDS planes of bf16: along k 64-byte rows of four 16-byte chunks, chunk c
-// of row r at c ^ g(r / 4 % 4) with g = 0, 2, 3, 1 (the four lane groups of a ds_read_b128 each hit sixteen different chunks); across k
-// as in TileLoader.
+// R x 32 of an operand: 256 threads, chunks of 8 values, LDS planes of bf16 laid out as TileLoader's
 template <typename E, int R, bool T>
 struct StagedOperand {
     static constexpr int P = sizeof(E) == 4 ? 3 : 1, CH = R / 64, CPR = R / 8, PLANE = R * SK * 2;
@@ -464,17 +474,23 @@ struct StagedOperand {
                 for (int h = 0; h < (sizeof(E) == 4 ? 2 : 1); ++h) v[i][h] = *(const u32x4_any*)(p + 4 * h);
             } else {
                 const long long left = row < (T ? K : rows) ? (T ? rows : K) - col : 0;          // elements of the chunk that exist
-                if constexpr (sizeof(E) == 4) {
-                    unsigned o[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = j < left ? ((const unsigned*)p)[j] : 0u;
-                    v[i][0] = u32x4{o[0], o[1], o[2], o[3]};
-                    v[i][1] = u32x4{o[4], o[5], o[6], o[7]};
-                } else {
-                    u16x8 o;
+                for (int h = 0; h < (sizeof(E) == 4 ? 2 : 1); ++h) v[i][h] = u32x4{0u, 0u, 0u, 0u};
+                if (left >= 8) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = j < left ? p[j] : (bf16_t)0;
-                    v[i][0] = __builtin_bit_cast(u32x4, o);
+                    for (int h = 0; h < (sizeof(E) == 4 ? 2 : 1); ++h) v[i][h] = *(const u32x4_any*)(p + 4 * h);
+                } else if (left > 0) {                                                           // the operand's last, partial chunk
+                    if constexpr (sizeof(E) == 4) {
+#pragma unroll
+                        for (int j = 0; j < 7; ++j)
+                            if (j < left) v[i][j / 4][j % 4] = ((const unsigned*)p)[j];
+                    } else {
+                        u16x8 o = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                        for (int j = 0; j < 7; ++j)
+                            if (j < left) o[j] = p[j];
+                        v[i][0] = __builtin_bit_cast(u32x4, o);
+                    }
                 }
             }
         }
@@ -488,8 +504,8 @@ struct StagedOperand {
                 const int k = e / CPR, c = e % CPR;
                 at = k * 2 * R + ((((c >> 1) ^ (((k & 3) | ((k >> 3 & 1) << 2)) & (R / 16 - 1))) * 2 + (c & 1)) * 16);
             } else {
-                const int r = e / 4, g = r >> 2 & 3;
-                at = r * 64 + (((e % 4) ^ ((g ^ (g >> 1)) & 1) << 1 ^ (g >> 1)) * 16);
+                const int r = e / 4;
+                at = r * 64 + (((e % 4) ^ chunk_key<SK>(r)) * 16);
             }
             if constexpr (sizeof(E) == 4) {
                 u32x4 o[3];
@@ -519,8 +535,7 @@ struct StagedReader {
 #pragma unroll
             for (int t = 0; t < NT; ++t) addr[t] = (unsigned)((8 * q + (r >> 2)) * 2 * R + (((w0 / 16 + t) ^ f) * 32) + 8 * (r & 3));
         } else {
-            const int g = r >> 2;
-            addr[0] = (unsigned)((w0 + r) * 64 + ((q ^ ((g ^ (g >> 1)) & 1) << 1 ^ (g >> 1)) * 16));
+            addr[0] = (unsigned)((w0 + r) * 64 + ((q ^ chunk_key<SK>(r)) * 16));
         }
     }
     __device__ __forceinline__ bf16x8 get(const unsigned char* plane, int t) const {
@@ -541,20 +556,24 @@ constexpr int staged_lds() {
     return tiles > ep ? tiles : ep;
 }
 
-// B x B tile, four waves of B/2 x B/2; the next step's operands wait in registers while this step's are multiplied
+// B x B tile, four waves of B/2 x B/2; the next D steps' operands wait in registers while this step's are multiplied (a small tile's step
+// is shorter than a memory access)
 template <int B, bool AT, bool BT, typename T, bool PART>
 __global__ __launch_bounds__(256, 2) void gemm_staged_kernel(TileArgs p) {
-    constexpr int WT = B / 2, MT = WT / 16, P = sizeof(T) == 4 ? 3 : 1, PLANE = B * SK * 2;
+    constexpr int WT = B / 2, MT = WT / 16, P = sizeof(T) == 4 ? 3 : 1, PLANE = B * SK * 2, D = B == 64 ? 3 : 1;
     __shared__ __align__(1024) unsigned char lds[staged_lds<B, T>()];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int tm, tn, split;
     tile_of_block(p, tm, tn, split);
     const long long m0 = (long long)tm * B;
     const int n0 = tn * B, wm = (wave >> 1) * WT, wn = (wave & 1) * WT;
-    StagedOperand<T, B, AT> sa;
-    StagedOperand<T, B, BT> sb;
-    sa.base = (const T*)p.a; sa.ld = p.lda; sa.row0 = m0; sa.rows = p.M;
-    sb.base = (const T*)p.b; sb.ld = p.ldb; sb.row0 = n0; sb.rows = p.N;
+    StagedOperand<T, B, AT> sa[D];
+    StagedOperand<T, B, BT> sb[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+        sa[d].base = (const T*)p.a; sa[d].ld = p.lda; sa[d].row0 = m0; sa[d].rows = p.M;
+        sb[d].base = (const T*)p.b; sb[d].ld = p.ldb; sb[d].row0 = n0; sb[d].rows = p.N;
+    }
     StagedReader<B, MT, AT> ra;
     StagedReader<B, MT, BT> rb;
     ra.init(wm, lane);
@@ -569,20 +588,25 @@ __global__ __launch_bounds__(256, 2) void gemm_staged_kernel(TileArgs p) {
             acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
             if constexpr (P == 3) low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-    if (s0 < s1) {
-        sa.load(s0 * SK, p.K, tid);
-        sb.load(s0 * SK, p.K, tid);
-    }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+        if (s0 + d < s1) {
+            sa[d].load((s0 + d) * SK, p.K, tid);
+            sb[d].load((s0 + d) * SK, p.K, tid);
+        }
     unsigned char* const ta = lds;
     unsigned char* const tb = lds + P * PLANE;
-    for (long long s = s0; s < s1; ++s) {
+    for (long long s = s0; s < s1; s += D) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        if (s + d >= s1) break;
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        sa.store(ta, tid);
-        sb.store(tb, tid);
+        sa[d].store(ta, tid);
+        sb[d].store(tb, tid);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s + 1 < s1) {
-            sa.load((s + 1) * SK, p.K, tid);
-            sb.load((s + 1) * SK, p.K, tid);
+        if (s + d + D < s1) {
+            sa[d].load((s + d + D) * SK, p.K, tid);
+            sb[d].load((s + d + D) * SK, p.K, tid);
         }
         bf16x8 fb[P][MT];
 #pragma unroll
@@ -605,6 +629,7 @@ __global__ __launch_bounds__(256, 2) void gemm_staged_kernel(TileArgs p) {
 #pragma unroll
             for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[0][j], fa[0], acc[i][j], 0, 0, 0);
         }
+      }
     }
     if constexpr (P == 3) {
 #pragma unroll

@@ -24,7 +24,7 @@ struct TilePlan { TileKind kind; long long tiles_m; int tiles_n, splits; size_t 
 static TilePlan tile_plan(bool direct, long long M, int N, long long K) {
     TilePlan t;
     auto tiles = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-    const long long steps = (K + (direct ? GK : SK) - 1) / (direct ? GK : SK);
+    const long long steps = (K + (direct ? 64 : SK) - 1) / (direct ? 64 : SK);
     if (direct) t.kind = M <= 32 ? TILE_32 : tiles(256, 256) >= 200 && steps >= 8 ? TILE_256 : TILE_128;
     else t.kind = tiles(128, 128) >= 384 ? STAGED_128 : STAGED_64;
     const int bm = t.kind == TILE_256 ? 256 : t.kind == TILE_32 ? 32 : t.kind == STAGED_64 ? 64 : 128;
@@ -53,11 +53,11 @@ static int join(const TileArgs& p, hipStream_t s) {
     return hip_check(hipGetLastError(), "linear join");
 }
 
-template <int BM, int BN, int WM, int WN, int NSTAGE, bool PIPE, bool AT, bool BT, typename T>
+template <int BM, int BN, int WM, int WN, int GK, int NSTAGE, bool PIPE, bool AT, bool BT, typename T>
 static void tile_go(const TileArgs& p, unsigned grid, hipStream_t s) {
     constexpr size_t lds = (size_t)NSTAGE * (BM + BN) * GK * 2;
-    if (p.splits > 1) hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, NSTAGE, PIPE, T, true>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
-    else hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, NSTAGE, PIPE, T, false>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
+    if (p.splits > 1) hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, GK, NSTAGE, PIPE, T, true>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
+    else hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, GK, NSTAGE, PIPE, T, false>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
 }
 template <int B, bool AT, bool BT, typename T>
 static void staged_go(const TileArgs& p, unsigned grid, hipStream_t s) {
@@ -76,9 +76,9 @@ static int tile_gemm(bool direct, TileArgs& p, float* part, hipStream_t s) {
     const unsigned g = (unsigned)grid;
     if constexpr (sizeof(T) == 2) {
         switch (t.kind) {
-            case TILE_256: tile_go<256, 256, 2, 4, 2, true, AT, BT, T>(p, g, s); break;
-            case TILE_128: tile_go<128, 128, 2, 2, 2, false, AT, BT, T>(p, g, s); break;
-            case TILE_32: tile_go<32, 128, 1, 4, 3, true, AT, BT, T>(p, g, s); break;
+            case TILE_256: tile_go<256, 256, 2, 4, 64, 2, true, AT, BT, T>(p, g, s); break;
+            case TILE_128: tile_go<128, 128, 2, 2, 64, 2, false, AT, BT, T>(p, g, s); break;
+            case TILE_32: tile_go<32, 128, 1, 4, 64, 3, true, AT, BT, T>(p, g, s); break;
             default: break;
         }
     }

@@ -58,7 +58,7 @@ struct ThinArgs {
 template <typename T, int MT>
 __global__ __launch_bounds__(64 * THIN_WAVES) void thin_fwd_kernel(ThinArgs p) {
     typedef typename ThinVec<T>::type vec;
-    constexpr int V = 16 / (int)sizeof(T), STEPS = 64 / (4 * V), AHEAD = MT == 1 ? 4 : 2;      // loads of a chunk of 64 k, chunks in flight
+    constexpr int V = 16 / (int)sizeof(T), STEPS = 64 / (4 * V), AHEAD = sizeof(T) == 4 || MT > 1 ? 2 : 4;      // loads of a chunk of 64 k, chunks in flight
     __shared__ f32x4 red[THIN_WAVES][MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
@@ -79,35 +79,39 @@ __global__ __launch_bounds__(64 * THIN_WAVES) void thin_fwd_kernel(ThinArgs p) {
     f32x4 acc[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int c = c0 + wave; c < c1; c += THIN_WAVES * AHEAD) {
-        vec fw[AHEAD][STEPS], fx[AHEAD][MT][STEPS];
+    // AHEAD chunks of the wave are in flight while one is multiplied; past the split: nothing is loaded or multiplied
+    vec fw[AHEAD][STEPS], fx[AHEAD][MT][STEPS];
+    auto load = [&](int u, int c) {
+        if (c < whole) {
+            const long long k = (long long)c * 64;
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int cu = c + u * THIN_WAVES;
-            if (cu < whole) {
-                const long long k = (long long)cu * 64;
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s) fw[u][s] = thin_load(wr + k + 4 * V * s);
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int s = 0; s < STEPS; ++s) fx[u][i][s] = thin_load(xr[i] + k + 4 * V * s);
-            } else {
-                const long long k = cu < c1 ? (long long)cu * 64 : K, left = K - V * q;      // past the split: zeros
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s) fw[u][s] = thin_load(wr, k + 4 * V * s, left);
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int s = 0; s < STEPS; ++s) fx[u][i][s] = thin_load(xr[i], k + 4 * V * s, left);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
+            for (int s = 0; s < STEPS; ++s) fw[u][s] = thin_load(wr + k + 4 * V * s);
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int s = 0; s < STEPS; ++s) acc[i] = thin_mac(fw[u][s], fx[u][i][s], acc[i]);
+                for (int s = 0; s < STEPS; ++s) fx[u][i][s] = thin_load(xr[i] + k + 4 * V * s);
+        } else if (c < c1) {
+            const long long k = (long long)c * 64, left = K - V * q;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) fw[u][s] = thin_load(wr, k + 4 * V * s, left);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) fx[u][i][s] = thin_load(xr[i], k + 4 * V * s, left);
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) load(u, c0 + wave + u * THIN_WAVES);
+    for (int c = c0 + wave; c < c1; c += THIN_WAVES * AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (c + u * THIN_WAVES >= c1) break;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[i] = thin_mac(fw[u][s], fx[u][i][s], acc[i]);
+            load(u, c + (AHEAD + u) * THIN_WAVES);
+        }
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) red[wave][i][lane] = acc[i];

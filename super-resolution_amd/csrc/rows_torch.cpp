@@ -1,0 +1,322 @@
+// PyTorch side of the row operators (srmi/rows.py): argument checks, output and workspace tensors, and the autograd nodes, over the
+// C ABI of include/srmi.h.  C++ because a row operator can be a 3 us kernel: the same nodes written in Python cost 18 us more in the
+// forward call and as much again in the backward one.
+//
+// Workspaces are tensors of the call: nothing is shared between streams, graphs or threads.
+#include <c10/hip/HIPStream.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <mutex>
+#include <tuple>
+#include <unordered_map>
+
+#include "../../include/srmi.h"
+
+namespace {
+
+using torch::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct SrmiFailure : std::runtime_error {
+    int code;
+    SrmiFailure(int c, const char* msg) : std::runtime_error(msg), code(c) {}
+};
+void check(int rc) {
+    if (rc) throw SrmiFailure(rc, srmi_last_error());
+}
+
+int dtype_code(const Tensor& t) {
+    if (t.scalar_type() == at::kFloat) return SRMI_F32;
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16, "srmi supports float32 and bfloat16 storage, got ", t.scalar_type());
+    return SRMI_BF16;
+}
+void require_cuda(const Tensor& t, const char* what) {
+    TORCH_CHECK(t.is_cuda(), "srmi: ", what, " is on ", t.device(),
+                "; the HIP kernels need a ROCm device tensor (there is deliberately no CPU fallback)");
+}
+void check_like(const Tensor& t, const char* what, at::ScalarType dtype, const Tensor& x, at::IntArrayRef shape) {
+    require_cuda(t, what);
+    TORCH_CHECK_TYPE(t.scalar_type() == dtype, "srmi.rows: ", what, " is ", t.scalar_type(), ", expected ", dtype);
+    TORCH_CHECK_VALUE(t.device() == x.device(), "srmi.rows: ", what, " is on ", t.device(), ", x on ", x.device());
+    TORCH_CHECK_VALUE(t.sizes() == shape, "srmi.rows: ", what, " has shape ", t.sizes(), ", expected ", shape);
+}
+int check_x(const Tensor& x) {
+    require_cuda(x, "input");
+    TORCH_CHECK_VALUE(x.dim() >= 1, "srmi.rows: x needs at least one axis");
+    return dtype_code(x);
+}
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+Tensor workspace(size_t bytes, const Tensor& like) {
+    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+// autograd counts the tensors a node was given, not its optional arguments
+typedef std::optional<Tensor> Opt;
+Opt opt(const Tensor& t) { return t.defined() ? Opt(t) : std::nullopt; }
+void once(const Tensor& dy) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && dy.requires_grad()), "srmi.rows: the backward passes are not differentiable themselves");
+}
+
+// `t` as [rows, last axis]: in place if the last axis is dense and the leading ones walk with one stride, else a copy
+std::tuple<Tensor, int64_t> strided_rows(const Tensor& t) {
+    const int64_t c = t.size(-1);
+    if (t.is_contiguous()) return {t, c};
+    if (t.stride(-1) == 1 || c <= 1) {
+        int64_t ld = -1, n = 1;
+        bool uniform = true;
+        for (int64_t i = t.dim() - 2; i >= 0 && uniform; --i) {
+            if (t.size(i) == 1) continue;
+            if (ld < 0) ld = t.stride(i);
+            else uniform = t.stride(i) == ld * n;
+            n *= t.size(i);
+        }
+        if (ld < 0) ld = c;
+        if (uniform && ld >= std::max<int64_t>(c, 1)) return {t, ld};
+    }
+    return {t.contiguous(), c};
+}
+int align_of(std::initializer_list<const Tensor*> ts) {
+    uintptr_t bits = 0;
+    for (const Tensor* t : ts) bits |= (uintptr_t)ptr(*t);
+    return bits & 15 ? 0 : 16;
+}
+
+// ---- linear --------------------------------------------------------------------------------------------------------------
+size_t linear_ws(const srmi_linear_desc& d, int pass) {
+    size_t n = 0;
+    check(srmi_linear_workspace_bytes(&d, pass, &n));
+    return n;
+}
+
+struct LinearOut { Tensor y, z, x, w; };
+
+LinearOut linear_run(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, int act, float param, bool want_z) {
+    const int64_t N = w.size(0), K = w.size(1);
+    LinearOut o;
+    int64_t ldx, ldw, ldr = 0;
+    std::tie(o.x, ldx) = strided_rows(x);
+    std::tie(o.w, ldw) = strided_rows(w);
+    Tensor rr, bb;
+    if (r.defined()) std::tie(rr, ldr) = strided_rows(r);
+    if (b.defined()) bb = b.contiguous();
+    auto shape = x.sizes().vec();
+    int64_t M = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) M *= shape[i];
+    shape.back() = N;
+    o.y = at::empty(shape, x.options());
+    if (want_z) o.z = at::empty({M, N}, x.options());
+    if (M == 0 || N == 0) return o;
+    TORCH_CHECK_VALUE(N <= INT32_MAX && K <= INT32_MAX, "srmi.rows.linear: more than 2^31 features");
+    const srmi_linear_desc d = {M, (int32_t)N, (int32_t)K, dtype_code(x), act, param, align_of({&o.x, &o.w}), ldx, ldw, ldr, 0};
+    const size_t bytes = linear_ws(d, SRMI_PASS_FWD);
+    const Tensor ws = workspace(bytes, x);
+    check(srmi_linear_fwd(&d, ptr(o.x), ptr(o.w), ptr(bb), ptr(rr), ptr(o.y), ptr(o.z), ptr(ws), bytes, stream_of(x)));
+    return o;
+}
+
+struct LinearFn : torch::autograd::Function<LinearFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Opt& ob, const Opt& orr, int64_t act, double param) {
+        const Tensor b = ob.value_or(Tensor()), r = orr.value_or(Tensor());
+        const bool need = wants_grad(x) || wants_grad(w) || wants_grad(b);
+        // ReLU and LeakyReLU keep the sign of z: without a residual on top y itself is enough for the backward pass
+        const bool by_sign = !r.defined() && (act == SRMI_ACT_RELU || (act == SRMI_ACT_LRELU && param > 0.0));
+        const bool slope = act != SRMI_ACT_NONE && need;
+        LinearOut o = linear_run(x, w, b, r, (int)act, (float)param, slope && !by_sign);
+        ctx->save_for_backward({wants_grad(w) ? o.x : Tensor(), wants_grad(x) ? o.w : Tensor(), slope ? (by_sign ? o.y : o.z) : Tensor()});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["param"] = param;
+        ctx->saved_data["xshape"] = x.sizes().vec();
+        ctx->saved_data["N"] = w.size(0);
+        ctx->saved_data["K"] = w.size(1);
+        ctx->saved_data["need"] = (int64_t)(wants_grad(x) | wants_grad(w) << 1 | wants_grad(b) << 2 | wants_grad(r) << 3);
+        ctx->saved_data["res"] = (int64_t)(2 + b.defined());                    // the residual's place among the tensors
+        return o.y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Tensor& dy = grads[0];
+        once(dy);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &s = saved[2];
+        const int64_t N = ctx->saved_data["N"].toInt(), K = ctx->saved_data["K"].toInt(), need = ctx->saved_data["need"].toInt();
+        const auto xshape = ctx->saved_data["xshape"].toIntVector();
+        // of the inputs that require a gradient, those that this backward pass was asked for
+        auto asked = [&](int i) { return (need >> i & 1) && ctx->needs_input_grad(i < 3 ? i : ctx->saved_data["res"].toInt()); };
+        Tensor dx, dw, db;
+        if (asked(0) || asked(1) || asked(2)) {
+            const c10::OptionalDeviceGuard guard(dy.device());
+            Tensor dyr;
+            int64_t lddy, ldx = K, ldw = K, M = 1;
+            std::tie(dyr, lddy) = strided_rows(dy);
+            if (x.defined()) ldx = std::get<1>(strided_rows(x));
+            if (w.defined()) ldw = std::get<1>(strided_rows(w));
+            for (size_t i = 0; i + 1 < xshape.size(); ++i) M *= xshape[i];
+            if (asked(0)) dx = at::empty(xshape, dy.options());
+            if (asked(1)) dw = at::empty({N, K}, dy.options());
+            if (asked(2)) db = at::empty({N}, dy.options());
+            const srmi_linear_desc d = {M, (int32_t)N, (int32_t)K, dtype_code(dy), (int32_t)ctx->saved_data["act"].toInt(),
+                                        (float)ctx->saved_data["param"].toDouble(), align_of({&x, &w, &dyr}), ldx, ldw, 0, lddy};
+            const size_t bytes = linear_ws(d, SRMI_PASS_BWD);
+            const Tensor ws = workspace(bytes, dy);
+            check(srmi_linear_bwd(&d, ptr(x), ptr(w), ptr(s), ptr(dyr), ptr(dx), ptr(dw), ptr(db), ptr(ws), bytes, stream_of(dy)));
+        }
+        return {dx, dw, db, asked(3) ? dy : Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor linear(const Tensor& x, const Tensor& w, const Opt& bias, const Opt& residual, int64_t act, double param) {
+    check_x(x);
+    const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+    TORCH_CHECK_VALUE(w.dim() == 2, "srmi.rows.linear: weight must be [out_features, in_features]");
+    check_like(w, "weight", x.scalar_type(), x, w.sizes());
+    TORCH_CHECK_VALUE(x.size(-1) == w.size(1), "srmi.rows.linear: x has ", x.size(-1), " features, weight ", w.sizes());
+    if (b.defined()) check_like(b, "bias", x.scalar_type(), x, {w.size(0)});
+    if (r.defined()) {
+        auto shape = x.sizes().vec();
+        shape.back() = w.size(0);
+        check_like(r, "residual", x.scalar_type(), x, shape);
+    }
+    const c10::OptionalDeviceGuard guard(x.device());
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b) || wants_grad(r)))
+        return LinearFn::apply(x, w, opt(b), opt(r), act, param);
+    return linear_run(x, w, b, r, (int)act, (float)param, false).y;
+}
+
+// ---- layer norm ------------------------------------------------------------------------------------------------------------
+int param_code(const Tensor& w, const Tensor& b) { return w.defined() ? dtype_code(w) : b.defined() ? dtype_code(b) : SRMI_F32; }
+
+std::tuple<Tensor, Tensor, Tensor, int64_t> norm_run(const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool keep) {
+    const int64_t C = x.size(-1), rows = x.numel() / C;
+    auto [xr, ldx] = strided_rows(x);
+    Tensor y = at::empty(x.sizes(), x.options()), stats;
+    if (keep) stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
+    if (rows) {
+        TORCH_CHECK_VALUE(C <= INT32_MAX, "srmi.rows.layer_norm: more than 2^31 features");
+        const Tensor wc = w.defined() ? w.contiguous() : w, bc = b.defined() ? b.contiguous() : b;
+        const srmi_norm_desc d = {rows, (int32_t)C, dtype_code(x), param_code(w, b), (float)eps, ldx, 0};
+        float* st = (float*)ptr(stats);
+        check(srmi_layer_norm_fwd(&d, ptr(xr), ptr(wc), ptr(bc), ptr(y), st, keep ? st + rows : nullptr, stream_of(x)));
+    }
+    return {y, stats, xr, ldx};
+}
+
+struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Opt& ow, const Opt& ob, double eps) {
+        const Tensor w = ow.value_or(Tensor()), b = ob.value_or(Tensor());
+        auto [y, stats, xr, ldx] = norm_run(x, w, b, eps, true);
+        ctx->save_for_backward({xr, w, stats});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["xshape"] = x.sizes().vec();
+        ctx->saved_data["ldx"] = ldx;
+        ctx->saved_data["param"] = (int64_t)param_code(w, b);
+        ctx->saved_data["need"] = (int64_t)(wants_grad(x) | wants_grad(w) << 1 | wants_grad(b) << 2);
+        ctx->saved_data["bias"] = (int64_t)(1 + w.defined());                   // the bias's place among the tensors
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Tensor& dy = grads[0];
+        once(dy);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &xr = saved[0], &stats = saved[2];
+        const Tensor w = saved[1].defined() ? saved[1].contiguous() : saved[1];
+        const auto xshape = ctx->saved_data["xshape"].toIntVector();
+        const int64_t C = xshape.back(), rows = stats.size(1), need = ctx->saved_data["need"].toInt();
+        const int pcode = (int)ctx->saved_data["param"].toInt();
+        auto asked = [&](int i) { return (need >> i & 1) && ctx->needs_input_grad(i < 2 ? i : ctx->saved_data["bias"].toInt()); };
+        const c10::OptionalDeviceGuard guard(dy.device());
+        auto [dyr, lddy] = strided_rows(dy);
+        const auto popt = dy.options().dtype(pcode == SRMI_F32 ? at::kFloat : at::kBFloat16);
+        const Tensor dx = asked(0) ? at::empty(xshape, dy.options()) : Tensor(), dw = asked(1) ? at::empty({C}, popt) : Tensor(),
+                     db = asked(2) ? at::empty({C}, popt) : Tensor();
+        const srmi_norm_desc d = {rows, (int32_t)C, dtype_code(dy), pcode, (float)ctx->saved_data["eps"].toDouble(), ctx->saved_data["ldx"].toInt(), lddy};
+        size_t bytes = 0;
+        if (dw.defined() || db.defined()) check(srmi_layer_norm_workspace_bytes(&d, &bytes));
+        const Tensor ws = workspace(bytes, dy);
+        const float* st = (const float*)ptr(stats);
+        check(srmi_layer_norm_bwd(&d, ptr(xr), ptr(w), st, st + rows, ptr(dyr), ptr(dx), ptr(dw), ptr(db), ptr(ws), bytes, stream_of(dy)));
+        return {dx, dw, db, Tensor()};
+    }
+};
+
+Tensor layer_norm(const Tensor& x, const Opt& weight, const Opt& bias, double eps) {
+    check_x(x);
+    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    const int64_t C = x.size(-1);
+    TORCH_CHECK_VALUE(C > 0, "srmi.rows.layer_norm: the last axis is empty");
+    TORCH_CHECK_VALUE(eps >= 0.0, "srmi.rows.layer_norm: eps must be >= 0");
+    const Tensor& p = w.defined() ? w : b;
+    const at::ScalarType pt = p.defined() && p.scalar_type() == at::kFloat ? at::kFloat : x.scalar_type();
+    if (w.defined()) check_like(w, "weight", pt, x, {C});
+    if (b.defined()) check_like(b, "bias", pt, x, {C});
+    const c10::OptionalDeviceGuard guard(x.device());
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) return LayerNormFn::apply(x, opt(w), opt(b), eps);
+    return std::get<0>(norm_run(x, w, b, eps, false));
+}
+
+// ---- dropout ---------------------------------------------------------------------------------------------------------------
+Tensor dropout_run(const Tensor& x_, const Tensor& residual, double p, uint64_t seed, uint64_t offset, const Tensor& rng) {
+    const Tensor x = x_.contiguous(), r = residual.defined() ? residual.contiguous() : residual;
+    Tensor y = at::empty(x.sizes(), x.options());
+    if (x.numel())
+        check(srmi_dropout(ptr(x), ptr(r), ptr(y), (size_t)x.numel(), dtype_code(x), p, seed, offset, (const uint64_t*)ptr(rng), stream_of(x)));
+    return y;
+}
+
+struct DropoutFn : torch::autograd::Function<DropoutFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Opt& orr, double p, int64_t seed, int64_t offset, const Opt& orng) {
+        const Tensor r = orr.value_or(Tensor()), rng = orng.value_or(Tensor());
+        ctx->save_for_backward({rng});              // an in-place write between the passes would change the mask: torch reports it
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["seed"] = seed;
+        ctx->saved_data["offset"] = offset;
+        ctx->saved_data["need"] = (int64_t)(wants_grad(x) | wants_grad(r) << 1);
+        return dropout_run(x, r, p, (uint64_t)seed, (uint64_t)offset, rng);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Tensor& dy = grads[0];
+        once(dy);
+        const Tensor rng = ctx->get_saved_variables()[0];
+        const int64_t need = ctx->saved_data["need"].toInt();
+        auto asked = [&](int i) { return (need >> i & 1) && ctx->needs_input_grad(i); };
+        const c10::OptionalDeviceGuard guard(dy.device());
+        Tensor dx;
+        if (asked(0))
+            dx = dropout_run(dy, Tensor(), ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(),
+                             (uint64_t)ctx->saved_data["offset"].toInt(), rng);
+        return {dx, asked(1) ? dy : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor dropout(const Tensor& x, const Opt& residual, double p, uint64_t seed, uint64_t offset, const Opt& device_rng) {
+    check_x(x);
+    const Tensor r = residual.value_or(Tensor()), rng = device_rng.value_or(Tensor());
+    TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "srmi.rows.dropout: p must be in [0, 1], got ", p);
+    if (rng.defined()) {
+        check_like(rng, "seed", at::kLong, x, {2});
+        TORCH_CHECK_VALUE(rng.is_contiguous(), "srmi.rows.dropout: the [seed, offset] tensor must be contiguous");
+    }
+    if (r.defined()) check_like(r, "residual", x.scalar_type(), x, x.sizes());
+    const c10::OptionalDeviceGuard guard(x.device());
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(r))) return DropoutFn::apply(x, opt(r), p, (int64_t)seed, (int64_t)offset, opt(rng));
+    return dropout_run(x, r, p, seed, offset, rng);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_rows, m) {
+    py::register_exception_translator([](std::exception_ptr e) {
+        try {
+            if (e) std::rethrow_exception(e);
+        } catch (const SrmiFailure& f) {
+            const py::object type = py::module_::import("srmi._lib").attr("SrmiError");
+            PyErr_SetObject(type.ptr(), type(f.code, f.what()).ptr());
+        }
+    });
+    const auto nogil = py::call_guard<py::gil_scoped_release>();
+    m.def("linear", &linear, nogil);
+    m.def("layer_norm", &layer_norm, nogil);
+    m.def("dropout", &dropout, nogil);
+    m.def("strided_rows", &strided_rows, nogil);
+}

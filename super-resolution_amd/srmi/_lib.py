@@ -223,6 +223,29 @@ def load():
     return lib
 
 
+_ROWS = None
+
+
+def load_rows():
+    """The PyTorch binding of the row operators (csrc/rows_torch.cpp), next to libsrmi.so, whose symbols it uses."""
+    global _ROWS
+    if _ROWS is None:
+        load()
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_rows.so")
+        if not os.path.exists(path):
+            raise SrmiLibraryError(f"{path} not found: build it with `python __graft_entry__.py build` "
+                                   "(or `make -C super-resolution_amd/csrc`); there is no fallback path")
+        from importlib import machinery, util
+        loader = machinery.ExtensionFileLoader("_rows", path)
+        try:
+            mod = util.module_from_spec(util.spec_from_loader("_rows", loader))
+            loader.exec_module(mod)
+        except ImportError as e:
+            raise SrmiLibraryError(f"cannot load {path}: {e}") from e
+        _ROWS = mod
+    return _ROWS
+
+
 def check(rc):
     if rc != 0:
         msg = load().srmi_last_error()
