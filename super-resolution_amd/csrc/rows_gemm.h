@@ -43,16 +43,15 @@ struct TileArgs {
     int act; float act_param;
 };
 
-// act(v + bias) + residual for V columns of one row, stored as T
+// act(v + bias) + residual for V columns of one row, stored as T; z, where wanted, on the way
 template <typename T, int V>
 __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const float* bias, long long m, int n) {
     constexpr bool FAST = sizeof(T) == 2;
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] += bias[j];
-    const bool whole = n + V <= p.N;
     if (p.z) {
         T* z = (T*)p.z + m * p.N + n;
-        if (whole) store_vec<V>(z, v);
+        if (n + V <= p.N) store_vec<V>(z, v);
         else {
 #pragma unroll
             for (int j = 0; j < V; ++j)
@@ -75,11 +74,10 @@ __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const 
 #undef SRMI_ROW_ACT
         default: break;
     }
-    T* y = (T*)p.y + m * p.ldy + n;
     if (p.residual) {
         const T* r = (const T*)p.residual + m * p.ldr + n;
         float q[V];
-        if (whole) load_vec<V>(r, q);
+        if (n + V <= p.N) load_vec<V>(r, q);
         else {
 #pragma unroll
             for (int j = 0; j < V; ++j) q[j] = n + j < p.N ? to_f32(r[j]) : 0.f;
@@ -87,7 +85,8 @@ __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const 
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] += q[j];
     }
-    if (whole) store_vec<V>(y, v);
+    T* y = (T*)p.y + m * p.ldy + n;
+    if (n + V <= p.N) store_vec<V>(y, v);
     else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
@@ -215,7 +214,7 @@ __device__ __forceinline__ void tile_of_block(const TileArgs& p, int& tm, int& t
 }
 
 constexpr int ER = 32;                                // rows of a wave's tile per epilogue pass
-constexpr int epilogue_bytes(int waves, int wtn) { return waves * ER * (wtn + 4) * 4; }
+constexpr int epilogue_bytes(int waves, int wtn) { return waves * ER * (wtn + 4) * 4; }      // reuses the operand stages
 
 // The wave's accumulators (tile at row m0, column n0): split sums as they are, or the finished output
 template <int WTM, int WTN, typename T, bool PART>
@@ -260,9 +259,7 @@ __device__ __forceinline__ void tile_store(const TileArgs& p, const f32x4 (&acc)
                 const int row = it * RPI + lane / LPR;
                 const long long m = m0 + pass * ER + row;
                 float v[8];
-                const f32x4 v0 = *(const f32x4*)(st + row * EP + c), v1 = *(const f32x4*)(st + row * EP + c + 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { v[j] = v0[j]; v[4 + j] = v1[j]; }
+                load_vec<8>(st + row * EP + c, v);
                 if (m < p.M && n < p.N) row_epilogue<T, 8>(p, v, bias, m, n);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -270,12 +267,13 @@ __device__ __forceinline__ void tile_store(const TileArgs& p, const f32x4 (&acc)
     }
 }
 
+// (two waves per SIMD as a bound keeps the accumulators out of the AGPRs, between which and the VGPRs the compiler otherwise moves them
+// every step)
 template <int BM, int BN, int WM, int WN, bool AT, bool BT, int GK, int NSTAGE, bool PIPE, typename T, bool PART>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_tile_kernel(TileArgs p) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(TileArgs p) {
     constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, MT = WTM / 16, NT = WTN / 16;
     constexpr int STAGE = (BM + BN) * GK * 2;
     constexpr int U = (BM + BN) * GK / 512 / NW;              // DMA instructions per wave and step
-    static_assert(epilogue_bytes(NW, WTN) <= NSTAGE * STAGE, "the epilogue reuses the operand stages");
     extern __shared__ __align__(1024) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int tm, tn, split;
@@ -454,48 +452,85 @@ __device__ __forceinline__ void split3(float x0, float x1, unsigned& hi, unsigne
     lo = pack_bf2(r0 - __builtin_bit_cast(float, mid << 16), r1 - __builtin_bit_cast(float, mid & 0xffff0000u));
 }
 
-// R x 32 of an operand: 256 threads, chunks of 8 values, LDS planes of bf16 laid out as TileLoader's
-template <typename E, int R, bool T>
-struct StagedOperand {
-    static constexpr int P = sizeof(E) == 4 ? 3 : 1, CH = R / 64, CPR = R / 8, PLANE = R * SK * 2;
-    u32x4 v[CH][sizeof(E) == 4 ? 2 : 1];
-    const E* base; long long ld, row0, rows;
+// One step's share of a thread: R x 32 of an operand over 256 threads, chunks of 8 values
+template <typename E, int R>
+struct StagedChunks {
+    u32x4 v[R / 64][sizeof(E) == 4 ? 2 : 1];
     static_assert(R % 64 == 0, "whole chunks per thread");
+};
 
-    __device__ __forceinline__ void load(long long k0, long long K, int tid) {
-        const bool inside = row0 + R <= rows && k0 + SK <= K;
+// Where the thread's chunks lie.  load(): a whole step, no tests - rows past the end repeat the last one along k, and across k the last
+// chunk runs over its row's end; what either produces is not stored.  load_last(): the last step of the operand, element by
+// element where a chunk is partial, zeros past K.  NARROW (across k, fewer than 8 columns): a chunk could run past the last row
+// from more than one row up, so every step is loaded that way.  LDS planes of bf16 are laid out as TileLoader's.
+template <typename E, int R, bool T, bool NARROW>
+struct StagedOperand {
+    static constexpr int P = sizeof(E) == 4 ? 3 : 1, H = sizeof(E) == 4 ? 2 : 1, CH = R / 64, CPR = R / 8, PLANE = R * SK * 2;
+    const E* p[CH];                    // of the step that is loaded next
+    long long inc, rows;
+    int k, K, col[CH];                 // k and K from the first step on
+
+    __device__ __forceinline__ void init(const void* base, long long ld, long long row0, long long rows_, long long k0, long long K_, int tid) {
+        rows = rows_; k = 0; K = (int)(K_ - k0 < 0x7fffffff ? K_ - k0 : 0x7fffffff);
+        inc = T ? SK * ld : SK;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int e = tid + 256 * i;
-            const long long row = T ? k0 + e / CPR : row0 + e / 4, col = T ? row0 + 8 * (e % CPR) : k0 + 8 * (e % 4);
-            const E* p = base + row * ld + col;
-            if (inside) {
-#pragma unroll
-                for (int h = 0; h < (sizeof(E) == 4 ? 2 : 1); ++h) v[i][h] = *(const u32x4_any*)(p + 4 * h);
+            long long r = T ? row0 + 8 * (e % CPR) : row0 + e / 4;
+            if (r >= rows) r = T ? (rows - 1) / 8 * 8 : rows - 1;
+            if constexpr (T) {
+                p[i] = (const E*)base + (k0 + e / CPR) * ld + r;
+                col[i] = (int)(rows - r < 8 ? rows - r : 8);                  // columns of the chunk that exist
             } else {
-                const long long left = row < (T ? K : rows) ? (T ? rows : K) - col : 0;          // elements of the chunk that exist
+                p[i] = (const E*)base + r * ld + k0 + 8 * (e % 4);
+            }
+        }
+    }
+    __device__ __forceinline__ void step() {
+        k += SK;
 #pragma unroll
-                for (int h = 0; h < (sizeof(E) == 4 ? 2 : 1); ++h) v[i][h] = u32x4{0u, 0u, 0u, 0u};
-                if (left >= 8) {
+        for (int i = 0; i < CH; ++i) p[i] += inc;
+    }
+    __device__ __forceinline__ void load(StagedChunks<E, R>& c, int tid) {
+        if constexpr (NARROW && T) {
+            load_last(c, tid);
+            step();
+        } else {
 #pragma unroll
-                    for (int h = 0; h < (sizeof(E) == 4 ? 2 : 1); ++h) v[i][h] = *(const u32x4_any*)(p + 4 * h);
-                } else if (left > 0) {                                                           // the operand's last, partial chunk
-                    if constexpr (sizeof(E) == 4) {
+            for (int i = 0; i < CH; ++i)
 #pragma unroll
-                        for (int j = 0; j < 7; ++j)
-                            if (j < left) v[i][j / 4][j % 4] = ((const unsigned*)p)[j];
-                    } else {
-                        u16x8 o = {0, 0, 0, 0, 0, 0, 0, 0};
+                for (int h = 0; h < H; ++h) c.v[i][h] = *(const u32x4_any*)(p[i] + 4 * h);
+            step();
+        }
+    }
+    // `ahead`: steps between the current one and the one to load
+    __device__ __forceinline__ void load_last(StagedChunks<E, R>& c, int tid, int ahead = 0) const {
 #pragma unroll
-                        for (int j = 0; j < 7; ++j)
-                            if (j < left) o[j] = p[j];
-                        v[i][0] = __builtin_bit_cast(u32x4, o);
-                    }
+        for (int i = 0; i < CH; ++i) {
+            const int e = tid + 256 * i, kk = k + ahead * SK + (T ? e / CPR : 8 * (e % 4));
+            const E* q = p[i] + ahead * inc;
+            const int left = T ? (kk < K ? col[i] : 0) : K - kk;
+#pragma unroll
+            for (int h = 0; h < H; ++h) c.v[i][h] = u32x4{0u, 0u, 0u, 0u};
+            if (left >= 8) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) c.v[i][h] = *(const u32x4_any*)(q + 4 * h);
+            } else if (left > 0) {
+                if constexpr (sizeof(E) == 4) {
+#pragma unroll
+                    for (int j = 0; j < 7; ++j)
+                        if (j < left) c.v[i][j / 4][j % 4] = ((const unsigned*)q)[j];
+                } else {
+                    u16x8 o = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 7; ++j)
+                        if (j < left) o[j] = q[j];
+                    c.v[i][0] = __builtin_bit_cast(u32x4, o);
                 }
             }
         }
     }
-    __device__ __forceinline__ void store(unsigned char* tile, int tid) const {
+    static __device__ __forceinline__ void store(const StagedChunks<E, R>& ch, unsigned char* tile, int tid) {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int e = tid + 256 * i;
@@ -511,7 +546,7 @@ struct StagedOperand {
                 u32x4 o[3];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const unsigned q0 = v[i][j >> 1][2 * (j & 1)], q1 = v[i][j >> 1][2 * (j & 1) + 1];
+                    const unsigned q0 = ch.v[i][j >> 1][2 * (j & 1)], q1 = ch.v[i][j >> 1][2 * (j & 1) + 1];
                     unsigned hi, mid, lo;
                     split3(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1), hi, mid, lo);
                     o[0][j] = hi; o[1][j] = mid; o[2][j] = lo;
@@ -519,7 +554,7 @@ struct StagedOperand {
 #pragma unroll
                 for (int t = 0; t < 3; ++t) *(u32x4*)(tile + t * PLANE + at) = o[t];
             } else {
-                *(u32x4*)(tile + at) = v[i][0];
+                *(u32x4*)(tile + at) = ch.v[i][0];
             }
         }
     }
@@ -552,13 +587,13 @@ struct StagedReader {
 
 template <int B, typename T>
 constexpr int staged_lds() {
-    constexpr int tiles = (sizeof(T) == 4 ? 3 : 1) * 2 * B * SK * 2, ep = epilogue_bytes(4, B / 2);
+    constexpr int tiles = (sizeof(T) == 4 ? 3 : 1) * 2 * B * SK * 2 * (B == 64 ? 2 : 1), ep = epilogue_bytes(4, B / 2);
     return tiles > ep ? tiles : ep;
 }
 
 // B x B tile, four waves of B/2 x B/2; the next D steps' operands wait in registers while this step's are multiplied (a small tile's step
 // is shorter than a memory access)
-template <int B, bool AT, bool BT, typename T, bool PART>
+template <int B, bool AT, bool BT, bool NARROW, typename T, bool PART>
 __global__ __launch_bounds__(256, 2) void gemm_staged_kernel(TileArgs p) {
     constexpr int WT = B / 2, MT = WT / 16, P = sizeof(T) == 4 ? 3 : 1, PLANE = B * SK * 2, D = B == 64 ? 3 : 1;
     __shared__ __align__(1024) unsigned char lds[staged_lds<B, T>()];
@@ -567,19 +602,21 @@ __global__ __launch_bounds__(256, 2) void gemm_staged_kernel(TileArgs p) {
     tile_of_block(p, tm, tn, split);
     const long long m0 = (long long)tm * B;
     const int n0 = tn * B, wm = (wave >> 1) * WT, wn = (wave & 1) * WT;
-    StagedOperand<T, B, AT> sa[D];
-    StagedOperand<T, B, BT> sb[D];
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-        sa[d].base = (const T*)p.a; sa[d].ld = p.lda; sa[d].row0 = m0; sa[d].rows = p.M;
-        sb[d].base = (const T*)p.b; sb[d].ld = p.ldb; sb[d].row0 = n0; sb[d].rows = p.N;
-    }
     StagedReader<B, MT, AT> ra;
     StagedReader<B, MT, BT> rb;
     ra.init(wm, lane);
     rb.init(wn, lane);
     const long long ksteps = (p.K + SK - 1) / SK;
-    const long long s0 = ksteps * split / p.splits, s1 = ksteps * (split + 1) / p.splits;
+    const long long s0 = ksteps * split / p.splits;
+    const int nsteps = (int)(ksteps * (split + 1) / p.splits - s0);
+    // whole steps, then the operand's last step if it is this split's
+    const bool tail = nsteps > 0 && s0 + nsteps == ksteps;
+    const int full = nsteps - tail;
+    StagedOperand<T, B, AT, NARROW> sa;
+    StagedOperand<T, B, BT, NARROW> sb;
+    sa.init(p.a, p.lda, m0, p.M, s0 * SK, p.K, tid);
+    sb.init(p.b, p.ldb, n0, p.N, s0 * SK, p.K, tid);
+    StagedChunks<T, B> ca[D], cb[D];
     f32x4 acc[MT][MT], low[P == 3 ? MT : 1][P == 3 ? MT : 1];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -588,26 +625,21 @@ __global__ __launch_bounds__(256, 2) void gemm_staged_kernel(TileArgs p) {
             acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
             if constexpr (P == 3) low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
+    // the last step's chunks come first where registers allow it: their latency would stand alone at the end
+    StagedChunks<T, B> la, lb;
+    if (B == 64 && tail) {
+        sa.load_last(la, tid, full);
+        sb.load_last(lb, tid, full);
+    }
 #pragma unroll
     for (int d = 0; d < D; ++d)
-        if (s0 + d < s1) {
-            sa[d].load((s0 + d) * SK, p.K, tid);
-            sb[d].load((s0 + d) * SK, p.K, tid);
+        if (d < full) {
+            sa.load(ca[d], tid);
+            sb.load(cb[d], tid);
         }
-    unsigned char* const ta = lds;
-    unsigned char* const tb = lds + P * PLANE;
-    for (long long s = s0; s < s1; s += D) {
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        if (s + d >= s1) break;
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        sa[d].store(ta, tid);
-        sb[d].store(tb, tid);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s + d + D < s1) {
-            sa[d].load((s + d + D) * SK, p.K, tid);
-            sb[d].load((s + d + D) * SK, p.K, tid);
-        }
+    constexpr int SET = 2 * P * PLANE;                                  // LDS of one step
+    auto multiply = [&](const unsigned char* ta) {
+        const unsigned char* tb = ta + P * PLANE;
         bf16x8 fb[P][MT];
 #pragma unroll
         for (int t = 0; t < P; ++t)
@@ -629,7 +661,35 @@ __global__ __launch_bounds__(256, 2) void gemm_staged_kernel(TileArgs p) {
 #pragma unroll
             for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[0][j], fa[0], acc[i][j], 0, 0, 0);
         }
-      }
+    };
+    int buf = 0;
+    for (int s = 0; s < full; s += D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            if (s + d >= full) break;
+            // two sets of LDS tiles where they fit (B = 64): a set is written again only after the barrier behind its reads
+            if constexpr (B != 64) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            sa.store(ca[d], lds + buf, tid);
+            sb.store(cb[d], lds + buf + P * PLANE, tid);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (s + d + D < full) {
+                sa.load(ca[d], tid);
+                sb.load(cb[d], tid);
+            }
+            multiply(lds + buf);
+            if constexpr (B == 64) buf ^= SET;
+        }
+    }
+    if (tail) {
+        if constexpr (B != 64) {
+            sa.load_last(la, tid);
+            sb.load_last(lb, tid);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        sa.store(la, lds, tid);
+        sb.store(lb, lds + P * PLANE, tid);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        multiply(lds);
     }
     if constexpr (P == 3) {
 #pragma unroll

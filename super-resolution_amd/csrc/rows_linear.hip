@@ -17,7 +17,7 @@ static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static int up8(int n) { return (n + 7) & ~7; }
 
 // ---- the tile product: shape -> kernel, tile, split --------------------------------------------------------------------------
-enum TileKind { TILE_256, TILE_128, TILE_32, STAGED_128, STAGED_64 };
+enum TileKind { TILE_256, TILE_128, TILE_128_SHORT, TILE_32, STAGED_128, STAGED_64 };
 struct TilePlan { TileKind kind; long long tiles_m; int tiles_n, splits; size_t part_bytes; };
 
 // direct: both operands can be read by the DMA
@@ -25,16 +25,22 @@ static TilePlan tile_plan(bool direct, long long M, int N, long long K) {
     TilePlan t;
     auto tiles = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     const long long steps = (K + (direct ? 64 : SK) - 1) / (direct ? 64 : SK);
-    if (direct) t.kind = M <= 32 ? TILE_32 : tiles(256, 256) >= 200 && steps >= 8 ? TILE_256 : TILE_128;
-    else t.kind = tiles(128, 128) >= 384 ? STAGED_128 : STAGED_64;
+    // bf16 by the length of K, in steps of 64.  256 x 256 tiles, one workgroup per CU: 1300-1400 TFLOP/s at 4096^3, where 128 x 128 reach
+    // 1070, if they fill the chip.  128 x 128 with 32 k per stage keep four workgroups per CU and hide a short K's prologue and
+    // epilogue behind each other: 36864 x 256 -> 1024 in 36 us against 41 with 64 k per stage (two workgroups); those win
+    // from K = 2048 on (4096^3: 128 against 187 us).
+    if (direct) t.kind = M <= 32 ? TILE_32 : steps >= 8 && tiles(256, 256) >= 200 ? TILE_256 : steps >= 32 ? TILE_128 : TILE_128_SHORT;
+    // the larger tile needs half the LDS traffic (190 against 120 TFLOP/s in f32), if it leaves every CU two workgroups of eight steps
+    else t.kind = M >= 8 && N >= 8 && tiles(128, 128) * (steps < 8 ? 1 : steps / 8) >= 512 ? STAGED_128 : STAGED_64;
     const int bm = t.kind == TILE_256 ? 256 : t.kind == TILE_32 ? 32 : t.kind == STAGED_64 ? 64 : 128;
     const int bn = t.kind == TILE_256 ? 256 : t.kind == STAGED_64 ? 64 : 128;
     t.tiles_m = (M + bm - 1) / bm;
     t.tiles_n = (N + bn - 1) / bn;
     t.splits = 1;
     const long long n = t.tiles_m * t.tiles_n;
-    if (n < 256 && n > 0) {
-        const long long s = 512 / n, most = steps / 4;
+    // split K where the tiles leave CUs without work, into as many workgroups as are resident (two per CU, three of the small tiles)
+    if (n > 0 && n <= (t.kind == STAGED_64 ? 384 : 256)) {
+        const long long s = (t.kind == STAGED_64 ? 768 : 512) / n, most = steps / (t.kind == STAGED_128 ? 8 : 4);
         t.splits = (int)(s < most ? (s < 128 ? s : 128) : most);
         if (t.splits < 1) t.splits = 1;
     }
@@ -55,14 +61,14 @@ static int join(const TileArgs& p, hipStream_t s) {
 
 template <int BM, int BN, int WM, int WN, int GK, int NSTAGE, bool PIPE, bool AT, bool BT, typename T>
 static void tile_go(const TileArgs& p, unsigned grid, hipStream_t s) {
-    constexpr size_t lds = (size_t)NSTAGE * (BM + BN) * GK * 2;
+    constexpr size_t stages = (size_t)NSTAGE * (BM + BN) * GK * 2, ep = epilogue_bytes(WM * WN, BN / WN), lds = stages > ep ? stages : ep;
     if (p.splits > 1) hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, GK, NSTAGE, PIPE, T, true>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
     else hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, GK, NSTAGE, PIPE, T, false>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
 }
-template <int B, bool AT, bool BT, typename T>
+template <int B, bool AT, bool BT, bool NARROW, typename T>
 static void staged_go(const TileArgs& p, unsigned grid, hipStream_t s) {
-    if (p.splits > 1) hipLaunchKernelGGL((gemm_staged_kernel<B, AT, BT, T, true>), dim3(grid), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((gemm_staged_kernel<B, AT, BT, T, false>), dim3(grid), dim3(256), 0, s, p);
+    if (p.splits > 1) hipLaunchKernelGGL((gemm_staged_kernel<B, AT, BT, NARROW, T, true>), dim3(grid), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((gemm_staged_kernel<B, AT, BT, NARROW, T, false>), dim3(grid), dim3(256), 0, s, p);
 }
 
 template <bool AT, bool BT, typename T>
@@ -77,13 +83,18 @@ static int tile_gemm(bool direct, TileArgs& p, float* part, hipStream_t s) {
     if constexpr (sizeof(T) == 2) {
         switch (t.kind) {
             case TILE_256: tile_go<256, 256, 2, 4, 64, 2, true, AT, BT, T>(p, g, s); break;
-            case TILE_128: tile_go<128, 128, 2, 2, 64, 2, false, AT, BT, T>(p, g, s); break;
+            case TILE_128: tile_go<128, 128, 2, 2, 64, 2, true, AT, BT, T>(p, g, s); break;
+            case TILE_128_SHORT: tile_go<128, 128, 2, 2, 32, 2, false, AT, BT, T>(p, g, s); break;
             case TILE_32: tile_go<32, 128, 1, 4, 64, 3, true, AT, BT, T>(p, g, s); break;
             default: break;
         }
     }
-    if (t.kind == STAGED_128) staged_go<128, AT, BT, T>(p, g, s);
-    else if (t.kind == STAGED_64) staged_go<64, AT, BT, T>(p, g, s);
+    const bool narrow = (AT && p.M < 8) || (BT && p.N < 8);
+    if (t.kind == STAGED_128) staged_go<128, AT, BT, false, T>(p, g, s);
+    else if (t.kind == STAGED_64 && !narrow) staged_go<64, AT, BT, false, T>(p, g, s);
+    else if constexpr (AT || BT) {
+        if (t.kind == STAGED_64) staged_go<64, AT, BT, true, T>(p, g, s);
+    }
     const int rc = hip_check(hipGetLastError(), "linear product");
     return rc || t.splits == 1 ? rc : join<T>(p, s);
 }
