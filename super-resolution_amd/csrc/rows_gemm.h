@@ -50,30 +50,15 @@ __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const 
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] += bias[j];
     if (p.z) {
-        T* z = (T*)p.z + m * p.N + n;
+        auto* z = (typename KeptZ<T>::type*)p.z + m * p.N + n;
         if (n + V <= p.N) store_vec<V>(z, v);
         else {
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (n + j < p.N) z[j] = from_f32<T>(v[j]);
+                if (n + j < p.N) store_vec<1>(z + j, v + j);
         }
     }
-    switch (p.act) {
-#define SRMI_ROW_ACT(CODE)                                                              \
-    case CODE: {                                                                        \
-        _Pragma("unroll") for (int j = 0; j < V; ++j) v[j] = row_act<FAST>(v[j], CODE, p.act_param); \
-        break;                                                                          \
-    }
-        SRMI_ROW_ACT(SRMI_ACT_RELU)
-        SRMI_ROW_ACT(SRMI_ACT_LRELU)
-        SRMI_ROW_ACT(SRMI_ACT_TANH)
-        SRMI_ROW_ACT(SRMI_ACT_SIGMOID)
-        SRMI_ROW_ACT(SRMI_ACT_GELU)
-        SRMI_ROW_ACT(SRMI_ACT_GELU_TANH)
-        SRMI_ROW_ACT(SRMI_ACT_SILU)
-#undef SRMI_ROW_ACT
-        default: break;
-    }
+    row_act_vec<V, FAST>(v, p.act, p.act_param);
     if (p.residual) {
         const T* r = (const T*)p.residual + m * p.ldr + n;
         float q[V];

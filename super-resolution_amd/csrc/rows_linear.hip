@@ -162,7 +162,7 @@ static bool dma_rows(const srmi_linear_desc& d, int cols, long long ld) {
 // products, before dz is rounded to bf16 (the matrix cores' operand type: half a step of 2^-8 per term of dx and dw, as in y itself).
 struct DzArgs {
     const void* dy; long long lddy;
-    const void* saved;                // dense [M, N]: z, or y where its sign says the same; NULL: act'(z) = 1
+    const void* saved;                // dense [M, N]: KeptZ<T> z, or y where its sign says the same; NULL: act'(z) = 1
     void* dz; int ldz;                // [M, ldz], zeros behind column N; NULL: only the sums are wanted
     float* part;                      // [gridDim.x][N] or NULL
     long long M; int N;
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
     float sum[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[j] = 0.f;
-    const bool whole = c + 8 <= p.N;
+    const bool whole = c + 8 <= p.N, kink = p.act == SRMI_ACT_RELU || p.act == SRMI_ACT_LRELU;
     if (c < p.N) {
         for (long long m = (long long)blockIdx.x * ny + ty; m < p.M; m += (long long)gridDim.x * ny) {
             float g[8];
@@ -190,14 +190,28 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
             }
             if (p.saved) {
                 float z[8];
-                const T* sv = (const T*)p.saved + m * p.N + c;
-                if (whole) load_vec<8>(sv, z);
-                else {
+                const auto* sv = (const typename KeptZ<T>::type*)p.saved + m * p.N + c;
+                if (sizeof(T) == 2 && kink) {
+                    // y (bf16) or z (half) may have been kept: sign bit and zero are the same in both
+                    const short* bits = (const short*)sv;
+                    short h[8];
+                    if (whole) {
+                        const u32x4 q = *(const u32x4_any*)bits;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) z[j] = c + j < p.N ? to_f32(sv[j]) : 0.f;
+                        for (int j = 0; j < 8; ++j) h[j] = (short)(q[j / 2] >> (16 * (j & 1)));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) h[j] = c + j < p.N ? bits[j] : (short)0;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z[j] = (h[j] & 0x7fff) == 0 ? 0.f : h[j] < 0 ? -1.f : 1.f;
+                } else if (whole) {
+                    load_vec<8>(sv, z);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z[j] = c + j < p.N ? (float)sv[j] : 0.f;
                 }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] *= row_act_slope<sizeof(T) == 2>(z[j], p.act, p.act_param);
+                row_slope_vec<8, sizeof(T) == 2>(g, z, p.act, p.act_param);
             }
             if (p.dz) store_vec<8>((T*)p.dz + m * p.ldz + c, g);
 #pragma unroll

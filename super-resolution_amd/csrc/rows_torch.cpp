@@ -107,7 +107,7 @@ LinearOut linear_run(const Tensor& x, const Tensor& w, const Tensor& b, const Te
     for (size_t i = 0; i + 1 < shape.size(); ++i) M *= shape[i];
     shape.back() = N;
     o.y = at::empty(shape, x.options());
-    if (want_z) o.z = at::empty({M, N}, x.options());
+    if (want_z) o.z = at::empty({M, N}, x.options().dtype(x.scalar_type() == at::kBFloat16 ? at::kHalf : at::kFloat));
     if (M == 0 || N == 0) return o;
     TORCH_CHECK_VALUE(N <= INT32_MAX && K <= INT32_MAX, "srmi.rows.linear: more than 2^31 features");
     const srmi_linear_desc d = {M, (int32_t)N, (int32_t)K, dtype_code(x), act, param, align_of({&o.x, &o.w}), ldx, ldw, ldr, 0};

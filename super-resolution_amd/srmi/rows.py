@@ -56,8 +56,8 @@ def linear(x, weight, bias=None, act=None, residual=None):
     an nn.ReLU / LeakyReLU / Tanh / Sigmoid / GELU (either form) / SiLU module.  All tensors share x's dtype (float32: the products
     have float32's accuracy; bfloat16: bf16 operands, f32 sums).
 
-    Training in bfloat16 keeps the pre-activation and forms ``dy * act'(z)`` in bfloat16, one rounding each (the bias gradient
-    sums the products before that rounding)."""
+    Training in bfloat16 rounds ``dy * act'(z)`` to bfloat16 once, as the products' operand (the bias gradient sums it before that
+    rounding); the pre-activation is kept as an IEEE half.  A float32 infinity in x or weight may come out as NaN."""
     _tensor(x, "x")
     _tensor(weight, "weight")
     _tensor(bias, "bias", True)
