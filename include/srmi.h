@@ -524,9 +524,10 @@ int srmi_linear_fwd(const srmi_linear_desc* d, const void* x, const void* w, con
 int srmi_linear_bwd(const srmi_linear_desc* d, const void* x, const void* w, const void* saved, const void* dy, void* dx, void* dw, void* db,
                     void* ws, size_t ws_bytes, void* stream);
 
+#define SRMI_NORM_MAX_C 0x2000000
 typedef struct srmi_norm_desc {
     int64_t rows;
-    int32_t C;                     /* normalised features, >= 1 */
+    int32_t C;                     /* normalised features, 1 .. SRMI_NORM_MAX_C */
     int32_t dtype, param_dtype;    /* of x, y, dy, dx / of weight, bias and their gradients */
     float eps;
     int64_t ldx, lddy;

@@ -50,6 +50,7 @@ static int check_norm(const srmi_norm_desc* d, const char* who) {
         set_error("%s: bad sizes rows=%lld C=%d", who, (long long)d->rows, d->C);
         return SRMI_EINVAL;
     }
+    if (d->C > SRMI_NORM_MAX_C) { set_error("%s: C=%d over 2^25", who, d->C); return SRMI_EUNSUPPORTED; }
     if (!is_dtype(d->dtype) || !is_dtype(d->param_dtype)) { set_error("%s: bad dtype", who); return SRMI_EINVAL; }
     if (!(d->eps >= 0.f)) { set_error("%s: eps must be >= 0", who); return SRMI_EINVAL; }
     if (d->ldx < d->C || d->lddy < 0 || (d->lddy && d->lddy < d->C)) {

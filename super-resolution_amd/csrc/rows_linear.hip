@@ -146,7 +146,7 @@ static int thin_bwd_go(const srmi_linear_desc& d, const float* dz, long long ldd
     }
     if (dw && d.N > 0 && d.K > 0) {
         p.t.M = d.N; p.t.N = d.K; p.t.K = d.M; p.t.y = dw; p.t.ldy = d.K;
-        hipLaunchKernelGGL(thin_wgrad_kernel, dim3((d.K + 255) / 256, (d.N + 63) / 64), dim3(256), 0, s, p, (const float*)x, (long long)d.ldx);
+        hipLaunchKernelGGL(thin_wgrad_kernel, dim3((unsigned)((d.K + 255) / 256) * ((d.N + 63) / 64)), dim3(256), 0, s, p, (const float*)x, (long long)d.ldx);
     }
     return hip_check(hipGetLastError(), "linear bwd");
 }
@@ -164,7 +164,7 @@ struct DzArgs {
     const void* dy; long long lddy;
     const void* saved;                // dense [M, N]: KeptZ<T> z, or y where its sign says the same; NULL: act'(z) = 1
     void* dz; int ldz;                // [M, ldz], zeros behind column N; NULL: only the sums are wanted
-    float* part;                      // [gridDim.x][N] or NULL
+    float* part; void* db;            // partial rows [gridDim.x][N], or the sums themselves (one workgroup per strip); both NULL: not wanted
     long long M; int N;
     int act; float act_param;
     int tx;
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
             for (int j = 0; j < 8; ++j) sum[j] += g[j];
         }
     }
-    if (!p.part) return;
+    if (!p.part && !p.db) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j) red[threadIdx.x * 8 + j] = sum[j];
     __syncthreads();
@@ -226,21 +226,29 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
         for (int q = 1; q < ny; ++q)
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] += red[(q * p.tx + tx) * 8 + j];
+        if (p.db) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (c + j < p.N) p.part[(size_t)blockIdx.x * p.N + c + j] = sum[j];
+            for (int j = 0; j < 8; ++j)
+                if (c + j < p.N) ((T*)p.db)[c + j] = from_f32<T>(sum[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j < p.N) p.part[(size_t)blockIdx.x * p.N + c + j] = sum[j];
+        }
     }
 }
 
-// lanes of 8 columns per row: a power of two; rows of a pass; workgroups of rows = partial rows of db: one per pass up to eight
-// workgroups per CU (36864 x 1024 gelu: 148 us with 256 workgroups, 52 with 1024)
-static int dz_tx(int N) {
+// lanes of 8 columns per row (a power of two), and workgroups of rows = partial rows of db.  One per pass up to eight workgroups per CU
+// (36864 x 1024 gelu: 148 us with 256 workgroups, 52 with 1024); up to 128 rows one workgroup walks them all, 32 at a time, and
+// no second launch adds anything.
+static int dz_tx(long long M, int N) {
     int tx = 1;
-    while (tx < 256 && tx * 8 < N) tx *= 2;
+    while (tx < (M <= 128 ? 8 : 256) && tx * 8 < N) tx *= 2;
     return tx;
 }
 static int dz_slots(long long M, int N) {
-    const int tx = dz_tx(N), strips = N / (tx * 8) + 1;
+    if (M <= 128) return 1;
+    const int tx = dz_tx(M, N), strips = N / (tx * 8) + 1;
     const long long want = (M + 256 / tx - 1) / (256 / tx), most = 2048 / strips < 64 ? 64 : 2048 / strips;
     return (int)(want < 1 ? 1 : want > most ? most : want);
 }
@@ -248,7 +256,7 @@ static int dz_slots(long long M, int N) {
 template <typename T>
 static int dz_launch(DzArgs& p, hipStream_t s) {
     if (p.N == 0) return SRMI_OK;
-    p.tx = dz_tx(p.N);
+    p.tx = dz_tx(p.M, p.N);
     const dim3 grid(dz_slots(p.M, p.N), (p.N + p.tx * 8 - 1) / (p.tx * 8));
     hipLaunchKernelGGL((linear_dz_kernel<T>), grid, dim3(256), 0, s, p);
     return hip_check(hipGetLastError(), "linear dz");
@@ -305,10 +313,12 @@ static int linear_bwd_t(const srmi_linear_desc& d, const void* x, const void* w,
     }
     if (db || (q.dz && d.M > 0)) {
         q.dy = dy; q.lddy = d.lddy; q.saved = own_dz(d) ? saved : nullptr;
-        q.part = db ? part : nullptr;
+        const int slots = dz_slots(d.M, d.N);
+        q.part = db && slots > 1 ? part : nullptr;
+        q.db = db && slots == 1 ? db : nullptr;
         q.M = d.M; q.N = d.N; q.act = d.act; q.act_param = d.act_param;
         if ((rc = dz_launch<T>(q, s))) return rc;
-        if (db && (rc = slot_sum_launch(part, dz_slots(d.M, d.N), d.N, d.N, db, nullptr, sizeof(T) == 2, s))) return rc;
+        if (q.part && (rc = slot_sum_launch(part, slots, d.N, d.N, db, nullptr, sizeof(T) == 2, s))) return rc;
     }
     if (thin_bwd(d)) return thin_bwd_go(d, (const float*)dz, lddz, x, w, dx, dw, s);
     part = (float*)(ws + db_bytes(d) + dz_bytes(d));

@@ -227,8 +227,9 @@ __global__ __launch_bounds__(64 * THIN_WAVES) void thin_dgrad_kernel(ThinArgs p)
 __global__ __launch_bounds__(256) void thin_wgrad_kernel(ThinArgs p, const float* x, long long ldx) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.y * 64, k0 = (blockIdx.x * 4 + wave) * 64;
     const int M = (int)p.t.K, N = (int)p.t.M, K = p.t.N;                     // dw is [N, K]
+    const unsigned kb = (K + 255) / 256;
+    const int n0 = (int)(blockIdx.x / kb) * 64, k0 = (int)(blockIdx.x % kb * 4 + wave) * 64;
     if (k0 >= K) return;
     f32x4 acc[4][4];
 #pragma unroll

@@ -3,6 +3,7 @@
 // forward call and as much again in the backward one.
 //
 // Workspaces are tensors of the call: nothing is shared between streams, graphs or threads.
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
@@ -58,6 +59,20 @@ typedef std::optional<Tensor> Opt;
 Opt opt(const Tensor& t) { return t.defined() ? Opt(t) : std::nullopt; }
 void once(const Tensor& dy) {
     TORCH_CHECK(!(at::GradMode::is_enabled() && dy.requires_grad()), "srmi.rows: the backward passes are not differentiable themselves");
+}
+
+// A backward pass that is captured must not meet a leaf whose accumulation node an eager graph, still alive, made on another stream:
+// autograd would make the capturing stream wait for that one, which ends the capture and with it the process.
+void check_capture(std::initializer_list<const Tensor*> leaves) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto here = c10::hip::getCurrentHIPStream();
+    for (const Tensor* t : leaves) {
+        if (!wants_grad(*t) || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto stream = node ? node->stream() : std::nullopt;
+        TORCH_CHECK(!stream || stream->id() == here.id(),
+                    "srmi.rows: graph capture over a leaf that an eager autograd graph of another stream still refers to; delete that graph first");
+    }
 }
 
 // `t` as [rows, last axis]: in place if the last axis is dense and the leading ones walk with one stride, else a copy
@@ -179,8 +194,10 @@ Tensor linear(const Tensor& x, const Tensor& w, const Opt& bias, const Opt& resi
         check_like(r, "residual", x.scalar_type(), x, shape);
     }
     const c10::OptionalDeviceGuard guard(x.device());
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b) || wants_grad(r)))
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b) || wants_grad(r))) {
+        check_capture({&x, &w, &b, &r});
         return LinearFn::apply(x, w, opt(b), opt(r), act, param);
+    }
     return linear_run(x, w, b, r, (int)act, (float)param, false).y;
 }
 
@@ -251,7 +268,10 @@ Tensor layer_norm(const Tensor& x, const Opt& weight, const Opt& bias, double ep
     if (w.defined()) check_like(w, "weight", pt, x, {C});
     if (b.defined()) check_like(b, "bias", pt, x, {C});
     const c10::OptionalDeviceGuard guard(x.device());
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) return LayerNormFn::apply(x, opt(w), opt(b), eps);
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) {
+        check_capture({&x, &w, &b});
+        return LayerNormFn::apply(x, opt(w), opt(b), eps);
+    }
     return std::get<0>(norm_run(x, w, b, eps, false));
 }
 
@@ -299,7 +319,10 @@ Tensor dropout(const Tensor& x, const Opt& residual, double p, uint64_t seed, ui
     }
     if (r.defined()) check_like(r, "residual", x.scalar_type(), x, x.sizes());
     const c10::OptionalDeviceGuard guard(x.device());
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(r))) return DropoutFn::apply(x, opt(r), p, (int64_t)seed, (int64_t)offset, opt(rng));
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(r))) {
+        check_capture({&x, &r});
+        return DropoutFn::apply(x, opt(r), p, (int64_t)seed, (int64_t)offset, opt(rng));
+    }
     return dropout_run(x, r, p, seed, offset, rng);
 }
 

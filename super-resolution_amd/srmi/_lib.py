@@ -19,6 +19,7 @@ ACT_NONE, ACT_PRELU, ACT_LRELU, ACT_RELU, ACT_TANH, ACT_SIGMOID, ACT_ADD_RELU = 
 ACT_GELU, ACT_GELU_TANH, ACT_SILU = 7, 8, 9        # row operators only
 PASS_FWD, PASS_BWD = 0, 1
 ROWS_MAX = 0xfffffffff
+NORM_MAX_C = 0x2000000
 SHUFFLE_CRD, SHUFFLE_DCR = 0, 1
 
 

@@ -11,9 +11,9 @@ convolutions of this package hand out (logical NCHW, channels_last storage) ente
 Storage is float32 or bfloat16 (one type per call); sums, statistics and activations are float32.  Rows may be strided (a
 channel slice of a wider buffer is read in place); anything whose last axis is not dense is copied first.  Outputs are dense.
 Results do not depend on timing: no atomics, the same call gives the same bits.  Calls may be captured into a HIP graph; nothing is
-kept between calls (workspaces come from torch's allocator, call by call), so graphs and streams share nothing.  As with any torch
-operator, capture a backward pass with leaves that no eager graph still alive has used (``torch.autograd.grad`` avoids the
-accumulation nodes altogether).
+kept between calls (workspaces come from torch's allocator, call by call), so graphs and streams share nothing.  Capturing a
+differentiable call whose leaves an eager autograd graph of another stream still refers to is refused (autograd would end the process in
+the captured backward pass): delete that graph first.
 
 Reference call sites these stand next to: ``nn.Linear`` + LeakyReLU (P/srgan_model.py:57-60), ``nn.BatchNorm2d`` (P/ops.py:24-26).
 The checks, tensors and autograd nodes are in csrc/rows_torch.cpp.  No fallback: CPU tensors raise; no ATen arithmetic.

@@ -55,7 +55,7 @@ def _lin(**kw):
 
 @pytest.mark.parametrize("field,value", [("M", -1), ("N", -1), ("K", -2), ("M", L.ROWS_MAX + 1), ("dtype", 2), ("act", L.ACT_PRELU),
                                          ("act", L.ACT_ADD_RELU), ("act", 10), ("act", -1), ("ldx", 15), ("ldw", 0), ("ldr", 7), ("lddy", 3),
-                                         ("ldr", -8)])
+                                         ("ldr", -8), ("N", (1 << 22) + 1), ("K", (1 << 22) + 1)])
 def test_linear_descriptor_refusals(field, value):
     lib, n = L.load(), C.c_size_t(0)
     d = _lin(**{field: value})
@@ -93,7 +93,8 @@ def test_linear_argument_refusals():
 
 
 @pytest.mark.parametrize("kw", [dict(rows=-1), dict(C=0), dict(C=-4), dict(dtype=5), dict(param_dtype=5), dict(eps=-1.0), dict(eps=float("nan")),
-                                dict(ldx=7), dict(lddy=7), dict(rows=L.ROWS_MAX + 1)])
+                                dict(ldx=7), dict(lddy=7), dict(rows=L.ROWS_MAX + 1),
+                                dict(C=L.NORM_MAX_C + 1, ldx=1 << 30, lddy=1 << 30)])
 def test_norm_descriptor_refusals(kw):
     lib, n = L.load(), C.c_size_t(0)
     d = L.NormDesc(4, 8, L.F32, L.F32, 1e-5, 8, 8)

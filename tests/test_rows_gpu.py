@@ -112,7 +112,9 @@ def check_linear(leaves, dy, dt, act, run=None):
 
 
 SIZES = [(1, 1, 1), (1, 16, 1), (2, 3, 5), (1, 1024, 264), (7, 64, 64), (16, 520, 72), (17, 1030, 33), (33, 2048, 16), (64, 96, 130),
-         (65, 64, 256), (129, 257, 129), (256, 128, 256), (300, 512, 200), (1000, 40, 24), (515, 1152, 384)]
+         (65, 64, 256), (129, 257, 129), (256, 128, 256), (300, 512, 200), (1000, 40, 24), (515, 1152, 384),
+         # fewer than eight columns on one side; K and M beyond 2048 (the longer k loop, sums split over workgroups); around 128 rows
+         (200, 5, 70), (200, 70, 3), (130, 1, 1), (300, 2056, 200), (2500, 72, 40), (128, 33, 77), (127, 64, 64), (70, 4100, 90)]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
@@ -120,6 +122,30 @@ SIZES = [(1, 1, 1), (1, 16, 1), (2, 3, 5), (1, 1024, 264), (7, 64, 64), (16, 520
 def test_linear_sizes(M, K, N, dt):
     leaves, dy = linear_case(M, K, N, dt, "gelu", True, True, 0, 1000 * M + K + N)
     check_linear(leaves, dy, dt, "gelu")
+
+
+def _large(M, K, N, dt, seed):
+    """y, dx, dw and db of act none against 64-bit products on the GPU; same bounds as check_linear"""
+    leaves, dy = linear_case(M, K, N, dt, "none", True, False, 0, seed)
+    x, w, b, _ = leaves
+    y = rows.linear(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    x64, w64, b64, dy64 = (t.detach().double() for t in (x, w, b, dy))
+    s = half_step(dt)
+    wt = w64.t().contiguous()
+    dyt = dy64.t().contiguous()
+    for got, want, mag, n in ((y, x64 @ wt + b64, x64.abs() @ wt.abs() + b64.abs(), K), (dx, dy64 @ w64, dy64.abs() @ w64.abs(), N),
+                              (dw, dyt @ x64, dyt.abs() @ x64.abs(), M), (db, dy64.sum(0), dy64.abs().sum(0), M)):
+        bound = (n + 8) * U * mag * (1 + s) + s * want.abs() + TINY
+        assert float(((got.double() - want).abs() - bound).max()) <= 0
+
+
+# enough tiles for each tile size, none of them whole: 256 x 256 in every product; f32 tiles of 128 with and without split sums
+@pytest.mark.parametrize("M,K,N,dt", [(3590, 520, 3608, "bf16"), (3590, 3608, 520, "bf16"), (616, 3608, 3592, "bf16"), (1100, 2100, 1090, "f32"),
+                                      (24000, 264, 136, "f32"), (2900, 300, 2950, "f32"), (1100, 2101, 1090, "bf16"), (24001, 263, 135, "bf16"),
+                                      (40000, 64, 64, "bf16"), (40000, 64, 64, "f32")])
+def test_linear_large(M, K, N, dt):
+    _large(M, K, N, dt, M + K + N)
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
@@ -236,6 +262,24 @@ def test_linear_partial_gradients():
         args = [t.detach().requires_grad_(j == k) for j, t in enumerate(leaves[:3])]
         (g,) = torch.autograd.grad(rows.linear(*args, act=nn.SiLU()), args[k], dy)
         assert torch.equal(g, full[k])
+
+
+def test_no_second_derivatives():
+    x = torch.randn(5, 8, device=DEV, requires_grad=True)
+    w = torch.randn(6, 8, device=DEV, requires_grad=True)
+    for f in (lambda: rows.linear(x, w, act=nn.Tanh()), lambda: rows.layer_norm(x), lambda: rows.dropout(x, 0.5, 1)):
+        dy = torch.ones_like(f()).requires_grad_()
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad(f(), x, dy, create_graph=True)
+        (g,) = torch.autograd.grad(f(), x, dy)
+        assert not g.requires_grad
+
+
+def test_library_errors_keep_their_type():
+    from srmi import _lib as L
+    x = torch.empty((1, (1 << 22) + 8), device=DEV, dtype=torch.bfloat16)
+    with pytest.raises(L.SrmiError, match="2\\^22"):
+        rows.linear(x, torch.empty((1, (1 << 22) + 8), device=DEV, dtype=torch.bfloat16))
 
 
 def test_linear_same_call_same_bits():
@@ -396,7 +440,7 @@ def philox(n, seed, offset):
 
 
 def test_philox_known_answers():
-    # published test vectors of Philox4x32-10: counter and key of all zeros and of all ones
+    # the published vector of Philox4x32-10 for counter and key zero
     assert [int(v) for v in philox(4, 0, 0)] == [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]
 
 
@@ -567,6 +611,30 @@ def _step(t, p, rng):
     return rows.dropout(h, 0.2, rng, residual=t)
 
 
+def test_training_on_two_streams_at_once():
+    gen = torch.Generator().manual_seed(30)
+    jobs = []
+    for i in range(2):
+        p = _mixer_params(128, 320, "f32", gen)
+        jobs.append((make((2000 + i, 128), "f32", gen).requires_grad_(), p, make((2000 + i, 128), "f32", gen)))
+
+    def job(t, p, dy):
+        y = rows.dropout(rows.linear(rows.linear(rows.layer_norm(t, p["g"], p["b"]), p["w1"], p["b1"], act=nn.GELU()), p["w2"], p["b2"]), 0.2, 1, 2,
+                         residual=t)
+        return [y] + list(torch.autograd.grad(y, [t] + list(p.values()), dy))
+
+    want = [job(*j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(3):
+        got = []
+        for j, s in zip(jobs, streams):
+            with torch.cuda.stream(s):
+                got.append(job(*j))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
 def test_two_streams_at_once():
     gen = torch.Generator().manual_seed(31)
     p = {k: v.detach() for k, v in _mixer_params(256, 512, "bf16", gen).items()}
@@ -623,6 +691,27 @@ def test_two_captured_graphs_replayed_in_turn():
             y = _step(tt, q, rng)
             want = [y] + list(torch.autograd.grad(y, [tt] + list(q.values()), dy))
             assert all(torch.equal(a, b) for a, b in zip(outs, want)), it
+
+
+def test_capture_refuses_leaves_of_a_living_eager_graph():
+    x = torch.randn(80, 64, device=DEV, requires_grad=True)
+    w = torch.randn(48, 64, device=DEV, requires_grad=True)
+    for f in (lambda: rows.linear(x, w), lambda: rows.layer_norm(x), lambda: rows.dropout(x, 0.5, 1)):
+        alive = f()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager autograd graph"):
+            with torch.cuda.graph(graph):
+                f()
+        torch.cuda.synchronize()
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = f()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = y.detach().clone()
+        del y, graph
+        assert torch.equal(got, f().detach())
 
 
 def test_offsets_past_32_bits():
