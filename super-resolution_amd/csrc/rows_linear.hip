@@ -100,15 +100,20 @@ static int tile_gemm(bool direct, TileArgs& p, float* part, hipStream_t s) {
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------------
-constexpr int THIN_ROWS = 64;
-static bool thin_fwd(const srmi_linear_desc& d) { return d.M <= THIN_ROWS; }
+// Forward: where the call then is one launch (bf16, 24 x 1024 -> 4096: 5.4 us against 4.6 + 4.5 of a split tile product and its join;
+// 48 x 1024 -> 1024: 6.6 against 5.5 + 4.0; f32, 24 x 333 -> 515: 5.9 against 7.5 + 3.4, but 48 x 1024 -> 1024 13.3 against 6.0 + 4.1),
+// and for one tile of rows where the operands do not take the DMA (f32, 16 x 18432 -> 1024: 22 + 4 us against 30 + 5; with
+// the DMA, bf16: 11.8 + 4.1 against 10.0 + 5.1; f32, 32 x 4096 -> 4096: 31 + 4 against 26 + 4).
+// f32 backward of one tile of rows: dx and dw of 16 x 18432 -> 1024 20 + 20 us against 39 + 28 of the tile products; of 32 x 4096 ->
+// 4096 51 + 24 against 31 + 25.
+constexpr int THIN_ROWS = 16;
+static bool thin_short(int K) { return K <= 2048; }       // four chunks of 64 for each of a workgroup's eight waves
 static bool thin_bwd(const srmi_linear_desc& d) { return d.M <= THIN_ROWS && d.dtype == SRMI_F32; }
 
-// splits of k: one if a workgroup's eight waves have no more than four chunks of 64 each (then the call is one launch), else as many as
-// give two workgroups per CU without leaving a wave without work
+// splits of k otherwise: as many as give two workgroups per CU without leaving a wave without work
 static int thin_splits(int N, int K) {
     const int tiles = (N + 15) / 16, chunks = (K + 63) / 64;
-    if (chunks <= 32 || tiles == 0) return 1;
+    if (thin_short(K) || tiles == 0) return 1;
     const int s = 512 / tiles, most = chunks / 8;
     return s < 1 ? 1 : s < most ? s : most;
 }
@@ -128,7 +133,7 @@ static int thin_fwd_go(const srmi_linear_desc& d, const void* x, const void* w, 
     const dim3 grid((unsigned)(p.t.tiles_n * p.t.splits)), block(64 * THIN_WAVES);
     if (d.M <= 16) hipLaunchKernelGGL((thin_fwd_kernel<T, 1>), grid, block, 0, s, p);
     else if (d.M <= 32) hipLaunchKernelGGL((thin_fwd_kernel<T, 2>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((thin_fwd_kernel<T, 4>), grid, block, 0, s, p);
+    else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((thin_fwd_kernel<T, 4>), grid, block, 0, s, p);
     const int rc = hip_check(hipGetLastError(), "linear fwd");
     return rc || p.t.splits == 1 ? rc : join<T>(p.t, s);
 }
@@ -139,10 +144,7 @@ static int thin_bwd_go(const srmi_linear_desc& d, const float* dz, long long ldd
     p.x = dz; p.ldx = lddz; p.w = w; p.ldw = d.ldw;
     if (dx && d.M > 0 && d.K > 0) {
         p.t.M = d.M; p.t.N = d.K; p.t.K = d.N; p.t.y = dx; p.t.ldy = d.K;
-        const dim3 grid((d.K + 63) / 64), block(64 * THIN_WAVES);
-        if (d.M <= 16) hipLaunchKernelGGL((thin_dgrad_kernel<1>), grid, block, 0, s, p);
-        else if (d.M <= 32) hipLaunchKernelGGL((thin_dgrad_kernel<2>), grid, block, 0, s, p);
-        else hipLaunchKernelGGL((thin_dgrad_kernel<4>), grid, block, 0, s, p);
+        hipLaunchKernelGGL(thin_dgrad_kernel, dim3((d.K + 63) / 64), dim3(64 * THIN_WAVES), 0, s, p);
     }
     if (dw && d.N > 0 && d.K > 0) {
         p.t.M = d.N; p.t.N = d.K; p.t.K = d.M; p.t.y = dw; p.t.ldy = d.K;
@@ -265,6 +267,9 @@ static int dz_launch(DzArgs& p, hipStream_t s) {
 // ---- entry points' bodies ---------------------------------------------------------------------------------------------------
 static bool own_dz(const srmi_linear_desc& d) { return d.act != SRMI_ACT_NONE; }
 static bool dma_fwd(const srmi_linear_desc& d) { return dma_rows(d, d.K, d.ldx) && dma_rows(d, d.K, d.ldw); }
+static bool thin_fwd(const srmi_linear_desc& d) {
+    return thin_short(d.K) ? d.M <= (d.dtype == SRMI_BF16 ? 64 : 32) : d.M <= THIN_ROWS && !dma_fwd(d);
+}
 static bool dma_dz(const srmi_linear_desc& d) { return own_dz(d) ? d.dtype == SRMI_BF16 : dma_rows(d, d.N, d.lddy); }
 static bool dma_dx(const srmi_linear_desc& d) { return dma_dz(d) && dma_rows(d, d.K, d.ldw); }
 static bool dma_dw(const srmi_linear_desc& d) { return dma_dz(d) && dma_rows(d, d.K, d.ldx); }

@@ -133,36 +133,25 @@ __global__ __launch_bounds__(64 * THIN_WAVES) void thin_fwd_kernel(ThinArgs p) {
     }
 }
 
-// dx[m, k] = sum_n dz[m, n] w[n, k], f32; workgroup: 64 columns, 16 MT rows
-template <int MT>
+// dx[m, k] = sum_n dz[m, n] w[n, k], f32, at most 16 rows; workgroup: 64 columns
 __global__ __launch_bounds__(64 * THIN_WAVES) void thin_dgrad_kernel(ThinArgs p) {
-    constexpr int RED = THIN_WAVES / 2;
-    __shared__ f32x4 red[RED][MT][4][64];
+    __shared__ f32x4 red[THIN_WAVES][4][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
     const int k0 = blockIdx.x * 64, N = (int)p.t.K;                         // contracted: the N of the layer
-    const long long m0 = (long long)blockIdx.y * (16 * MT);
     const float* w = (const float*)p.w;
-    const float* zr[MT];
+    const float* zr = (const float*)p.x + min(r, (int)p.t.M - 1) * p.ldx;
+    f32x4 acc[4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const long long m = m0 + 16 * i + r;
-        zr[i] = (const float*)p.x + (m < p.t.M ? m : p.t.M - 1) * p.ldx;
-    }
-    f32x4 acc[MT][4];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int chunks = (N + 15) / 16;
     const bool whole = k0 + 64 <= p.t.N;
     for (int c = wave; c < chunks; c += 2 * THIN_WAVES) {
-        f32x4 fz[2][MT], fw[2][4];
+        f32x4 fz[2], fw[2][4];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int n = (c + u * THIN_WAVES) * 16 + 4 * q;                // contraction element s of lane group q: n + s
-#pragma unroll
-            for (int i = 0; i < MT; ++i) fz[u][i] = thin_load(zr[i], n, N);
+            fz[u] = thin_load(zr, n, N);
             if (whole) {
 #pragma unroll
                 for (int s = 0; s < 4; ++s) fw[u][s] = thin_load(w + (long long)min(n + s, N - 1) * p.ldw + k0 + 4 * r);
@@ -178,48 +167,31 @@ __global__ __launch_bounds__(64 * THIN_WAVES) void thin_dgrad_kernel(ThinArgs p)
             for (int s = 0; s < 4; ++s) {
                 if (n + s >= N) fw[u][s] = f32x4{0.f, 0.f, 0.f, 0.f};        // the repeated last row, which might not be finite
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[u][s][j], fz[u][i][s], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[u][s][j], fz[u][s], acc[j], 0, 0, 0);
             }
         }
     }
-    // eight accumulators in two halves: waves 4..7 hand theirs to waves 0..3, those add up in wave order
-    if (wave >= RED) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) red[wave - RED][i][j][lane] = acc[i][j];
-    }
+    for (int j = 0; j < 4; ++j) red[wave][j][lane] = acc[j];
     __syncthreads();
-    if (wave < RED) {
+    // element i of tile j of lane (r, q): column k0 + 16 q + 4 i + j of row r; wave i < 4 adds up and stores those four columns
+    const int i = wave;
+    if (i >= 4) return;
+    float v[4];
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+    for (int j = 0; j < 4; ++j) {
+        v[j] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) red[wave][i][j][lane] += acc[i][j];
+        for (int k = 0; k < THIN_WAVES; ++k) v[j] += ((const float*)&red[k][j][lane])[i];
     }
-    __syncthreads();
-    // element i of tile j of lane (r, q): column k0 + 16 q + 4 i + j of row r: 16 consecutive columns a lane
-    for (int e = threadIdx.x; e < MT * 4 * 64; e += 64 * THIN_WAVES) {
-        const int i = e / 256, part = (e >> 6) & 3, ln = e & 63;             // the lane's four columns 4 part .. 4 part + 3
-        float v[4];
+    const int k = k0 + 16 * q + 4 * i;
+    if (r >= p.t.M || k >= p.t.N) return;
+    float* y = (float*)p.t.y + r * p.t.ldy + k;
+    if (k + 4 <= p.t.N) store_vec<4>(y, v);
+    else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[j] = 0.f;
-#pragma unroll
-            for (int k = 0; k < RED; ++k) v[j] += ((const float*)&red[k][i][j][ln])[part];
-        }
-        const long long m = m0 + 16 * i + (ln & 15);
-        const int k = k0 + 16 * (ln >> 4) + 4 * part;
-        if (m < p.t.M && k < p.t.N) {
-            float* y = (float*)p.t.y + m * p.t.ldy + k;
-            if (k + 4 <= p.t.N) store_vec<4>(y, v);
-            else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (k + j < p.t.N) y[j] = v[j];
-            }
-        }
+        for (int j = 0; j < 4; ++j)
+            if (k + j < p.t.N) y[j] = v[j];
     }
 }
 

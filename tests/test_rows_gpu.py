@@ -124,6 +124,15 @@ def test_linear_sizes(M, K, N, dt):
     check_linear(leaves, dy, dt, "gelu")
 
 
+# both sides of 16, 32 and 64 rows, short and long K, whole and ragged chunks of K (K % 8 != 0: rows off the 16-byte boundaries)
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("M", [1, 15, 16, 17, 32, 33, 64, 65])
+@pytest.mark.parametrize("K,N", [(2048, 72), (2047, 33), (4104, 72), (4101, 35)])
+def test_linear_few_rows(M, K, N, dt):
+    leaves, dy = linear_case(M, K, N, dt, "lrelu", True, M % 2 == 0, 0, 10 * M + K)
+    check_linear(leaves, dy, dt, "lrelu")
+
+
 def _large(M, K, N, dt, seed):
     """y, dx, dw and db of act none against 64-bit products on the GPU; same bounds as check_linear"""
     leaves, dy = linear_case(M, K, N, dt, "none", True, False, 0, seed)
