@@ -5,12 +5,14 @@
 // Workspaces are tensors of the call: nothing is shared between streams, graphs or threads.
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <algorithm>
 #include <mutex>
 #include <tuple>
-#include <unordered_map>
+#include <unordered_set>
 
 #include "../../include/srmi.h"
 
@@ -57,21 +59,38 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 // autograd counts the tensors a node was given, not its optional arguments
 typedef std::optional<Tensor> Opt;
 Opt opt(const Tensor& t) { return t.defined() ? Opt(t) : std::nullopt; }
-void once(const Tensor& dy) {
-    TORCH_CHECK(!(at::GradMode::is_enabled() && dy.requires_grad()), "srmi.rows: the backward passes are not differentiable themselves");
+constexpr char ONCE[] = "srmi.rows: the backward passes are not differentiable themselves";
+void once(const Tensor& dy) { TORCH_CHECK(!(at::GradMode::is_enabled() && dy.requires_grad()), ONCE); }
+// A gradient that depends on tensors that require one themselves: under create_graph=True differentiating it raises, instead of
+// passing for a constant.
+void once_more(Tensor& g, bool depends) {
+    if (!g.defined() || !depends || !at::GradMode::is_enabled()) return;
+    torch::autograd::DelayedError node(ONCE, 1);
+    g = node.apply({g.detach().requires_grad_()})[0];
 }
 
 // A backward pass that is captured must not meet a leaf whose accumulation node an eager graph, still alive, made on another stream:
-// autograd would make the capturing stream wait for that one, which ends the capture and with it the process.
-void check_capture(std::initializer_list<const Tensor*> leaves) {
+// autograd would make the capturing stream wait for that one, which ends the capture and with it the process.  Looked for in
+// the operands and in everything they were computed from.
+void check_capture(std::initializer_list<const Tensor*> operands) {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
     const auto here = c10::hip::getCurrentHIPStream();
-    for (const Tensor* t : leaves) {
-        if (!wants_grad(*t) || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        const auto stream = node ? node->stream() : std::nullopt;
-        TORCH_CHECK(!stream || stream->id() == here.id(),
-                    "srmi.rows: graph capture over a leaf that an eager autograd graph of another stream still refers to; delete that graph first");
+    std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+    std::unordered_set<torch::autograd::Node*> seen;
+    auto push = [&](std::shared_ptr<torch::autograd::Node> node) {
+        if (node && seen.insert(node.get()).second) todo.push_back(std::move(node));
+    };
+    for (const Tensor* t : operands)
+        if (wants_grad(*t)) push(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    while (!todo.empty()) {
+        const auto node = todo.back();
+        todo.pop_back();
+        if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) {
+            const auto stream = node->stream();
+            TORCH_CHECK(!stream || stream->id() == here.id(),
+                        "srmi.rows: graph capture over a leaf that an eager autograd graph of another stream still refers to; delete that graph first");
+        }
+        for (const auto& edge : node->next_edges()) push(edge.function);
     }
 }
 
@@ -176,6 +195,10 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
             const size_t bytes = linear_ws(d, SRMI_PASS_BWD);
             const Tensor ws = workspace(bytes, dy);
             check(srmi_linear_bwd(&d, ptr(x), ptr(w), ptr(s), ptr(dyr), ptr(dx), ptr(dw), ptr(db), ptr(ws), bytes, stream_of(dy)));
+            const bool slope = d.act != SRMI_ACT_NONE;
+            once_more(dx, slope || (need & 2));
+            once_more(dw, slope || (need & 1));
+            once_more(db, slope);
         }
         return {dx, dw, db, asked(3) ? dy : Tensor(), Tensor(), Tensor()};
     }
@@ -245,14 +268,16 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
         const c10::OptionalDeviceGuard guard(dy.device());
         auto [dyr, lddy] = strided_rows(dy);
         const auto popt = dy.options().dtype(pcode == SRMI_F32 ? at::kFloat : at::kBFloat16);
-        const Tensor dx = asked(0) ? at::empty(xshape, dy.options()) : Tensor(), dw = asked(1) ? at::empty({C}, popt) : Tensor(),
-                     db = asked(2) ? at::empty({C}, popt) : Tensor();
+        Tensor dx = asked(0) ? at::empty(xshape, dy.options()) : Tensor(), dw = asked(1) ? at::empty({C}, popt) : Tensor();
+        const Tensor db = asked(2) ? at::empty({C}, popt) : Tensor();
         const srmi_norm_desc d = {rows, (int32_t)C, dtype_code(dy), pcode, (float)ctx->saved_data["eps"].toDouble(), ctx->saved_data["ldx"].toInt(), lddy};
         size_t bytes = 0;
         if (dw.defined() || db.defined()) check(srmi_layer_norm_workspace_bytes(&d, &bytes));
         const Tensor ws = workspace(bytes, dy);
         const float* st = (const float*)ptr(stats);
         check(srmi_layer_norm_bwd(&d, ptr(xr), ptr(w), st, st + rows, ptr(dyr), ptr(dx), ptr(dw), ptr(db), ptr(ws), bytes, stream_of(dy)));
+        once_more(dx, true);
+        once_more(dw, need & 1);
         return {dx, dw, db, Tensor()};
     }
 };

@@ -284,6 +284,25 @@ def test_no_second_derivatives():
         assert not g.requires_grad
 
 
+def test_second_derivatives_are_refused_not_zero():
+    # the first derivative under create_graph=True has its value; differentiating it raises although dy itself is a constant
+    x = torch.randn(5, 8, device=DEV, requires_grad=True)
+    w = torch.randn(6, 8, device=DEV, requires_grad=True)
+    v = torch.randn(8, device=DEV, requires_grad=True)
+    for f, ts in ((lambda: rows.linear(x, w, act=nn.Tanh()), (x, w)), (lambda: rows.linear(x, w), (x, w)),
+                  (lambda: rows.layer_norm(x, v), (x, v))):
+        first = torch.autograd.grad(f().sum(), ts)
+        kept = torch.autograd.grad(f().sum(), ts, create_graph=True)
+        for a, b in zip(first, kept):
+            assert torch.equal(a, b.detach())
+            with pytest.raises(RuntimeError, match="not differentiable"):
+                ((b ** 2).sum() + (x ** 2).sum() + (w ** 2).sum()).backward()
+    # nothing to refuse where the gradient is a constant: dx of a product with frozen weights
+    y = rows.linear(x, w.detach())
+    (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    assert not g.requires_grad
+
+
 def test_library_errors_keep_their_type():
     from srmi import _lib as L
     x = torch.empty((1, (1 << 22) + 8), device=DEV, dtype=torch.bfloat16)
@@ -721,6 +740,29 @@ def test_capture_refuses_leaves_of_a_living_eager_graph():
         got = y.detach().clone()
         del y, graph
         assert torch.equal(got, f().detach())
+
+
+def test_capture_refuses_leaves_behind_the_operands():
+    # the leaf that an eager graph still refers to is not an operand itself: an operand was computed from it
+    x = torch.randn(80, 64, device=DEV, requires_grad=True)
+    w = torch.randn(48, 64, device=DEV, requires_grad=True)
+    alive = x * 2.0
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        with torch.cuda.graph(graph):
+            rows.layer_norm(rows.linear((x + 1.0).relu(), w.detach()))
+    torch.cuda.synchronize()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (g,) = torch.autograd.grad(rows.layer_norm(rows.linear((x + 1.0).relu(), w.detach())), x, torch.ones(80, 48, device=DEV))
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    got = g.clone()
+    del graph
+    (want,) = torch.autograd.grad(rows.layer_norm(rows.linear((x + 1.0).relu(), w.detach())), x, torch.ones(80, 48, device=DEV))
+    assert torch.equal(got, want)
 
 
 def test_offsets_past_32_bits():
