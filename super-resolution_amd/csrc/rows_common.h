@@ -83,6 +83,7 @@ template <typename T> struct KeptZ { typedef float type; };
 template <> struct KeptZ<bf16_t> { typedef _Float16 type; };
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+// ReLU and LeakyReLU need to know whether z > 0, of every z: below its least half, 2^-24, a positive z is kept as that.
 __device__ __forceinline__ _Float16 keep_half(float v) { return (_Float16)(fabsf(v) > 65504.f ? copysignf(65504.f, v) : v); }
 template <int V>
 __device__ __forceinline__ void store_vec(_Float16* p, const float* v) {
@@ -106,7 +107,7 @@ __device__ __forceinline__ void load_vec(const _Float16* p, float* v) {
     for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
 }
 
-// exp and division of the epilogues.  Where the result is stored in bf16 (half a step = 2^-9 of the value) the hardware's
+// exp and division of the epilogues.  Where the result is stored in bf16 (half a step = 2^-8 of the value) the hardware's
 // 2^x and reciprocal, a few 2^-23 off, are enough; f32 results take the library's functions.
 template <bool FAST> __device__ __forceinline__ float exp_(float v) {
     if constexpr (FAST) return __builtin_amdgcn_exp2f(v * 1.442695040888963f);
@@ -164,13 +165,13 @@ __device__ __forceinline__ float row_act(float z, int act, float param) {
     }
 }
 
-// d act / d z at z, its limit at infinities.  tanh and sigmoid from e = exp(-k|z|): 1 - t^2 and s (1 - s) would cancel for large |z|.
+// d act / d z at z, its limit at infinities; at the kinks torch's: 0 counts as negative.  tanh and sigmoid from e = exp(-k|z|): 1 - t^2 and s (1 - s) would cancel for large |z|.
 template <bool FAST>
 __device__ __forceinline__ float row_act_slope(float z, int act, float param) {
     z = bounded(z, 100.f);
     switch (act) {
         case SRMI_ACT_RELU: return z <= 0.f ? 0.f : 1.f;
-        case SRMI_ACT_LRELU: return z < 0.f ? param : 1.f;
+        case SRMI_ACT_LRELU: return z > 0.f ? 1.f : param;
         case SRMI_ACT_TANH: {
             const float e = exp_<FAST>(-2.f * fabsf(z)), d = 1.f + e;
             return div_<FAST>(4.f * e, d * d);
@@ -198,6 +199,8 @@ __device__ __forceinline__ float row_act_slope(float z, int act, float param) {
         default: return 1.f;
     }
 }
+
+__device__ __forceinline__ bool is_kink(int act) { return act == SRMI_ACT_RELU || act == SRMI_ACT_LRELU; }
 
 // v = act(v) / g *= act'(z) for V values: one branch on the (uniform) activation, not one per value
 #define SRMI_ROW_ACTS(CASE) \

@@ -51,11 +51,18 @@ __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const 
     for (int j = 0; j < V; ++j) v[j] += bias[j];
     if (p.z) {
         auto* z = (typename KeptZ<T>::type*)p.z + m * p.N + n;
-        if (n + V <= p.N) store_vec<V>(z, v);
+        float k[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) k[j] = v[j];
+        if (sizeof(T) == 2 && is_kink(p.act)) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) k[j] = v[j] > 0.f ? fmaxf(v[j], 0x1p-24f) : v[j];
+        }
+        if (n + V <= p.N) store_vec<V>(z, k);
         else {
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (n + j < p.N) store_vec<1>(z + j, v + j);
+                if (n + j < p.N) store_vec<1>(z + j, k + j);
         }
     }
     row_act_vec<V, FAST>(v, p.act, p.act_param);

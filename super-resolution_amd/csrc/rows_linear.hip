@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
     float sum[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[j] = 0.f;
-    const bool whole = c + 8 <= p.N, kink = p.act == SRMI_ACT_RELU || p.act == SRMI_ACT_LRELU;
+    const bool whole = c + 8 <= p.N, kink = is_kink(p.act);
     if (c < p.N) {
         for (long long m = (long long)blockIdx.x * ny + ty; m < p.M; m += (long long)gridDim.x * ny) {
             float g[8];

@@ -264,6 +264,23 @@ def test_linear_slopes_at_infinity_and_nan():
                 assert act in ("relu", "lrelu") or torch.isnan(db[4])
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("res", [False, True])
+@pytest.mark.parametrize("act,lo", [("relu", 0.0), ("lrelu", 0.2)])
+def test_linear_slopes_at_and_next_to_the_kink(act, lo, res, dt):
+    # z = b where x is zero (the rows a batch is padded with): 0 counts as negative, as in torch; far below a half's least value
+    # the sign of z still decides
+    x = torch.zeros(70, 8, device=DEV, dtype=DT[dt])
+    w = torch.ones(16, 8, device=DEV, dtype=DT[dt])
+    z = [0.0, -0.0, 1e-8, -1e-8, 1e-20, -1e-20, 1e-30, -1e-30] + [0.0] * 8
+    b = torch.tensor(z, device=DEV, dtype=DT[dt]).requires_grad_()
+    r = torch.ones(70, 16, device=DEV, dtype=DT[dt]) if res else None
+    y = rows.linear(x, w, b, act=ACTS[act], residual=r)
+    (db,) = torch.autograd.grad(y, b, torch.ones_like(y))
+    want = torch.tensor([70.0 if v > 0 else 70 * lo for v in z], dtype=torch.float64)
+    torch.testing.assert_close(db.double().cpu(), want, rtol=2.0 ** -8, atol=0)       # sums of 70 in f32, one rounding
+
+
 def test_linear_partial_gradients():
     leaves, dy = linear_case(40, 32, 24, "bf16", "silu", True, False, 0, 12)
     full = torch.autograd.grad(rows.linear(leaves[0], leaves[1], leaves[2], act=nn.SiLU()), leaves[:3], dy)
