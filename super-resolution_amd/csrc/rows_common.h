@@ -53,26 +53,46 @@ __device__ __forceinline__ void load_vec(const bf16_t* p, float* o) {
         }
     }
 }
+// W values to any element's address; `past`: past the caches (below)
+template <int W, typename Q>
+__device__ __forceinline__ void put(Q* p, const Q* v, bool past) {
+    if (past) {
+        asm volatile("");                    // (keeps the compiler from merging the two kinds of store into ordinary ones)
+#pragma unroll
+        for (int i = 0; i < W; ++i) __builtin_nontemporal_store(v[i], p + i);
+        asm volatile("");
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) p[i] = v[i];
+    }
+}
+// An output larger than the eight L2s together is stored past them: nothing of it is there when it is read, and the operands that are read
+// next to it stay.  147456 x 256 bf16 (75 MB): layer norm's backward pass 42 us against 48, dropout 34 + 26 against 42 + 31; a
+// 16384 x 4096 product 450 against 470.  Smaller ones are better left in the caches: 9216 x 1024 (19 MB) of dz written past
+// them cost the product that reads it 16.4 us instead of 14.4, and the kernel that writes it gained nothing.
+constexpr size_t STREAM_BYTES = 32u << 20;
 template <int V>
-__device__ __forceinline__ void store_vec(float* p, const float* v) {
+__device__ __forceinline__ void store_vec(float* p, const float* v, bool past = false) {
     if constexpr (V == 1) {
         p[0] = v[0];
     } else {
+        f32x4_any q[V / 4];
 #pragma unroll
-        for (int i = 0; i < V; i += 4) *(f32x4_any*)(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+        for (int i = 0; i < V / 4; ++i) q[i] = f32x4_any{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        put<V / 4>((f32x4_any*)p, q, past);
     }
 }
 template <int V>
-__device__ __forceinline__ void store_vec(bf16_t* p, const float* v) {
+__device__ __forceinline__ void store_vec(bf16_t* p, const float* v, bool past = false) {
     if constexpr (V == 1) {
         p[0] = f2bf(v[0]);
     } else if constexpr (V == 4) {
-        *(u32x2_any*)p = u32x2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
+        const u32x2_any q = {pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
+        put<1>((u32x2_any*)p, &q, past);
     } else {
-#pragma unroll
-        for (int i = 0; i < V; i += 8)
-            *(u32x4_any*)(p + i) = u32x4{pack_bf2(v[i], v[i + 1]), pack_bf2(v[i + 2], v[i + 3]), pack_bf2(v[i + 4], v[i + 5]),
-                                     pack_bf2(v[i + 6], v[i + 7])};
+        static_assert(V == 8, "one 16-byte store");
+        const u32x4_any q = {pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])};
+        put<1>((u32x4_any*)p, &q, past);
     }
 }
 
@@ -86,16 +106,18 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 // ReLU and LeakyReLU need to know whether z > 0, of every z: below its least half, 2^-24, a positive z is kept as that.
 __device__ __forceinline__ _Float16 keep_half(float v) { return (_Float16)(fabsf(v) > 65504.f ? copysignf(65504.f, v) : v); }
 template <int V>
-__device__ __forceinline__ void store_vec(_Float16* p, const float* v) {
+__device__ __forceinline__ void store_vec(_Float16* p, const float* v, bool past = false) {
     if constexpr (V == 1) {
         p[0] = keep_half(v[0]);
     } else if constexpr (V == 4) {
-        *(u32x2_any*)p = __builtin_bit_cast(u32x2, f16x4{keep_half(v[0]), keep_half(v[1]), keep_half(v[2]), keep_half(v[3])});
+        const u32x2_any q = __builtin_bit_cast(u32x2_any, f16x4{keep_half(v[0]), keep_half(v[1]), keep_half(v[2]), keep_half(v[3])});
+        put<1>((u32x2_any*)p, &q, past);
     } else {
         f16x8 h;
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[j] = keep_half(v[j]);
-        *(u32x4_any*)p = __builtin_bit_cast(u32x4, h);
+        const u32x4_any q = __builtin_bit_cast(u32x4_any, h);
+        put<1>((u32x4_any*)p, &q, past);
     }
 }
 template <int V>

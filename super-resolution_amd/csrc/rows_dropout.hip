@@ -33,8 +33,8 @@ __device__ __forceinline__ void philox4(unsigned long long ctr, unsigned long lo
     o[0] = c0; o[1] = c1; o[2] = c2; o[3] = c3;
 }
 
-// 16 bytes per lane and step: 4 or 8 elements, whole Philox blocks
-template <typename T>
+// 16 bytes per lane and step: 4 or 8 elements, whole Philox blocks.  PAST: y goes past the caches
+template <typename T, bool PAST>
 __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
     const unsigned long long seed = a.rng ? a.rng[0] : a.seed, offset = a.rng ? a.rng[1] : a.offset;
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
             }
         }
         if (whole) {
-            store_vec<V>(y + i, v);
+            store_vec<V>(y + i, v, PAST);
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j)
@@ -79,7 +79,8 @@ static void dropout_go(const DropArgs& a, hipStream_t s) {
     constexpr int V = 16 / (int)sizeof(T);
     long long grid = (a.n + 256 * V - 1) / (256 * V);
     if (grid > 8192) grid = 8192;
-    hipLaunchKernelGGL((dropout_kernel<T>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    if ((size_t)a.n * sizeof(T) > STREAM_BYTES) hipLaunchKernelGGL((dropout_kernel<T, true>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((dropout_kernel<T, false>), dim3((unsigned)grid), dim3(256), 0, s, a);
 }
 
 int dropout(const void* x, const void* residual, void* y, long long n, double p, unsigned long long seed, unsigned long long offset,

@@ -1,13 +1,13 @@
 // The tile product of the row operators: C[m, n] = sum_k A(m, k) B(n, k), bf16 operands, f32 sums on the matrix cores.
 //
-// A workgroup owns a BM x BN tile and walks K in steps of 64.  Operand tiles go straight from memory to LDS
+// A workgroup owns a BM x BN tile and walks K in steps of GK (64, or 32 where K is short).  Operand tiles go straight from memory to LDS
 // (buffer_load_dwordx4 ... lds: no register round trip), up to NSTAGE steps ahead of the step being multiplied, with one barrier
 // per step.  An operand may be stored along k ([row][k], like x and w in x w^T) or across it ([k][row], like w in dz w and both
 // operands of dz^T x): the second kind is read from LDS with the transposing read (ds_read_b64_tr_b16), so that no operand is ever
 // re-laid out in memory.
 //
 // LDS layouts, both free of bank conflicts:
-//   along k    128-byte rows of eight 16-byte chunks, chunk c of row r at position c ^ (r & 7);
+//   along k    rows of GK / 8 16-byte chunks, chunk c of row r at position c ^ chunk_key(r);
 //   across k   one row per k, columns in 32-byte pairs of chunks, pair p of row k at position p ^ ((k & 3) | (k >> 3 & 1) << 2):
 //              the eight k rows that half a wave's transposing read touches fall on eight different pairs.
 // The DMA writes LDS linearly, so the permutation is applied to the global address of each lane.
@@ -41,6 +41,7 @@ struct TileArgs {
     const void* bias; const void* residual; void* y; void* z;
     long long ldr, ldy;                              // z is dense [M, N]
     int act; float act_param;
+    bool past;                                       // y and z go past the caches
 };
 
 // act(v + bias) + residual for V columns of one row, stored as T; z, where wanted, on the way
@@ -58,7 +59,7 @@ __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const 
 #pragma unroll
             for (int j = 0; j < V; ++j) k[j] = v[j] > 0.f ? fmaxf(v[j], 0x1p-24f) : v[j];
         }
-        if (n + V <= p.N) store_vec<V>(z, k);
+        if (n + V <= p.N) store_vec<V>(z, k, p.past);
         else {
 #pragma unroll
             for (int j = 0; j < V; ++j)
@@ -78,7 +79,7 @@ __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const 
         for (int j = 0; j < V; ++j) v[j] += q[j];
     }
     T* y = (T*)p.y + m * p.ldy + n;
-    if (n + V <= p.N) store_vec<V>(y, v);
+    if (n + V <= p.N) store_vec<V>(y, v, p.past);
     else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
@@ -152,7 +153,7 @@ struct TileLoader {
             }
         }
     }
-    // address of step `step` (64 k each), and the distance to the next step
+    // address of step `step` (GK k each), and the distance to the next step
     __device__ __forceinline__ unsigned long long at(long long step) const { return (unsigned long long)(uintptr_t)base + 2 * step * GK * (T ? ld : 1); }
     __device__ __forceinline__ unsigned long long stride() const { return 2 * GK * (unsigned long long)(T ? ld : 1); }
     // request the wave's i-th KiB; klim: k of the step that exist, lds: byte address of the tile

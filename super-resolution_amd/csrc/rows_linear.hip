@@ -38,8 +38,9 @@ static TilePlan tile_plan(bool direct, long long M, int N, long long K) {
     t.tiles_n = (N + bn - 1) / bn;
     t.splits = 1;
     const long long n = t.tiles_m * t.tiles_n;
-    // split K where the tiles leave CUs without work, into as many workgroups as are resident (two per CU, three of the small tiles)
-    if (n > 0 && n <= (t.kind == STAGED_64 ? 384 : 256)) {
+    // split K where the tiles leave CUs without work, into as many workgroups as are resident (two per CU, three of the small tiles; one
+    // of 256 x 256, which are chosen only where they fill the chip)
+    if (t.kind != TILE_256 && n > 0 && n <= (t.kind == STAGED_64 ? 384 : 256)) {
         const long long s = (t.kind == STAGED_64 ? 768 : 512) / n, most = steps / (t.kind == STAGED_128 ? 8 : 4);
         t.splits = (int)(s < most ? (s < 128 ? s : 128) : most);
         if (t.splits < 1) t.splits = 1;
@@ -47,6 +48,9 @@ static TilePlan tile_plan(bool direct, long long M, int N, long long K) {
     t.part_bytes = t.splits > 1 ? up256((size_t)t.splits * M * up8(N) * sizeof(float)) : 0;
     return t;
 }
+
+template <typename T>
+static bool stream_past(long long rows, long long cols) { return (size_t)rows * cols * sizeof(T) > STREAM_BYTES; }
 
 template <typename T>
 static int join(const TileArgs& p, hipStream_t s) {
@@ -62,8 +66,13 @@ static int join(const TileArgs& p, hipStream_t s) {
 template <int BM, int BN, int WM, int WN, int GK, int NSTAGE, bool PIPE, bool AT, bool BT, typename T>
 static void tile_go(const TileArgs& p, unsigned grid, hipStream_t s) {
     constexpr size_t stages = (size_t)NSTAGE * (BM + BN) * GK * 2, ep = epilogue_bytes(WM * WN, BN / WN), lds = stages > ep ? stages : ep;
-    if (p.splits > 1) hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, GK, NSTAGE, PIPE, T, true>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
-    else hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, GK, NSTAGE, PIPE, T, false>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
+    if constexpr (BM < 256) {
+        if (p.splits > 1) {
+            hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, GK, NSTAGE, PIPE, T, true>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, AT, BT, GK, NSTAGE, PIPE, T, false>), dim3(grid), dim3(64 * WM * WN), lds, s, p);
 }
 template <int B, bool AT, bool BT, bool NARROW, typename T>
 static void staged_go(const TileArgs& p, unsigned grid, hipStream_t s) {
@@ -79,6 +88,7 @@ static int tile_gemm(bool direct, TileArgs& p, float* part, hipStream_t s) {
     if (grid > 0x7fffffff) { set_error("linear: more than 2^31 tiles"); return SRMI_EUNSUPPORTED; }
     p.tiles_m = (int)t.tiles_m; p.tiles_n = t.tiles_n; p.splits = t.splits;
     p.part = part; p.part_ld = up8(p.N);
+    p.past = stream_past<T>(p.M, p.N);
     const unsigned g = (unsigned)grid;
     if constexpr (sizeof(T) == 2) {
         switch (t.kind) {
@@ -126,6 +136,7 @@ template <typename T>
 static int thin_fwd_go(const srmi_linear_desc& d, const void* x, const void* w, const TileArgs& t, float* part, hipStream_t s) {
     ThinArgs p;
     p.t = t;
+    p.t.past = stream_past<T>(d.M, d.N);
     p.t.tiles_n = (d.N + 15) / 16;
     p.t.splits = thin_splits(d.N, d.K);
     p.t.part = part; p.t.part_ld = up8(d.N);
@@ -170,6 +181,7 @@ struct DzArgs {
     long long M; int N;
     int act; float act_param;
     int tx;
+    bool past;                        // dz goes past the caches
 };
 
 template <typename T>
@@ -215,7 +227,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
                 }
                 row_slope_vec<8, sizeof(T) == 2>(g, z, p.act, p.act_param);
             }
-            if (p.dz) store_vec<8>((T*)p.dz + m * p.ldz + c, g);
+            if (p.dz) store_vec<8>((T*)p.dz + m * p.ldz + c, g, p.past);
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] += g[j];
         }
@@ -259,6 +271,7 @@ template <typename T>
 static int dz_launch(DzArgs& p, hipStream_t s) {
     if (p.N == 0) return SRMI_OK;
     p.tx = dz_tx(p.M, p.N);
+    p.past = stream_past<T>(p.M, p.ldz);
     const dim3 grid(dz_slots(p.M, p.N), (p.N + p.tx * 8 - 1) / (p.tx * 8));
     hipLaunchKernelGGL((linear_dz_kernel<T>), grid, dim3(256), 0, s, p);
     return hip_check(hipGetLastError(), "linear dz");

@@ -23,6 +23,7 @@ struct NormArgs {
     long long rows;
     int C, p_bf16;
     float eps;
+    bool past;                         // y goes past the caches
 };
 
 template <int LANES>
@@ -42,8 +43,8 @@ __device__ __forceinline__ void load_cols(const T* p, int c, int C, float fill, 
     }
 }
 template <int V, bool TAIL, typename T>
-__device__ __forceinline__ void store_cols(T* p, int c, int C, const float* o) {
-    if (!TAIL || c + V <= C) store_vec<V>(p + c, o);
+__device__ __forceinline__ void store_cols(T* p, int c, int C, const float* o, bool past = false) {
+    if (!TAIL || c + V <= C) store_vec<V>(p + c, o, past);
     else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
                 float o[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) o[j] = v[i * V + j] * rstd * w[i * V + j] + b[i * V + j];
-                store_cols<V, TAIL>(y, c, a.C, o);
+                store_cols<V, TAIL>(y, c, a.C, o, a.past);
             }
         }
         if (a.mean && l == 0) { a.mean[r] = mean; a.rstd[r] = rstd; }
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
                     float o[V];
 #pragma unroll
                     for (int j = 0; j < V; ++j) o[j] = rstd * (g[i * V + j] - c1 - xh[i * V + j] * c2);
-                    store_cols<V, TAIL>(dx, c, a.C, o);
+                    store_cols<V, TAIL>(dx, c, a.C, o, a.past);
                 }
             }
         }
@@ -235,7 +236,7 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
             if (a.b) load_param<V, true>(a.b, a.p_bf16, c, a.C, b);
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = (v[j] - mean) * rstd * w[j] + b[j];
-            store_cols<V, true>(y, c, a.C, v);
+            store_cols<V, true>(y, c, a.C, v, a.past);
         }
         if (a.mean && threadIdx.x == 0) { a.mean[r] = mean; a.rstd[r] = rstd; }
     }
@@ -269,7 +270,7 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
                     if (!pass) { s1 += g[j]; s2 += g[j] * xh[j]; }
                     else g[j] = rstd * (g[j] - c1 - xh[j] * c2);
                 }
-                if (pass) store_cols<V, true>(dx, c, a.C, g);
+                if (pass) store_cols<V, true>(dx, c, a.C, g, a.past);
             }
         }
     }
@@ -402,6 +403,7 @@ static void norm_dispatch(const NormArgs& a, int slots, hipStream_t s) {
 static void fill_args(NormArgs* a, const srmi_norm_desc& d, const void* x, const void* w, const void* b) {
     a->x = x; a->ldx = d.ldx; a->w = w; a->b = b; a->rows = d.rows; a->C = d.C; a->p_bf16 = d.param_dtype == SRMI_BF16; a->eps = d.eps;
     a->dy = nullptr; a->lddy = 0; a->part = nullptr;
+    a->past = (size_t)d.rows * d.C * (d.dtype == SRMI_BF16 ? 2 : 4) > STREAM_BYTES;
 }
 
 int norm_fwd(const srmi_norm_desc& d, const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, hipStream_t s) {
