@@ -98,13 +98,14 @@ __device__ __forceinline__ void store_vec(bf16_t* p, const float* v, bool past =
 
 // What the forward pass keeps of a pre-activation for the backward pass: f32 for f32 rows; for bf16 rows an IEEE half - the same two bytes,
 // but 11 significant bits, so that act'(z) adds nothing visible to the one rounding of dz = dy act'(z) (with bf16 the gradients'
-// error grew from 1.41 to 1.6 times that of one rounding).  Beyond +-65504, where every slope is constant, it is cut.
+// error grew from 1.41 to 1.6 times that of one rounding).  Beyond +-65504 it is an infinity, where every slope has the
+// same limit as at 100.
 template <typename T> struct KeptZ { typedef float type; };
 template <> struct KeptZ<bf16_t> { typedef _Float16 type; };
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 // ReLU and LeakyReLU need to know whether z > 0, of every z: below its least half, 2^-24, a positive z is kept as that.
-__device__ __forceinline__ _Float16 keep_half(float v) { return (_Float16)(fabsf(v) > 65504.f ? copysignf(65504.f, v) : v); }
+__device__ __forceinline__ _Float16 keep_half(float v) { return (_Float16)v; }
 template <int V>
 __device__ __forceinline__ void store_vec(_Float16* p, const float* v, bool past = false) {
     if constexpr (V == 1) {
@@ -175,9 +176,9 @@ __device__ __forceinline__ float row_act(float z, int act, float param) {
         case SRMI_ACT_GELU:
             if constexpr (FAST) {
                 float E, q;
-                const float b = bounded(z, 100.f);
-                normal_tail(b, E, q);
-                return (z < 0.f ? 0.f : z) - fabsf(b) * q;
+                const float t = fabsf(z) > 100.f ? 100.f : fabsf(z);           // (NaN stays)
+                normal_tail(t, E, q);
+                return __builtin_amdgcn_fmed3f(z, 0.f, __builtin_inff()) - t * q;
             } else {
                 return 0.5f * z * erfcf(-0.70710678118654752f * z);
             }
