@@ -9,6 +9,9 @@
 // The backward keeps dw / db of a lane's columns in registers over all the rows its group visits, adds the groups of a
 // workgroup in LDS and stores ONE partial row per workgroup; a second launch adds the partial rows in index order.  No
 // atomics: the same input gives the same bits.
+//
+// 147456 x 256 bf16: forward 26 us (5.8 TB/s), backward 42 us (5.4 TB/s) + 6 for the partial rows; 8281 x 771 f32, rows off the line
+// boundaries: 13.4 and 19.8 us (3.8 TB/s both), + 4.
 #include "rows_common.h"
 
 namespace srmi {
@@ -343,7 +346,7 @@ static int norm_lanes(int C, int dtype) {
 }
 
 // Workgroups of the backward = partial rows of dw / db: eight per CU where there are rows for them (147456 x 256 bf16: 58 us with 512
-// workgroups, 47 with 2048) and the partial rows stay below an eighth of x's bytes.
+// workgroups, 47 with 2048, 42 with dx past the caches) and the partial rows stay below an eighth of x's bytes.
 int norm_slots(const srmi_norm_desc& d) {
     const long long esz = d.dtype == SRMI_BF16 ? 2 : 4, per = 256 / norm_lanes(d.C, d.dtype);
     long long most = d.rows * esz / 64;

@@ -814,3 +814,50 @@ def test_offsets_past_32_bits():
     for i, cc in bits:
         keep = torch.tensor([v >= 2 ** 31 for v in cc])
         assert torch.equal(flat[i:i + 4].float().cpu(), torch.where(keep, 2 * src[i:i + 4].float().cpu(), torch.zeros(4)))
+
+
+def test_backward_offsets_past_32_bits():
+    # y, z and dy of more than 2^32 elements: everything but the last rows is zero, so the gradients are those of the last rows alone
+    k, n, m, far = 8, 520, (1 << 23) + 1000, 3000                            # 4.36e9 elements, 8.7 GB in bf16
+    gen = torch.Generator().manual_seed(43)
+    x = torch.zeros((m, k), dtype=torch.bfloat16, device=DEV)
+    x[-far:] = make((far, k), "bf16", gen)
+    w = make((n, k), "bf16", gen, k ** -0.5)
+    dy = torch.zeros((m, n), dtype=torch.bfloat16, device=DEV)
+    dy[-far:] = make((far, n), "bf16", gen)
+    leaves = x.requires_grad_(), w.requires_grad_()
+    y = rows.linear(*leaves, act=nn.GELU())
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    xs, ws = x[-far:].detach().clone().requires_grad_(), w.detach().clone().requires_grad_()
+    short = rows.linear(xs, ws, act=nn.GELU())
+    dxs, dws = torch.autograd.grad(short, (xs, ws), dy[-far:])
+    assert not y[:-far].any() and not dx[:-far].any()
+    x64, w64, dy64 = x[-far:].detach().double().cpu(), w.detach().double().cpu(), dy[-far:].double().cpu()
+    f, g = act64(x64 @ w64.t(), "gelu")
+    # two roundings of the storage type on either side of a sum (dz, and the result) and the slope's own error, as in check_linear
+    s = 2.0 ** -8
+    dz = dy64 * g
+    edz = s * dz.abs() + dy64.abs() * (0.8 * (2.0 ** -11 * (x64 @ w64.t()).abs() + 2.0 ** -25) + FN["bf16"] * (g.abs() + 0.01)) * (1 + s)
+    for got, near, want, e, c in ((dx[-far:], dxs, dz @ w64, edz @ w64.abs(), n), (dw, dws, dz.t() @ x64, edz.t() @ x64.abs(), far)):
+        bound = (e + (c + 8) * U * 2 * e / s) * (1 + s) + s * want.abs() + TINY
+        assert_within(near, want, bound, "short")
+        assert_within(got, want, bound, "far")
+    del y, dy, dx, short
+    c = 1024
+    x = torch.ones(((1 << 21) + 1000, c), dtype=torch.bfloat16, device=DEV)  # 2.15e9 elements
+    x[-far:] = make((far, c), "bf16", gen)
+    v = make((c,), "bf16", gen).requires_grad_()
+    dy = torch.zeros_like(x)
+    dy[-far:] = make((far, c), "bf16", gen)
+    x.requires_grad_()
+    dx, dv = torch.autograd.grad(rows.layer_norm(x, v), (x, v), dy)
+    xs = x[-far:].detach().clone().requires_grad_()
+    dxs, dvs = torch.autograd.grad(rows.layer_norm(xs, v), (xs, v), dy[-far:])
+    assert torch.equal(dx[-far:], dxs) and not dx[:-far].any()
+    # dv: the same f32 terms in another order, rounded once
+    d64, t64 = dy[-far:].double().cpu(), xs.detach().double().cpu()
+    xh = (t64 - t64.mean(1, keepdim=True)) / torch.sqrt(t64.var(1, unbiased=False, keepdim=True) + 1e-5)
+    want = (d64 * xh).sum(0)
+    bound = (far + c + 64) * U * (d64.abs() * (xh.abs() + 1)).sum(0) * (1 + s) + s * want.abs() + TINY
+    assert_within(dv, want, bound, "far dv")
+    assert_within(dvs, want, bound, "near dv")
