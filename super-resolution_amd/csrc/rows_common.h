@@ -53,9 +53,9 @@ __device__ __forceinline__ void load_vec(const bf16_t* p, float* o) {
         }
     }
 }
-// W values to any element's address; `past`: past the caches (below)
-template <int W, typename Q>
-__device__ __forceinline__ void put(Q* p, const Q* v, bool past) {
+// W times 16 bytes (or 8 bytes) to any element's address; `past`: past the caches (below)
+template <int W>
+__device__ __forceinline__ void put(u32x4_any* p, const u32x4* v, bool past) {
     if (past) {
         asm volatile("");                    // (keeps the compiler from merging the two kinds of store into ordinary ones)
 #pragma unroll
@@ -64,6 +64,15 @@ __device__ __forceinline__ void put(Q* p, const Q* v, bool past) {
     } else {
 #pragma unroll
         for (int i = 0; i < W; ++i) p[i] = v[i];
+    }
+}
+__device__ __forceinline__ void put(u32x2_any* p, const u32x2& v, bool past) {
+    if (past) {
+        asm volatile("");
+        __builtin_nontemporal_store(v, p);
+        asm volatile("");
+    } else {
+        *p = v;
     }
 }
 // An output larger than the eight L2s together is stored past them: nothing of it is there when it is read, and the operands that are read
@@ -76,10 +85,10 @@ __device__ __forceinline__ void store_vec(float* p, const float* v, bool past = 
     if constexpr (V == 1) {
         p[0] = v[0];
     } else {
-        f32x4_any q[V / 4];
+        u32x4 q[V / 4];
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i) q[i] = f32x4_any{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
-        put<V / 4>((f32x4_any*)p, q, past);
+        for (int i = 0; i < V / 4; ++i) q[i] = __builtin_bit_cast(u32x4, f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]});
+        put<V / 4>((u32x4_any*)p, q, past);
     }
 }
 template <int V>
@@ -87,11 +96,10 @@ __device__ __forceinline__ void store_vec(bf16_t* p, const float* v, bool past =
     if constexpr (V == 1) {
         p[0] = f2bf(v[0]);
     } else if constexpr (V == 4) {
-        const u32x2_any q = {pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
-        put<1>((u32x2_any*)p, &q, past);
+        put((u32x2_any*)p, u32x2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])}, past);
     } else {
         static_assert(V == 8, "one 16-byte store");
-        const u32x4_any q = {pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])};
+        const u32x4 q = {pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])};
         put<1>((u32x4_any*)p, &q, past);
     }
 }
@@ -111,13 +119,12 @@ __device__ __forceinline__ void store_vec(_Float16* p, const float* v, bool past
     if constexpr (V == 1) {
         p[0] = keep_half(v[0]);
     } else if constexpr (V == 4) {
-        const u32x2_any q = __builtin_bit_cast(u32x2_any, f16x4{keep_half(v[0]), keep_half(v[1]), keep_half(v[2]), keep_half(v[3])});
-        put<1>((u32x2_any*)p, &q, past);
+        put((u32x2_any*)p, __builtin_bit_cast(u32x2, f16x4{keep_half(v[0]), keep_half(v[1]), keep_half(v[2]), keep_half(v[3])}), past);
     } else {
         f16x8 h;
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[j] = keep_half(v[j]);
-        const u32x4_any q = __builtin_bit_cast(u32x4_any, h);
+        const u32x4 q = __builtin_bit_cast(u32x4, h);
         put<1>((u32x4_any*)p, &q, past);
     }
 }

@@ -5,7 +5,9 @@
 //
 // HBM-bound: x is read once and stays in registers for both moments (the variance is summed from the deviations, not as
 // E[x^2] - mean^2, which cancels), y is written once.  A row belongs to LANES lanes of one wave - 8 for 64 bf16 channels, 64
-// from 512 up - so that every lane moves 16 B and narrow maps still fill the wave.  All statistics are f32.
+// from 512 up - so that every lane moves 16 B and narrow maps still fill the wave; above 2048 columns to the four waves of a
+// workgroup (4096 x 4096 bf16, against re-reading the row: forward 13.5 us / 17, backward 24 + 6 / 56 + 4 with dw in a pass of its
+// own; 16384 x 8192: 136 / 137, 185 + 11 / 294 + 11).  All statistics are f32.
 // The backward keeps dw / db of a lane's columns in registers over all the rows its group visits, adds the groups of a
 // workgroup in LDS and stores ONE partial row per workgroup; a second launch adds the partial rows in index order.  No
 // atomics: the same input gives the same bits.
@@ -29,11 +31,38 @@ struct NormArgs {
     bool past;                         // y goes past the caches
 };
 
+// sums over a row's lanes: part of a wave, or (256) the workgroup, whose four waves meet in `red`
 template <int LANES>
-__device__ __forceinline__ float group_sum(float v) {
+__device__ __forceinline__ float lane_sum(float v) {
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
+}
+struct Sum2 { float a, b; };
+template <int LANES>
+__device__ __forceinline__ Sum2 group_sum2(float a, float b, float (*red)[4]) {
+    if constexpr (LANES <= 64) {
+        return {lane_sum<LANES>(a), lane_sum<LANES>(b)};
+    } else {
+        a = lane_sum<64>(a);
+        b = lane_sum<64>(b);
+        __syncthreads();                     // the sums before these have been read
+        if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = a; red[1][threadIdx.x >> 6] = b; }
+        __syncthreads();
+        return {red[0][0] + red[0][1] + red[0][2] + red[0][3], red[1][0] + red[1][1] + red[1][2] + red[1][3]};
+    }
+}
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v, float* red) {
+    if constexpr (LANES <= 64) {
+        return lane_sum<LANES>(v);
+    } else {
+        v = lane_sum<64>(v);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        return red[0] + red[1] + red[2] + red[3];
+    }
 }
 
 // V columns from c on; TAIL: those past C read as `fill` (rows need no alignment: rows_common.h)
@@ -63,6 +92,7 @@ __device__ __forceinline__ void load_param(const void* p, int p_bf16, int c, int
 template <typename T, int LANES, int ITER, bool TAIL>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
+    __shared__ float red[4];
     const int l = threadIdx.x % LANES;
     const long long ngroups = (long long)gridDim.x * (256 / LANES);
     float w[ITER * V], b[ITER * V];
@@ -91,7 +121,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
 #pragma unroll
             for (int j = 0; j < V; ++j) s += v[i * V + j];
         }
-        const float mean = group_sum<LANES>(s) * inv;
+        const float mean = group_sum<LANES>(s, red) * inv;
         float q = 0.f;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
@@ -103,7 +133,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
                 }
             }
         }
-        const float rstd = 1.f / sqrtf(group_sum<LANES>(q) * inv + a.eps);
+        const float rstd = 1.f / sqrtf(group_sum<LANES>(q, red) * inv + a.eps);
         T* y = (T*)a.y + r * (long long)a.C;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
@@ -123,7 +153,8 @@ template <typename T, int LANES, int ITER, bool TAIL>
 __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
     constexpr int G = 256 / LANES;
-    __shared__ float red[G > 1 ? G : 1][LANES * V];
+    __shared__ float red[G][LANES * V];
+    __shared__ float sums[2][4];
     const int l = threadIdx.x % LANES, gr = threadIdx.x / LANES;
     const long long ngroups = (long long)gridDim.x * G;
     float w[ITER * V], dw[ITER * V], db[ITER * V];
@@ -159,7 +190,8 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
             }
         }
         if (a.y) {
-            const float c1 = group_sum<LANES>(s1) * inv, c2 = group_sum<LANES>(s2) * inv;
+            const Sum2 t = group_sum2<LANES>(s1, s2, sums);
+            const float c1 = t.a * inv, c2 = t.b * inv;
             T* dx = (T*)a.y + r * (long long)a.C;
 #pragma unroll
             for (int i = 0; i < ITER; ++i) {
@@ -197,14 +229,6 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
 }
 
 // ---- rows too wide for registers: a workgroup per row, the row re-read from L1 / L2 ------------------------------------
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = group_sum<64>(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
-}
-
 template <typename T>
 __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
@@ -220,7 +244,7 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
 #pragma unroll
             for (int j = 0; j < V; ++j) s += v[j];
         }
-        const float mean = block_sum(s, red) * inv;
+        const float mean = group_sum<256>(s, red) * inv;
         float q = 0.f;
         for (int c = threadIdx.x * V; c < a.C; c += 256 * V) {
             float v[V];
@@ -229,7 +253,7 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
             for (int j = 0; j < V; ++j)
                 if (c + j < a.C) { v[j] -= mean; q += v[j] * v[j]; }
         }
-        const float rstd = 1.f / sqrtf(block_sum(q, red) * inv + a.eps);
+        const float rstd = 1.f / sqrtf(group_sum<256>(q, red) * inv + a.eps);
         for (int c = threadIdx.x * V; c < a.C; c += 256 * V) {
             float v[V], w[V], b[V];
             load_cols<V, true>(x, c, a.C, 0.f, v);
@@ -248,7 +272,7 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
-    __shared__ float red[4];
+    __shared__ float red[2][4];
     const float inv = 1.f / (float)a.C;
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = (const T*)a.x + r * a.ldx;
@@ -258,7 +282,11 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
         float s1 = 0.f, s2 = 0.f;
         for (int pass = 0; pass < 2; ++pass) {
             float c1 = 0.f, c2 = 0.f;
-            if (pass) { c1 = block_sum(s1, red) * inv; c2 = block_sum(s2, red) * inv; }
+            if (pass) {
+                const Sum2 t = group_sum2<256>(s1, s2, red);
+                c1 = t.a * inv;
+                c2 = t.b * inv;
+            }
             for (int c = threadIdx.x * V; c < a.C; c += 256 * V) {
                 float xh[V], g[V], w[V];
                 load_cols<V, true>(x, c, a.C, 0.f, xh);
@@ -338,11 +366,11 @@ int slot_sum_launch(const float* part, int slots, int n, int n0, void* o0, void*
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-static constexpr int NORM_WIDE = 2048;      // widest row kept in registers: 32 values a lane; the re-reading kernels take what is wider
+static constexpr int NORM_WIDE = 8192;      // widest row kept in registers: 32 values a lane; the re-reading kernels take what is wider
 
 static int norm_lanes(int C, int dtype) {
     const int v = dtype == SRMI_BF16 ? 8 : 4;
-    return C <= 8 * v ? 8 : C <= 16 * v ? 16 : C <= 32 * v ? 32 : 64;
+    return C <= 8 * v ? 8 : C <= 16 * v ? 16 : C <= 32 * v ? 32 : C <= 2048 ? 64 : 256;
 }
 
 // Workgroups of the backward = partial rows of dw / db: eight per CU where there are rows for them (147456 x 256 bf16: 58 us with 512
@@ -350,7 +378,13 @@ static int norm_lanes(int C, int dtype) {
 int norm_slots(const srmi_norm_desc& d) {
     const long long esz = d.dtype == SRMI_BF16 ? 2 : 4, per = 256 / norm_lanes(d.C, d.dtype);
     long long most = d.rows * esz / 64;
-    most = most < 64 ? 64 : most > 2048 ? 2048 : most;
+    // rows of a workgroup's width: two per CU at least (4096 x 4096 bf16: 33 + 5 us with 256 workgroups, 24 + 6 with 512)
+    const int least = per == 1 ? 512 : 64;
+    most = most < least ? least : most > 2048 ? 2048 : most;
+    // wide rows: a workgroup owns a strip of columns of its rows, so fewer slots fill the chip
+    const long long strips = d.C > NORM_WIDE ? (d.C * esz + 4095) / 4096 : 1;
+    if (most > 2048 / strips) most = 2048 / strips;
+    if (most < 1) most = 1;
     const long long want = (d.rows + per - 1) / per;
     return (int)(want < 1 ? 1 : want > most ? most : want);
 }
@@ -378,7 +412,9 @@ static void norm_rows(const NormArgs& a, int slots, hipStream_t s) {
         case 32: norm_go<BWD, T, 32, 1, TAIL>(a, slots, s); return;
         default: break;
     }
-    if (C <= 64 * V) norm_go<BWD, T, 64, 1, TAIL>(a, slots, s);
+    if (C > 4096) norm_go<BWD, T, 256, 32 / V, TAIL>(a, slots, s);
+    else if (C > 2048) norm_go<BWD, T, 256, 16 / V, TAIL>(a, slots, s);
+    else if (C <= 64 * V) norm_go<BWD, T, 64, 1, TAIL>(a, slots, s);
     else if (C <= 128 * V) norm_go<BWD, T, 64, 2, TAIL>(a, slots, s);
     else if (C <= 256 * V) norm_go<BWD, T, 64, 4, TAIL>(a, slots, s);
     else if constexpr (V == 4) norm_go<BWD, T, 64, 8, TAIL>(a, slots, s);

@@ -418,6 +418,13 @@ def test_norm_widths(c, dt):
         check_norm(*norm_case(n, c, dt, dt, True, 0, c + n), dt, dt)
 
 
+# a row per workgroup, and more rows than workgroups: every sum is taken again and again in the same shared memory
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("n,c,pitch", [(1300, 4096, 0), (1100, 2049, 7), (700, 8191, 0), (600, 8192, 8), (2100, 8193, 0)])
+def test_norm_many_wide_rows(n, c, pitch, dt):
+    check_norm(*norm_case(n, c, dt, "f32", True, pitch, n + c), dt, "f32")
+
+
 @pytest.mark.parametrize("dt,pdt", [("bf16", "f32"), ("bf16", "bf16"), ("f32", "f32")])
 @pytest.mark.parametrize("affine", [True, False])
 @pytest.mark.parametrize("pitch", [0, 3, 8])
