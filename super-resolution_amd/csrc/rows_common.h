@@ -8,6 +8,7 @@ typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(bf16_t v) { return bf2f(v); }
+__device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) { return f2bf(v); }
@@ -135,6 +136,17 @@ __device__ __forceinline__ void load_vec(const _Float16* p, float* v) {
     const f16x8 h = __builtin_bit_cast(f16x8, q);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
+}
+
+// The first `left` (1 .. V - 1) of V elements, zeros behind them.  Past the last one it is loaded again: loads that each stand behind a
+// test of their own would wait for one another.
+template <int V, typename T>
+__device__ __forceinline__ void load_some(const T* p, int left, float* o) {
+    T t[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) t[j] = p[min(j, left - 1)];
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = j < left ? to_f32(t[j]) : 0.f;
 }
 
 // exp and division of the epilogues.  Where the result is stored in bf16 (half a step = 2^-8 of the value) the hardware's

@@ -71,10 +71,7 @@ __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const 
         const T* r = (const T*)p.residual + m * p.ldr + n;
         float q[V];
         if (n + V <= p.N) load_vec<V>(r, q);
-        else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) q[j] = n + j < p.N ? to_f32(r[j]) : 0.f;
-        }
+        else load_some<V>(r, p.N - n, q);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] += q[j];
     }
@@ -89,8 +86,13 @@ __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const 
 
 template <typename T, int V>
 __device__ __forceinline__ void load_bias(const TileArgs& p, int n, float* bias) {
+    const T* b = (const T*)p.bias + n;
+    if (p.bias && n + V <= p.N) load_vec<V>(b, bias);
+    else if (p.bias && n < p.N) load_some<V>(b, p.N - n, bias);
+    else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) bias[j] = p.bias && n + j < p.N ? to_f32(((const T*)p.bias)[n + j]) : 0.f;
+        for (int j = 0; j < V; ++j) bias[j] = 0.f;
+    }
 }
 
 // 1 KiB of an operand tile: lane l's 16 bytes go to LDS byte `dst` + 16 l.  (The resource may come from a v_readfirstlane: five

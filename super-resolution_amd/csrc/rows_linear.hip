@@ -198,10 +198,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
             float g[8];
             const T* dy = (const T*)p.dy + m * p.lddy + c;
             if (whole) load_vec<8>(dy, g);
-            else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] = c + j < p.N ? to_f32(dy[j]) : 0.f;
-            }
+            else load_some<8>(dy, p.N - c, g);
             if (p.saved) {
                 float z[8];
                 const auto* sv = (const typename KeptZ<T>::type*)p.saved + m * p.N + c;
@@ -215,15 +212,14 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
                         for (int j = 0; j < 8; ++j) h[j] = (short)(q[j / 2] >> (16 * (j & 1)));
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) h[j] = c + j < p.N ? bits[j] : (short)0;
+                        for (int j = 0; j < 8; ++j) h[j] = bits[min(j, p.N - c - 1)];
                     }
 #pragma unroll
                     for (int j = 0; j < 8; ++j) z[j] = (h[j] & 0x7fff) == 0 ? 0.f : h[j] < 0 ? -1.f : 1.f;
                 } else if (whole) {
                     load_vec<8>(sv, z);
                 } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) z[j] = c + j < p.N ? (float)sv[j] : 0.f;
+                    load_some<8>(sv, p.N - c, z);
                 }
                 row_slope_vec<8, sizeof(T) == 2>(g, z, p.act, p.act_param);
             }
