@@ -5,15 +5,17 @@
 //
 // HBM-bound: x is read once and stays in registers for both moments (the variance is summed from the deviations, not as
 // E[x^2] - mean^2, which cancels), y is written once.  A row belongs to LANES lanes of one wave - 8 for 64 bf16 channels, 64
-// from 512 up - so that every lane moves 16 B and narrow maps still fill the wave; above 2048 columns to the four waves of a
-// workgroup (4096 x 4096 bf16, against re-reading the row: forward 13.5 us / 17, backward 24 + 6 / 56 + 4 with dw in a pass of its
-// own; 16384 x 8192: 136 / 137, 185 + 11 / 294 + 11).  All statistics are f32.
+// from 512 up - so that every lane moves 16 B and narrow maps still fill the wave; above four chunks a lane (2048 bf16, 1024 f32
+// columns) to the four waves of a workgroup (4096 x 4096 bf16, against re-reading the row: forward 12.7 us / 17, backward 24 + 6 /
+// 56 + 4 with dw in a pass of its own; 16384 x 8192: 92 / 137, 150 + 11 / 294 + 11; f32 16384 x 2048, against 32 values a lane of
+// one wave: backward 64 / 87.  Four chunks a lane of one wave, bf16 16384 x 2048: backward 36 / 44 with one chunk of four waves).
+// All statistics are f32.
 // The backward keeps dw / db of a lane's columns in registers over all the rows its group visits, adds the groups of a
 // workgroup in LDS and stores ONE partial row per workgroup; a second launch adds the partial rows in index order.  No
 // atomics: the same input gives the same bits.
 //
-// 147456 x 256 bf16: forward 26 us (5.8 TB/s), backward 42 us (5.4 TB/s) + 6 for the partial rows; 8281 x 771 f32, rows off the line
-// boundaries: 13.4 and 19.8 us (3.8 TB/s both), + 4.
+// 147456 x 256 bf16: forward 26 us (5.8 TB/s), backward 40 us (5.6 TB/s) + 6 for the partial rows; 8281 x 771 f32, rows off the line
+// boundaries: 12.8 and 17.9 us (4.0 and 4.3 TB/s), + 4.
 #include "rows_common.h"
 
 namespace srmi {
@@ -65,14 +67,63 @@ __device__ __forceinline__ float group_sum(float v, float* red) {
     }
 }
 
-// V columns from c on; TAIL: those past C read as `fill` (rows need no alignment: rows_common.h)
-template <int V, bool TAIL, typename T>
-__device__ __forceinline__ void load_cols(const T* p, int c, int C, float fill, float* o) {
-    if (!TAIL || c + V <= C) load_vec<V>(p + c, o);
-    else {
+// A lane's chunks of a row, 16 bytes each as they lie in memory (rows need no alignment: rows_common.h), zeros past C.  Apart from the
+// conversion so that all loads of a row are on their way before the first is looked at: a lane's second chunk may lie past the
+// row's end, and behind that test a conversion would wait for its own load alone.  TAIL: the row's last columns, C % V of
+// them, are one lane's chunk number C / V / LANES.
+__device__ __forceinline__ u32x4 load_tail(const float* p, int left) {
+    float t[4];
+    load_some<4>(p, left, t);
+    return __builtin_bit_cast(u32x4, f32x4{t[0], t[1], t[2], t[3]});
+}
+__device__ __forceinline__ u32x4 load_tail(const bf16_t* p, int left) {
+    u32x4 q;
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = c + j < C ? to_f32(p[c + j]) : fill;
+    for (int j = 0; j < 4; ++j) {
+        const unsigned lo = p[min(2 * j, left - 1)], hi = p[min(2 * j + 1, left - 1)];
+        q[j] = (2 * j < left ? lo : 0u) | (2 * j + 1 < left ? hi << 16 : 0u);
     }
+    return q;
+}
+template <int LANES, int ITER, bool TAIL, typename T>
+__device__ __forceinline__ void load_row(const T* p, int l, int C, u32x4* raw) {
+    constexpr int V = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (i * LANES + l) * V;
+        raw[i] = u32x4{0u, 0u, 0u, 0u};
+        if (c + (TAIL ? V : 1) <= C) raw[i] = *(const u32x4_any*)(p + c);
+        else if (TAIL && ITER == 1 && c < C) raw[i] = load_tail(p + c, C - c);
+    }
+    if constexpr (TAIL && ITER > 1) {                                    // one copy of these loads, not one for every chunk
+        const int last = C / V;
+        if (l == last % LANES) {
+            const u32x4 q = load_tail(p + last * V, C - last * V);
+#pragma unroll
+            for (int i = 0; i < ITER; ++i)
+                if (i == last / LANES) raw[i] = q;
+        }
+    }
+}
+__device__ __forceinline__ void unpack(const u32x4& q, float* o, float) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const unsigned v = q[j];
+        o[j] = __builtin_bit_cast(float, v);
+    }
+}
+__device__ __forceinline__ void unpack(const u32x4& q, float* o, bf16_t) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const unsigned v = q[j];
+        o[2 * j] = __builtin_bit_cast(float, v << 16);
+        o[2 * j + 1] = __builtin_bit_cast(float, v & 0xffff0000u);
+    }
+}
+template <int V, bool TAIL, typename T>
+__device__ __forceinline__ void load_cols(const T* p, int c, int C, float* o) {
+    if (!TAIL || c + V <= C) load_vec<V>(p + c, o);
+    else load_some<V>(p + c, C - c, o);
 }
 template <int V, bool TAIL, typename T>
 __device__ __forceinline__ void store_cols(T* p, int c, int C, const float* o, bool past = false) {
@@ -85,8 +136,8 @@ __device__ __forceinline__ void store_cols(T* p, int c, int C, const float* o, b
 }
 template <int V, bool TAIL>
 __device__ __forceinline__ void load_param(const void* p, int p_bf16, int c, int C, float* o) {
-    if (p_bf16) load_cols<V, TAIL>((const bf16_t*)p, c, C, 0.f, o);
-    else load_cols<V, TAIL>((const float*)p, c, C, 0.f, o);
+    if (p_bf16) load_cols<V, TAIL>((const bf16_t*)p, c, C, o);
+    else load_cols<V, TAIL>((const float*)p, c, C, o);
 }
 
 template <typename T, int LANES, int ITER, bool TAIL>
@@ -109,15 +160,12 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
     const float inv = 1.f / (float)a.C;
     for (long long r = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; r < a.rows; r += ngroups) {
         const T* x = (const T*)a.x + r * a.ldx;
+        u32x4 raw[ITER];
+        load_row<LANES, ITER, TAIL>(x, l, a.C, raw);
         float v[ITER * V], s = 0.f;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            const int c = (i * LANES + l) * V;
-            if (c < a.C) load_cols<V, TAIL>(x, c, a.C, 0.f, v + i * V);
-            else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[i * V + j] = 0.f;
-            }
+            unpack(raw[i], v + i * V, T());
 #pragma unroll
             for (int j = 0; j < V; ++j) s += v[i * V + j];
         }
@@ -150,7 +198,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
 }
 
 template <typename T, int LANES, int ITER, bool TAIL>
-__global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
+__global__ __launch_bounds__(256, 2) void norm_bwd_kernel(NormArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
     constexpr int G = 256 / LANES;
     __shared__ float red[G][LANES * V];
@@ -170,13 +218,16 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
         const T* x = (const T*)a.x + r * a.ldx;
         const T* dy = (const T*)a.dy + r * a.lddy;
         const float mean = a.mean[r], rstd = a.rstd[r];
+        u32x4 rx[ITER], rg[ITER];                                       // 0 past the end: adds nothing below
+        load_row<LANES, ITER, TAIL>(x, l, a.C, rx);
+        load_row<LANES, ITER, TAIL>(dy, l, a.C, rg);
         float xh[ITER * V], g[ITER * V], s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int c = (i * LANES + l) * V;
             if (c < a.C) {
-                load_cols<V, TAIL>(x, c, a.C, 0.f, xh + i * V);
-                load_cols<V, TAIL>(dy, c, a.C, 0.f, g + i * V);         // 0 past the end: adds nothing below
+                unpack(rx[i], xh + i * V, T());
+                unpack(rg[i], g + i * V, T());
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const int k = i * V + j;
@@ -240,7 +291,7 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
         float s = 0.f;
         for (int c = threadIdx.x * V; c < a.C; c += 256 * V) {
             float v[V];
-            load_cols<V, true>(x, c, a.C, 0.f, v);
+            load_cols<V, true>(x, c, a.C, v);
 #pragma unroll
             for (int j = 0; j < V; ++j) s += v[j];
         }
@@ -248,7 +299,7 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
         float q = 0.f;
         for (int c = threadIdx.x * V; c < a.C; c += 256 * V) {
             float v[V];
-            load_cols<V, true>(x, c, a.C, 0.f, v);
+            load_cols<V, true>(x, c, a.C, v);
 #pragma unroll
             for (int j = 0; j < V; ++j)
                 if (c + j < a.C) { v[j] -= mean; q += v[j] * v[j]; }
@@ -256,7 +307,7 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
         const float rstd = 1.f / sqrtf(group_sum<256>(q, red) * inv + a.eps);
         for (int c = threadIdx.x * V; c < a.C; c += 256 * V) {
             float v[V], w[V], b[V];
-            load_cols<V, true>(x, c, a.C, 0.f, v);
+            load_cols<V, true>(x, c, a.C, v);
 #pragma unroll
             for (int j = 0; j < V; ++j) { w[j] = 1.f; b[j] = 0.f; }
             if (a.w) load_param<V, true>(a.w, a.p_bf16, c, a.C, w);
@@ -289,8 +340,8 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
             }
             for (int c = threadIdx.x * V; c < a.C; c += 256 * V) {
                 float xh[V], g[V], w[V];
-                load_cols<V, true>(x, c, a.C, 0.f, xh);
-                load_cols<V, true>(dy, c, a.C, 0.f, g);
+                load_cols<V, true>(x, c, a.C, xh);
+                load_cols<V, true>(dy, c, a.C, g);
 #pragma unroll
                 for (int j = 0; j < V; ++j) w[j] = 1.f;
                 if (a.w) load_param<V, true>(a.w, a.p_bf16, c, a.C, w);
@@ -318,8 +369,8 @@ __global__ __launch_bounds__(256) void norm_wide_dw_kernel(NormArgs a) {
     for (int j = 0; j < V; ++j) dw[j] = db[j] = 0.f;
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         float x[V], dy[V];
-        load_cols<V, true>((const T*)a.x + r * a.ldx, c, a.C, 0.f, x);
-        load_cols<V, true>((const T*)a.dy + r * a.lddy, c, a.C, 0.f, dy);
+        load_cols<V, true>((const T*)a.x + r * a.ldx, c, a.C, x);
+        load_cols<V, true>((const T*)a.dy + r * a.lddy, c, a.C, dy);
         const float mean = a.mean[r], rstd = a.rstd[r];
 #pragma unroll
         for (int j = 0; j < V; ++j) { dw[j] += dy[j] * ((x[j] - mean) * rstd); db[j] += dy[j]; }
@@ -370,11 +421,11 @@ static constexpr int NORM_WIDE = 8192;      // widest row kept in registers: 32 
 
 static int norm_lanes(int C, int dtype) {
     const int v = dtype == SRMI_BF16 ? 8 : 4;
-    return C <= 8 * v ? 8 : C <= 16 * v ? 16 : C <= 32 * v ? 32 : C <= 2048 ? 64 : 256;
+    return C <= 8 * v ? 8 : C <= 16 * v ? 16 : C <= 32 * v ? 32 : C <= 256 * v ? 64 : 256;
 }
 
 // Workgroups of the backward = partial rows of dw / db: eight per CU where there are rows for them (147456 x 256 bf16: 58 us with 512
-// workgroups, 47 with 2048, 42 with dx past the caches) and the partial rows stay below an eighth of x's bytes.
+// workgroups, 47 with 2048, 40 with dx past the caches) and the partial rows stay below an eighth of x's bytes.
 int norm_slots(const srmi_norm_desc& d) {
     const long long esz = d.dtype == SRMI_BF16 ? 2 : 4, per = 256 / norm_lanes(d.C, d.dtype);
     long long most = d.rows * esz / 64;
@@ -412,12 +463,12 @@ static void norm_rows(const NormArgs& a, int slots, hipStream_t s) {
         case 32: norm_go<BWD, T, 32, 1, TAIL>(a, slots, s); return;
         default: break;
     }
-    if (C > 4096) norm_go<BWD, T, 256, 32 / V, TAIL>(a, slots, s);
-    else if (C > 2048) norm_go<BWD, T, 256, 16 / V, TAIL>(a, slots, s);
-    else if (C <= 64 * V) norm_go<BWD, T, 64, 1, TAIL>(a, slots, s);
+    if (C <= 64 * V) norm_go<BWD, T, 64, 1, TAIL>(a, slots, s);
     else if (C <= 128 * V) norm_go<BWD, T, 64, 2, TAIL>(a, slots, s);
     else if (C <= 256 * V) norm_go<BWD, T, 64, 4, TAIL>(a, slots, s);
-    else if constexpr (V == 4) norm_go<BWD, T, 64, 8, TAIL>(a, slots, s);
+    else if (C <= 512 * V) norm_go<BWD, T, 256, 2, TAIL>(a, slots, s);
+    else if (C <= 1024 * V) norm_go<BWD, T, 256, 4, TAIL>(a, slots, s);
+    else if constexpr (V == 4) norm_go<BWD, T, 256, 8, TAIL>(a, slots, s);
 }
 
 template <bool BWD, typename T>
