@@ -138,6 +138,41 @@ __device__ __forceinline__ void load_vec(const _Float16* p, float* v) {
     for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
 }
 
+// 16 bytes of storage as f32
+__device__ __forceinline__ void unpack(const u32x4& q, float* o, float) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const unsigned v = q[j];
+        o[j] = __builtin_bit_cast(float, v);
+    }
+}
+__device__ __forceinline__ void unpack(const u32x4& q, float* o, bf16_t) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const unsigned v = q[j];
+        o[2 * j] = __builtin_bit_cast(float, v << 16);
+        o[2 * j + 1] = __builtin_bit_cast(float, v & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void unpack(const u32x4& q, float* o, _Float16) {
+    const f16x8 h = __builtin_bit_cast(f16x8, q);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = (float)h[j];
+}
+// eight elements as they lie in memory: loads whose conversion comes later do not wait for one another
+template <typename T>
+struct Raw8 {
+    u32x4 q[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int h = 0; h < (int)sizeof(T) / 2; ++h) q[h] = ((const u32x4_any*)p)[h];
+    }
+    __device__ __forceinline__ void get(float* o) const {
+#pragma unroll
+        for (int h = 0; h < (int)sizeof(T) / 2; ++h) unpack(q[h], o + 4 * h, T());
+    }
+};
+
 // The first `left` (1 .. V - 1) of V elements, zeros behind them.  Past the last one it is loaded again: loads that each stand behind a
 // test of their own would wait for one another.
 template <int V, typename T>

@@ -48,6 +48,10 @@ struct TileArgs {
 template <typename T, int V>
 __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const float* bias, long long m, int n) {
     constexpr bool FAST = sizeof(T) == 2;
+    float q[V];
+    Raw8<T> raw;                                      // of the residual, on its way during the activation
+    const T* r = p.residual ? (const T*)p.residual + m * p.ldr + n : nullptr;
+    if (V == 8 && r && n + V <= p.N) raw.load(r);
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] += bias[j];
     if (p.z) {
@@ -67,11 +71,11 @@ __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const 
         }
     }
     row_act_vec<V, FAST>(v, p.act, p.act_param);
-    if (p.residual) {
-        const T* r = (const T*)p.residual + m * p.ldr + n;
-        float q[V];
-        if (n + V <= p.N) load_vec<V>(r, q);
-        else load_some<V>(r, p.N - n, q);
+    if (r) {
+        if (n + V <= p.N) {
+            if constexpr (V == 8) raw.get(q);
+            else load_vec<V>(r, q);
+        } else load_some<V>(r, p.N - n, q);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] += q[j];
     }

@@ -195,29 +195,29 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
     const bool whole = c + 8 <= p.N, kink = is_kink(p.act);
     if (c < p.N) {
         for (long long m = (long long)blockIdx.x * ny + ty; m < p.M; m += (long long)gridDim.x * ny) {
-            float g[8];
+            typedef typename KeptZ<T>::type Z;
             const T* dy = (const T*)p.dy + m * p.lddy + c;
-            if (whole) load_vec<8>(dy, g);
+            const Z* sv = p.saved ? (const Z*)p.saved + m * p.N + c : nullptr;
+            Raw8<T> rg;
+            Raw8<Z> rz;
+            if (whole) {
+                rg.load(dy);
+                if (sv) rz.load(sv);
+            }
+            float g[8];
+            if (whole) rg.get(g);
             else load_some<8>(dy, p.N - c, g);
-            if (p.saved) {
+            if (sv) {
                 float z[8];
-                const auto* sv = (const typename KeptZ<T>::type*)p.saved + m * p.N + c;
                 if (sizeof(T) == 2 && kink) {
                     // y (bf16) or z (half) may have been kept: sign bit and zero are the same in both
-                    const short* bits = (const short*)sv;
                     short h[8];
-                    if (whole) {
-                        const u32x4 q = *(const u32x4_any*)bits;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) h[j] = (short)(q[j / 2] >> (16 * (j & 1)));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) h[j] = bits[min(j, p.N - c - 1)];
-                    }
+                    for (int j = 0; j < 8; ++j) h[j] = whole ? (short)(rz.q[0][j / 2] >> (16 * (j & 1))) : ((const short*)sv)[min(j, p.N - c - 1)];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) z[j] = (h[j] & 0x7fff) == 0 ? 0.f : h[j] < 0 ? -1.f : 1.f;
                 } else if (whole) {
-                    load_vec<8>(sv, z);
+                    rz.get(z);
                 } else {
                     load_some<8>(sv, p.N - c, z);
                 }

@@ -105,21 +105,6 @@ __device__ __forceinline__ void load_row(const T* p, int l, int C, u32x4* raw) {
         }
     }
 }
-__device__ __forceinline__ void unpack(const u32x4& q, float* o, float) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const unsigned v = q[j];
-        o[j] = __builtin_bit_cast(float, v);
-    }
-}
-__device__ __forceinline__ void unpack(const u32x4& q, float* o, bf16_t) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const unsigned v = q[j];
-        o[2 * j] = __builtin_bit_cast(float, v << 16);
-        o[2 * j + 1] = __builtin_bit_cast(float, v & 0xffff0000u);
-    }
-}
 template <int V, bool TAIL, typename T>
 __device__ __forceinline__ void load_cols(const T* p, int c, int C, float* o) {
     if (!TAIL || c + V <= C) load_vec<V>(p + c, o);
