@@ -397,14 +397,42 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(TileArgs p) 
 // Adds the split sums and applies the epilogue; 8 columns of a row belong to SL lanes, lane k of which adds splits k, k + SL, ... in
 // order (their loads are independent: with few outputs and many splits the launch is bound by memory latency), then lane 0 adds
 // the SL sums in order.
+// The workgroups behind the first `blocks` add another call's partial rows (db's, see linear_dz_kernel): 16 columns and 16 lanes each, lane
+// k adds rows k, k + 16, ... in order, then the lanes are added in order.  One launch instead of two (4 us and the gap between them).
+struct SlotSum {
+    const float* part; int slots, n;      // [slots][n]
+    void* out;
+};
+template <typename T>
+__device__ __forceinline__ void slot_sum_block(const SlotSum& s, unsigned block, float (*red)[17]) {
+    const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4, c = (int)block * 16 + cl;
+    float v = 0.f;
+    if (c < s.n) {
+#pragma unroll 16
+        for (int k = sl; k < s.slots; k += 16) v += s.part[(size_t)k * s.n + c];
+    }
+    red[sl][cl] = v;
+    __syncthreads();
+    if (sl == 0 && c < s.n) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k) v += red[k][cl];
+        ((T*)s.out)[c] = from_f32<T>(v);
+    }
+}
+
 template <typename T, int SL>
-__global__ __launch_bounds__(256) void gemm_join_kernel(TileArgs p) {
+__global__ __launch_bounds__(256) void gemm_join_kernel(TileArgs p, unsigned blocks, SlotSum other) {
     constexpr int G = 256 / SL;
     __shared__ f32x4 red[SL > 1 ? 256 : 1][2];
+    __shared__ float rows[16][17];
+    if (blockIdx.x >= blocks) {
+        slot_sum_block<T>(other, blockIdx.x - blocks, rows);
+        return;
+    }
     const int cols = p.part_ld / 8, g = threadIdx.x % G, sl = threadIdx.x / G;
     const long long n8 = p.M * cols;
     const size_t slot = (size_t)p.M * p.part_ld;
-    for (long long e0 = (long long)blockIdx.x * G; e0 < n8; e0 += (long long)gridDim.x * G) {
+    for (long long e0 = (long long)blockIdx.x * G; e0 < n8; e0 += (long long)blocks * G) {
         const long long e = e0 + g, m = e / cols;
         const int n = (int)(e - m * cols) * 8;
         f32x4 v0 = {0.f, 0.f, 0.f, 0.f}, v1 = v0;

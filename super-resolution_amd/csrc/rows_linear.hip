@@ -53,14 +53,18 @@ template <typename T>
 static bool stream_past(long long rows, long long cols) { return (size_t)rows * cols * sizeof(T) > STREAM_BYTES; }
 
 template <typename T>
-static int join(const TileArgs& p, hipStream_t s) {
+static int join(const TileArgs& p, const SlotSum& other, hipStream_t s) {
     const long long n8 = p.M * (p.part_ld / 8);
     const bool wide = p.splits >= 8;
     const long long g = wide ? (n8 + 31) / 32 : (n8 + 255) / 256;
-    const dim3 grid((unsigned)(g > 4096 ? 4096 : g));
-    if (wide) hipLaunchKernelGGL((gemm_join_kernel<T, 8>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((gemm_join_kernel<T, 1>), grid, dim3(256), 0, s, p);
+    const unsigned blocks = (unsigned)(g > 4096 ? 4096 : g);
+    const dim3 grid(blocks + (other.part ? (other.n + 15) / 16 : 0));
+    if (wide) hipLaunchKernelGGL((gemm_join_kernel<T, 8>), grid, dim3(256), 0, s, p, blocks, other);
+    else hipLaunchKernelGGL((gemm_join_kernel<T, 1>), grid, dim3(256), 0, s, p, blocks, other);
     return hip_check(hipGetLastError(), "linear join");
+}
+static int slot_sum(const SlotSum& q, int out_bf16, hipStream_t s) {
+    return q.part ? slot_sum_launch(q.part, q.slots, q.n, q.n, q.out, nullptr, out_bf16, s) : SRMI_OK;
 }
 
 template <int BM, int BN, int WM, int WN, int GK, int NSTAGE, bool PIPE, bool AT, bool BT, typename T>
@@ -80,9 +84,10 @@ static void staged_go(const TileArgs& p, unsigned grid, hipStream_t s) {
     else hipLaunchKernelGGL((gemm_staged_kernel<B, AT, BT, NARROW, T, false>), dim3(grid), dim3(256), 0, s, p);
 }
 
+// other: partial rows that are to be added as well, by the join if there is one
 template <bool AT, bool BT, typename T>
-static int tile_gemm(bool direct, TileArgs& p, float* part, hipStream_t s) {
-    if (p.M == 0 || p.N == 0) return SRMI_OK;
+static int tile_gemm(bool direct, TileArgs& p, float* part, hipStream_t s, const SlotSum& other = {}) {
+    if (p.M == 0 || p.N == 0) return slot_sum(other, sizeof(T) == 2, s);
     const TilePlan t = tile_plan(direct, p.M, p.N, p.K);
     const long long grid = t.tiles_m * t.tiles_n * t.splits;
     if (grid > 0x7fffffff) { set_error("linear: more than 2^31 tiles"); return SRMI_EUNSUPPORTED; }
@@ -106,7 +111,7 @@ static int tile_gemm(bool direct, TileArgs& p, float* part, hipStream_t s) {
         if (t.kind == STAGED_64) staged_go<64, AT, BT, true, T>(p, g, s);
     }
     const int rc = hip_check(hipGetLastError(), "linear product");
-    return rc || t.splits == 1 ? rc : join<T>(p, s);
+    return rc ? rc : t.splits == 1 ? slot_sum(other, sizeof(T) == 2, s) : join<T>(p, other, s);
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------------
@@ -146,7 +151,7 @@ static int thin_fwd_go(const srmi_linear_desc& d, const void* x, const void* w, 
     else if (d.M <= 32) hipLaunchKernelGGL((thin_fwd_kernel<T, 2>), grid, block, 0, s, p);
     else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((thin_fwd_kernel<T, 4>), grid, block, 0, s, p);
     const int rc = hip_check(hipGetLastError(), "linear fwd");
-    return rc || p.t.splits == 1 ? rc : join<T>(p.t, s);
+    return rc || p.t.splits == 1 ? rc : join<T>(p.t, SlotSum{}, s);
 }
 
 // dx and dw of f32 layers; dz: f32 rows
@@ -171,7 +176,7 @@ static bool dma_rows(const srmi_linear_desc& d, int cols, long long ld) {
 
 // ---- dz = dy * act'(saved) and the partial column sums of dz -----------------------------------------------------------------
 // Workgroup (slot of rows, strip of columns): tx lanes of 8 columns, 256 / tx rows at a time; the sums of a workgroup's rows
-// are added in LDS and stored as one partial row, a second launch adds the partial rows in index order.  db sums the f32
+// are added in LDS and stored as one partial row; slot_sum_block (or a launch of its own) adds the partial rows in index order.  db sums the f32
 // products, before dz is rounded to bf16 (the matrix cores' operand type: half a step of 2^-8 per term of dx and dw, as in y itself).
 struct DzArgs {
     const void* dy; long long lddy;
@@ -325,6 +330,7 @@ static int linear_bwd_t(const srmi_linear_desc& d, const void* x, const void* w,
         dz = q.dz = ws + db_bytes(d);
         lddz = q.ldz = up8(d.N);
     }
+    SlotSum sum = {};
     if (db || (q.dz && d.M > 0)) {
         q.dy = dy; q.lddy = d.lddy; q.saved = own_dz(d) ? saved : nullptr;
         const int slots = dz_slots(d.M, d.N);
@@ -332,7 +338,7 @@ static int linear_bwd_t(const srmi_linear_desc& d, const void* x, const void* w,
         q.db = db && slots == 1 ? db : nullptr;
         q.M = d.M; q.N = d.N; q.act = d.act; q.act_param = d.act_param;
         if ((rc = dz_launch<T>(q, s))) return rc;
-        if (q.part && (rc = slot_sum_launch(part, slots, d.N, d.N, db, nullptr, sizeof(T) == 2, s))) return rc;
+        if (q.part) sum = {part, slots, d.N, db};
     }
     if (thin_bwd(d)) return thin_bwd_go(d, (const float*)dz, lddz, x, w, dx, dw, s);
     part = (float*)(ws + db_bytes(d) + dz_bytes(d));
@@ -349,9 +355,9 @@ static int linear_bwd_t(const srmi_linear_desc& d, const void* x, const void* w,
         p.b = x; p.ldb = d.ldx;
         p.M = d.N; p.N = d.K; p.K = d.M;
         p.y = dw; p.ldy = d.K;
-        if ((rc = tile_gemm<true, true, T>(dma_dw(d), p, part, s))) return rc;
+        return tile_gemm<true, true, T>(dma_dw(d), p, part, s, sum);
     }
-    return SRMI_OK;
+    return slot_sum(sum, sizeof(T) == 2, s);
 }
 
 int linear_bwd(const srmi_linear_desc& d, const void* x, const void* w, const void* saved, const void* dy, void* dx, void* dw, void* db,

@@ -181,7 +181,7 @@ def test_linear_leading_axes(lead, dt):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
-@pytest.mark.parametrize("M,K,N", [(0, 8, 5), (4, 0, 6), (4, 8, 0), (0, 0, 0)])
+@pytest.mark.parametrize("M,K,N", [(0, 8, 5), (4, 0, 6), (4, 8, 0), (0, 0, 0), (300, 0, 40), (300, 8, 0)])
 @pytest.mark.parametrize("act", ["none", "gelu"])
 def test_linear_empty(M, K, N, dt, act):
     leaves, dy = linear_case(M, K, N, dt, act, True, True, 0, 8)
