@@ -77,7 +77,7 @@ __device__ __forceinline__ void put(u32x2_any* p, const u32x2& v, bool past) {
     }
 }
 // An output larger than the eight L2s together is stored past them: nothing of it is there when it is read, and the operands that are read
-// next to it stay.  147456 x 256 bf16 (75 MB): layer norm's backward pass 42 us against 48, dropout 34 + 26 against 42 + 31; a
+// next to it stay.  147456 x 256 bf16 (75 MB): layer norm's backward pass 40 us against 48, dropout 34 + 26 against 42 + 31; a
 // 16384 x 4096 product 450 against 470.  Smaller ones are better left in the caches: 9216 x 1024 (19 MB) of dz written past
 // them cost the product that reads it 16.4 us instead of 14.4, and the kernel that writes it gained nothing.
 constexpr size_t STREAM_BYTES = 32u << 20;

@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs p) {
 }
 
 // lanes of 8 columns per row (a power of two), and workgroups of rows = partial rows of db.  One per pass up to eight workgroups per CU
-// (36864 x 1024 gelu, 226 MB: 148 us with 256 workgroups, 47 with 1024); up to 128 rows one workgroup walks them all, 32 at a time, and
+// (36864 x 1024 gelu, 226 MB: 148 us with 256 workgroups, 43 with 1024); up to 128 rows one workgroup walks them all, 32 at a time, and
 // no second launch adds anything.
 static int dz_tx(long long M, int N) {
     int tx = 1;
