@@ -25,10 +25,10 @@ static TilePlan tile_plan(bool direct, long long M, int N, long long K) {
     TilePlan t;
     auto tiles = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     const long long steps = (K + (direct ? 64 : SK) - 1) / (direct ? 64 : SK);
-    // bf16 by the length of K, in steps of 64.  256 x 256 tiles, one workgroup per CU: 1300-1400 TFLOP/s at 4096^3, where 128 x 128 reach
-    // 1070, if they fill the chip.  128 x 128 with 32 k per stage keep four workgroups per CU and hide a short K's prologue and
-    // epilogue behind each other: 36864 x 256 -> 1024 in 36 us against 41 with 64 k per stage (two workgroups); those win
-    // from K = 2048 on (4096^3: 128 against 187 us).
+    // bf16 by the length of K, in steps of 64.  256 x 256 tiles, one workgroup per CU, if they fill the chip: 1280-1380 TFLOP/s at 4096^3
+    // and 8192^3, where 128 x 128 reach 1070 (4864 x 4096 x 4096, 304 tiles: 177 us against 170; 6400, 400 tiles: 183 against 214).
+    // 128 x 128 with 32 k per stage keep four workgroups per CU and hide a short K's prologue and epilogue behind each other: 36864 x
+    // 256 -> 1024 in 36 us against 41 with 64 k per stage (two workgroups); those win from K = 2048 on (4096^3: 128 against 187 us).
     if (direct) t.kind = M <= 32 ? TILE_32 : steps >= 8 && tiles(256, 256) >= 200 ? TILE_256 : steps >= 32 ? TILE_128 : TILE_128_SHORT;
     // the larger tile needs half the LDS traffic (190 against 120 TFLOP/s in f32), if it leaves every CU two workgroups of eight steps
     else t.kind = M >= 8 && N >= 8 && tiles(128, 128) * (steps < 8 ? 1 : steps / 8) >= 512 ? STAGED_128 : STAGED_64;
