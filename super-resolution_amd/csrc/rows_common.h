@@ -4,8 +4,6 @@
 
 namespace srmi {
 
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(bf16_t v) { return bf2f(v); }
 __device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
@@ -20,22 +18,16 @@ typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef u32x2 u32x2_any __attribute__((aligned(2)));
 template <int V>
 __device__ __forceinline__ void load_vec(const float* p, float* o) {
-    if constexpr (V == 1) {
-        o[0] = p[0];
-    } else {
 #pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            const f32x4 q = *(const f32x4_any*)(p + i);
+    for (int i = 0; i < V; i += 4) {
+        const f32x4 q = *(const f32x4_any*)(p + i);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[i + j] = q[j];
-        }
+        for (int j = 0; j < 4; ++j) o[i + j] = q[j];
     }
 }
 template <int V>
 __device__ __forceinline__ void load_vec(const bf16_t* p, float* o) {
-    if constexpr (V == 1) {
-        o[0] = bf2f(p[0]);
-    } else if constexpr (V == 4) {
+    if constexpr (V == 4) {
         const u32x2 q = *(const u32x2_any*)p;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -94,9 +86,7 @@ __device__ __forceinline__ void store_vec(float* p, const float* v, bool past = 
 }
 template <int V>
 __device__ __forceinline__ void store_vec(bf16_t* p, const float* v, bool past = false) {
-    if constexpr (V == 1) {
-        p[0] = f2bf(v[0]);
-    } else if constexpr (V == 4) {
+    if constexpr (V == 4) {
         put((u32x2_any*)p, u32x2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])}, past);
     } else {
         static_assert(V == 8, "one 16-byte store");
@@ -128,14 +118,6 @@ __device__ __forceinline__ void store_vec(_Float16* p, const float* v, bool past
         const u32x4 q = __builtin_bit_cast(u32x4, h);
         put<1>((u32x4_any*)p, &q, past);
     }
-}
-template <int V>
-__device__ __forceinline__ void load_vec(const _Float16* p, float* v) {
-    static_assert(V == 8, "the backward pass reads whole chunks");
-    const u32x4 q = *(const u32x4_any*)p;
-    const f16x8 h = __builtin_bit_cast(f16x8, q);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
 }
 
 // 16 bytes of storage as f32
@@ -242,7 +224,8 @@ __device__ __forceinline__ float row_act(float z, int act, float param) {
     }
 }
 
-// d act / d z at z, its limit at infinities; at the kinks torch's: 0 counts as negative.  tanh and sigmoid from e = exp(-k|z|): 1 - t^2 and s (1 - s) would cancel for large |z|.
+// d act / d z at z, its limit at infinities; at the kinks torch's: 0 counts as negative.  tanh and sigmoid from e = exp(-k|z|): 1 - t^2
+// and s (1 - s) would cancel for large |z|.
 template <bool FAST>
 __device__ __forceinline__ float row_act_slope(float z, int act, float param) {
     z = bounded(z, 100.f);
