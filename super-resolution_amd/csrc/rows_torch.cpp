@@ -69,6 +69,14 @@ void once_more(Tensor& g, bool depends) {
     g = node.apply({g.detach().requires_grad_()})[0];
 }
 
+// Saved-tensor hooks decide what a backward pass gets back: another layout is as good (torch.autograd.graph.save_on_cpu hands back dense rows
+// for strided ones), so strides come from the restored tensor, never from the forward pass; another type, place or shape
+// is refused, since the kernels would read past it.
+void check_restored(const Tensor& t, const char* what, at::ScalarType dtype, at::Device device, at::IntArrayRef shape) {
+    TORCH_CHECK(t.device() == device && t.scalar_type() == dtype && t.sizes() == shape, "srmi.rows: a saved-tensor hook handed back ", what,
+                " as ", t.scalar_type(), " ", t.sizes(), " on ", t.device(), ", saved was ", dtype, " ", shape, " on ", device);
+}
+
 // A backward pass that is captured must not meet a leaf whose accumulation node an eager graph, still alive, made on another stream:
 // autograd would make the capturing stream wait for that one, which ends the capture and with it the process.  Looked for in
 // the operands and in everything they were computed from.
@@ -227,7 +235,9 @@ Tensor linear(const Tensor& x, const Tensor& w, const Opt& bias, const Opt& resi
 // ---- layer norm ------------------------------------------------------------------------------------------------------------
 int param_code(const Tensor& w, const Tensor& b) { return w.defined() ? dtype_code(w) : b.defined() ? dtype_code(b) : SRMI_F32; }
 
-std::tuple<Tensor, Tensor, Tensor, int64_t> norm_run(const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool keep) {
+struct NormOut { Tensor y, stats, x; };
+
+NormOut norm_run(const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool keep) {
     const int64_t C = x.size(-1), rows = x.numel() / C;
     auto [xr, ldx] = strided_rows(x);
     Tensor y = at::empty(x.sizes(), x.options()), stats;
@@ -239,38 +249,40 @@ std::tuple<Tensor, Tensor, Tensor, int64_t> norm_run(const Tensor& x, const Tens
         float* st = (float*)ptr(stats);
         check(srmi_layer_norm_fwd(&d, ptr(xr), ptr(wc), ptr(bc), ptr(y), st, keep ? st + rows : nullptr, stream_of(x)));
     }
-    return {y, stats, xr, ldx};
+    return {y, stats, xr};
 }
 
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Opt& ow, const Opt& ob, double eps) {
         const Tensor w = ow.value_or(Tensor()), b = ob.value_or(Tensor());
-        auto [y, stats, xr, ldx] = norm_run(x, w, b, eps, true);
-        ctx->save_for_backward({xr, w, stats});
+        NormOut o = norm_run(x, w, b, eps, true);
+        ctx->save_for_backward({o.x, w, o.stats});
         ctx->saved_data["eps"] = eps;
         ctx->saved_data["xshape"] = x.sizes().vec();
-        ctx->saved_data["ldx"] = ldx;
         ctx->saved_data["param"] = (int64_t)param_code(w, b);
         ctx->saved_data["need"] = (int64_t)(wants_grad(x) | wants_grad(w) << 1 | wants_grad(b) << 2);
         ctx->saved_data["bias"] = (int64_t)(1 + w.defined());                   // the bias's place among the tensors
-        return y;
+        return o.y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const Tensor& dy = grads[0];
         once(dy);
         const auto saved = ctx->get_saved_variables();
-        const Tensor &xr = saved[0], &stats = saved[2];
-        const Tensor w = saved[1].defined() ? saved[1].contiguous() : saved[1];
         const auto xshape = ctx->saved_data["xshape"].toIntVector();
-        const int64_t C = xshape.back(), rows = stats.size(1), need = ctx->saved_data["need"].toInt();
+        const int64_t C = xshape.back(), rows = dy.numel() / C, need = ctx->saved_data["need"].toInt();
         const int pcode = (int)ctx->saved_data["param"].toInt();
+        check_restored(saved[0], "layer_norm's x", dy.scalar_type(), dy.device(), xshape);
+        check_restored(saved[2], "layer_norm's statistics", at::kFloat, dy.device(), {2, rows});
+        if (saved[1].defined()) check_restored(saved[1], "layer_norm's weight", pcode == SRMI_F32 ? at::kFloat : at::kBFloat16, dy.device(), {C});
         auto asked = [&](int i) { return (need >> i & 1) && ctx->needs_input_grad(i < 2 ? i : ctx->saved_data["bias"].toInt()); };
         const c10::OptionalDeviceGuard guard(dy.device());
-        auto [dyr, lddy] = strided_rows(dy);
+        const auto [xr, ldx] = strided_rows(saved[0]);
+        const auto [dyr, lddy] = strided_rows(dy);
+        const Tensor stats = saved[2].contiguous(), w = saved[1].defined() ? saved[1].contiguous() : Tensor();
         const auto popt = dy.options().dtype(pcode == SRMI_F32 ? at::kFloat : at::kBFloat16);
         Tensor dx = asked(0) ? at::empty(xshape, dy.options()) : Tensor(), dw = asked(1) ? at::empty({C}, popt) : Tensor();
         const Tensor db = asked(2) ? at::empty({C}, popt) : Tensor();
-        const srmi_norm_desc d = {rows, (int32_t)C, dtype_code(dy), pcode, (float)ctx->saved_data["eps"].toDouble(), ctx->saved_data["ldx"].toInt(), lddy};
+        const srmi_norm_desc d = {rows, (int32_t)C, dtype_code(dy), pcode, (float)ctx->saved_data["eps"].toDouble(), ldx, lddy};
         size_t bytes = 0;
         if (dw.defined() || db.defined()) check(srmi_layer_norm_workspace_bytes(&d, &bytes));
         const Tensor ws = workspace(bytes, dy);
@@ -297,7 +309,7 @@ Tensor layer_norm(const Tensor& x, const Opt& weight, const Opt& bias, double ep
         check_capture({&x, &w, &b});
         return LayerNormFn::apply(x, opt(w), opt(b), eps);
     }
-    return std::get<0>(norm_run(x, w, b, eps, false));
+    return norm_run(x, w, b, eps, false).y;
 }
 
 // ---- dropout ---------------------------------------------------------------------------------------------------------------

@@ -868,3 +868,37 @@ def test_backward_offsets_past_32_bits():
     bound = (far + c + 64) * U * (d64.abs() * (xh.abs() + 1)).sum(0) * (1 + s) + s * want.abs() + TINY
     assert_within(dv, want, bound, "far dv")
     assert_within(dvs, want, bound, "near dv")
+
+
+# ---- saved-tensor hooks --------------------------------------------------------------------------------------------------
+def _columns_first(t):
+    """an equal tensor whose last axis is not dense"""
+    return t.detach().transpose(-1, -2).contiguous().transpose(-1, -2) if t.dim() > 1 else t.detach().clone()
+
+
+# the saved tensor comes back with another pitch (dense, from the host), or with columns that have to be copied
+HOOKS = {"save_on_cpu": lambda: torch.autograd.graph.save_on_cpu(),
+         "columns_first": lambda: torch.autograd.graph.saved_tensors_hooks(_columns_first, lambda t: t)}
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("hook", sorted(HOOKS))
+@pytest.mark.parametrize("n,c", [(100, 64), (7, 33), (3, 9000)])
+def test_norm_backward_under_saved_tensor_hooks(n, c, hook, dt):
+    x, w, b, dy = norm_case(n, c, dt, "f32", True, 32, n + c)
+    want = torch.autograd.grad(rows.layer_norm(x, w, b), (x, w, b), dy)
+    with HOOKS[hook]():
+        y = rows.layer_norm(x, w, b)
+        got = torch.autograd.grad(y, (x, w, b), dy)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("bad", [lambda t: t[:1], lambda t: t.double(), lambda t: t.cpu()])
+def test_norm_refuses_what_a_hook_changed(bad):
+    x, w, b, dy = norm_case(20, 48, "f32", "f32", True, 0, 1)
+    for k in range(3):                                                       # x, weight, statistics, in the order they are saved
+        order = iter(range(3))
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: bad(t.detach()) if next(order) == k else t.detach(), lambda t: t):
+            y = rows.layer_norm(x, w, b)
+        with pytest.raises(RuntimeError, match="saved-tensor hook handed back"):
+            torch.autograd.grad(y, (x, w, b), dy)
