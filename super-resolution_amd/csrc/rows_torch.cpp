@@ -174,6 +174,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         ctx->saved_data["N"] = w.size(0);
         ctx->saved_data["K"] = w.size(1);
         ctx->saved_data["need"] = (int64_t)(wants_grad(x) | wants_grad(w) << 1 | wants_grad(b) << 2 | wants_grad(r) << 3);
+        ctx->saved_data["by_sign"] = by_sign;
         ctx->saved_data["res"] = (int64_t)(2 + b.defined());                    // the residual's place among the tensors
         return o.y;
     }
@@ -181,20 +182,27 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         const Tensor& dy = grads[0];
         once(dy);
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &s = saved[2];
         const int64_t N = ctx->saved_data["N"].toInt(), K = ctx->saved_data["K"].toInt(), need = ctx->saved_data["need"].toInt();
         const auto xshape = ctx->saved_data["xshape"].toIntVector();
+        int64_t M = 1;
+        for (size_t i = 0; i + 1 < xshape.size(); ++i) M *= xshape[i];
+        if (saved[0].defined()) check_restored(saved[0], "linear's x", dy.scalar_type(), dy.device(), xshape);
+        if (saved[1].defined()) check_restored(saved[1], "linear's weight", dy.scalar_type(), dy.device(), {N, K});
+        if (saved[2].defined()) {
+            if (ctx->saved_data["by_sign"].toBool()) check_restored(saved[2], "linear's output", dy.scalar_type(), dy.device(), dy.sizes());
+            else check_restored(saved[2], "linear's pre-activation", dy.scalar_type() == at::kBFloat16 ? at::kHalf : at::kFloat, dy.device(), {M, N});
+        }
         // of the inputs that require a gradient, those that this backward pass was asked for
         auto asked = [&](int i) { return (need >> i & 1) && ctx->needs_input_grad(i < 3 ? i : ctx->saved_data["res"].toInt()); };
         Tensor dx, dw, db;
         if (asked(0) || asked(1) || asked(2)) {
             const c10::OptionalDeviceGuard guard(dy.device());
-            Tensor dyr;
-            int64_t lddy, ldx = K, ldw = K, M = 1;
+            Tensor dyr, x, w;
+            int64_t lddy, ldx = K, ldw = K;
             std::tie(dyr, lddy) = strided_rows(dy);
-            if (x.defined()) ldx = std::get<1>(strided_rows(x));
-            if (w.defined()) ldw = std::get<1>(strided_rows(w));
-            for (size_t i = 0; i + 1 < xshape.size(); ++i) M *= xshape[i];
+            if (saved[0].defined()) std::tie(x, ldx) = strided_rows(saved[0]);
+            if (saved[1].defined()) std::tie(w, ldw) = strided_rows(saved[1]);
+            const Tensor s = saved[2].defined() ? saved[2].contiguous() : Tensor();
             if (asked(0)) dx = at::empty(xshape, dy.options());
             if (asked(1)) dw = at::empty({N, K}, dy.options());
             if (asked(2)) db = at::empty({N}, dy.options());

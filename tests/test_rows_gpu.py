@@ -902,3 +902,29 @@ def test_norm_refuses_what_a_hook_changed(bad):
             y = rows.layer_norm(x, w, b)
         with pytest.raises(RuntimeError, match="saved-tensor hook handed back"):
             torch.autograd.grad(y, (x, w, b), dy)
+
+
+# "none" and "gelu" keep nothing / the pre-activation, "relu" the output itself
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("hook", sorted(HOOKS))
+@pytest.mark.parametrize("act", ["none", "gelu", "relu"])
+@pytest.mark.parametrize("M,K,N,pitch", [(100, 72, 40, 24), (5, 72, 40, 24), (60, 33, 21, 13)])
+def test_linear_backward_under_saved_tensor_hooks(M, K, N, pitch, act, hook, dt):
+    leaves, dy = linear_case(M, K, N, dt, act, True, False, pitch, M + K)
+
+    def run():
+        with HOOKS[hook]():
+            return rows.linear(*leaves[:3], act=ACTS[act])
+    check_linear(leaves, dy, dt, act, run=run)
+
+
+@pytest.mark.parametrize("act", ["gelu", "relu"])
+@pytest.mark.parametrize("bad", [lambda t: t[:1], lambda t: t.double(), lambda t: t.cpu()])
+def test_linear_refuses_what_a_hook_changed(bad, act):
+    leaves, dy = linear_case(20, 48, 24, "f32", act, True, False, 0, 2)
+    for k in range(3):                                                       # x, weight, and what the slope is taken from
+        order = iter(range(3))
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: bad(t.detach()) if next(order) == k else t.detach(), lambda t: t):
+            y = rows.linear(*leaves[:3], act=ACTS[act])
+        with pytest.raises(RuntimeError, match="saved-tensor hook handed back"):
+            torch.autograd.grad(y, leaves[:3], dy)
