@@ -342,7 +342,11 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const Tensor& dy = grads[0];
         once(dy);
-        const Tensor rng = ctx->get_saved_variables()[0];
+        Tensor rng = ctx->get_saved_variables()[0];
+        if (rng.defined()) {
+            check_restored(rng, "dropout's [seed, offset]", at::kLong, dy.device(), {2});
+            rng = rng.contiguous();
+        }
         const int64_t need = ctx->saved_data["need"].toInt();
         auto asked = [&](int i) { return (need >> i & 1) && ctx->needs_input_grad(i); };
         const c10::OptionalDeviceGuard guard(dy.device());

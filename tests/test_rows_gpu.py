@@ -928,3 +928,21 @@ def test_linear_refuses_what_a_hook_changed(bad, act):
             y = rows.linear(*leaves[:3], act=ACTS[act])
         with pytest.raises(RuntimeError, match="saved-tensor hook handed back"):
             torch.autograd.grad(y, leaves[:3], dy)
+
+
+def test_dropout_device_counter_under_saved_tensor_hooks():
+    x = torch.randn(40, 33, device=DEV, requires_grad=True)
+    rng = torch.tensor([11, 5], dtype=torch.int64, device=DEV)
+    dy = torch.randn(40, 33, device=DEV)
+    (want,) = torch.autograd.grad(rows.dropout(x, 0.3, 11, 5), x, dy)
+    apart = torch.tensor([11, 0, 5, 0], device=DEV)[::2]                     # equal, not dense
+    for unpack in (lambda t: t, lambda t: apart):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), unpack):
+            y = rows.dropout(x, 0.3, rng)
+            (got,) = torch.autograd.grad(y, x, dy)
+        assert torch.equal(got, want)
+    for bad in (lambda t: t[:1], lambda t: t.cpu(), lambda t: t.int(), lambda t: t.float()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), bad):
+            y = rows.dropout(x, 0.3, rng)
+            with pytest.raises(RuntimeError, match="saved-tensor hook handed back"):
+                torch.autograd.grad(y, x, dy)
