@@ -3,6 +3,7 @@
 // forward call and as much again in the backward one.
 //
 // Workspaces are tensors of the call: nothing is shared between streams, graphs or threads.
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
@@ -56,11 +57,20 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_de
 Tensor workspace(size_t bytes, const Tensor& like) {
     return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
+// A tangent of forward-mode AD would be lost: the operators have no such formula, and a result without a tangent passes for a constant.
+void check_tangents(std::initializer_list<const Tensor*> operands) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : operands)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "srmi.rows: forward-mode automatic differentiation is not supported");
+}
 // autograd counts the tensors a node was given, not its optional arguments
 typedef std::optional<Tensor> Opt;
 Opt opt(const Tensor& t) { return t.defined() ? Opt(t) : std::nullopt; }
 constexpr char ONCE[] = "srmi.rows: the backward passes are not differentiable themselves";
-void once(const Tensor& dy) { TORCH_CHECK(!(at::GradMode::is_enabled() && dy.requires_grad()), ONCE); }
+void once(const Tensor& dy) {
+    check_tangents({&dy});
+    TORCH_CHECK(!(at::GradMode::is_enabled() && dy.requires_grad()), ONCE);
+}
 // A gradient that depends on tensors that require one themselves: under create_graph=True differentiating it raises, instead of
 // passing for a constant.
 void once_more(Tensor& g, bool depends) {
@@ -221,8 +231,9 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 };
 
 Tensor linear(const Tensor& x, const Tensor& w, const Opt& bias, const Opt& residual, int64_t act, double param) {
-    check_x(x);
     const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+    check_tangents({&x, &w, &b, &r});
+    check_x(x);
     TORCH_CHECK_VALUE(w.dim() == 2, "srmi.rows.linear: weight must be [out_features, in_features]");
     check_like(w, "weight", x.scalar_type(), x, w.sizes());
     TORCH_CHECK_VALUE(x.size(-1) == w.size(1), "srmi.rows.linear: x has ", x.size(-1), " features, weight ", w.sizes());
@@ -303,8 +314,9 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
 };
 
 Tensor layer_norm(const Tensor& x, const Opt& weight, const Opt& bias, double eps) {
-    check_x(x);
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    check_tangents({&x, &w, &b});
+    check_x(x);
     const int64_t C = x.size(-1);
     TORCH_CHECK_VALUE(C > 0, "srmi.rows.layer_norm: the last axis is empty");
     TORCH_CHECK_VALUE(eps >= 0.0, "srmi.rows.layer_norm: eps must be >= 0");
@@ -359,8 +371,9 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
 };
 
 Tensor dropout(const Tensor& x, const Opt& residual, double p, uint64_t seed, uint64_t offset, const Opt& device_rng) {
-    check_x(x);
     const Tensor r = residual.value_or(Tensor()), rng = device_rng.value_or(Tensor());
+    check_tangents({&x, &r});
+    check_x(x);
     TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "srmi.rows.dropout: p must be in [0, 1], got ", p);
     if (rng.defined()) {
         check_like(rng, "seed", at::kLong, x, {2});

@@ -147,3 +147,26 @@ def test_strided_rows_finds_uniform_strides():
     maps = torch.randn(2, 6, 4, 5).to(memory_format=torch.channels_last).permute(0, 2, 3, 1)
     t, ld = rows._strided_rows(maps)
     assert t is maps and ld == 6
+
+
+def _calls(x, v, w):
+    """every operator with `x` as each of its operands (x [8, 8], v [8], w [8, 8] plain)"""
+    return [lambda: rows.linear(x, w), lambda: rows.linear(w, x), lambda: rows.linear(w, w, residual=x), lambda: rows.linear(w, w, x[0]),
+            lambda: rows.layer_norm(x), lambda: rows.layer_norm(w, x[0]), lambda: rows.layer_norm(w, v, x[0]),
+            lambda: rows.dropout(x, 0.5, 1), lambda: rows.dropout(w, 0.5, 1, residual=x)]
+
+
+def test_tangents_are_refused():
+    # an output without a tangent would pass for a constant
+    import torch.autograd.forward_ad as fwAD
+    v, w = torch.randn(8), torch.randn(8, 8)
+    with fwAD.dual_level():
+        x = fwAD.make_dual(torch.randn(8, 8), torch.randn(8, 8))
+        for call in _calls(x, v, w):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        with fwAD._set_fwd_grad_enabled(False):                              # nothing to lose
+            for call in _calls(x, v, w):
+                with pytest.raises(RuntimeError, match="no CPU fallback"):
+                    call()

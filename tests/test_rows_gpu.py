@@ -946,3 +946,18 @@ def test_dropout_device_counter_under_saved_tensor_hooks():
             y = rows.dropout(x, 0.3, rng)
             with pytest.raises(RuntimeError, match="saved-tensor hook handed back"):
                 torch.autograd.grad(y, x, dy)
+
+
+# ---- transforms that the operators cannot follow ---------------------------------------------------------------------------
+def test_tangents_are_refused_in_both_passes():
+    import torch.autograd.forward_ad as fwAD
+    x, w = torch.randn(5, 8, device=DEV), torch.randn(6, 8, device=DEV)
+    with fwAD.dual_level():
+        for f in (lambda t: rows.linear(t, w), lambda t: rows.layer_norm(t), lambda t: rows.dropout(t, 0.5, 1)):
+            leaf = x.clone().requires_grad_()
+            y = f(leaf)
+            dy = fwAD.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(RuntimeError, match="forward-mode"):          # forward over reverse
+                torch.autograd.grad(y, leaf, dy)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f(fwAD.make_dual(x, torch.ones_like(x)))
