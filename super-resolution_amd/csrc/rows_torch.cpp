@@ -4,10 +4,12 @@
 //
 // Workspaces are tensors of the call: nothing is shared between streams, graphs or threads.
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -63,11 +65,25 @@ void check_tangents(std::initializer_list<const Tensor*> operands) {
     for (const Tensor* t : operands)
         TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "srmi.rows: forward-mode automatic differentiation is not supported");
 }
+// The dispatcher sees the allocations of a call and no operator, and the kernels read the operands' own storage.  What records calls to run
+// them again (torch.jit.trace, make_fx, torch.export) would replay an output nobody writes, and a wrapper tensor (FakeTensor,
+// DTensor) has no storage of its own: both are refused.  Modes that only watch (FlopCounterMode) or keep and recompute
+// (selective checkpointing) get correct results and are let through.
+void check_recorders(std::initializer_list<const Tensor*> operands) {
+    typedef c10::impl::TorchDispatchModeKey Mode;
+    bool recording = torch::jit::tracer::isTracing();
+    for (Mode m : {Mode::FAKE, Mode::PROXY, Mode::FUNCTIONAL}) recording |= c10::impl::TorchDispatchModeTLS::get_mode(m).has_value();
+    TORCH_CHECK_NOT_IMPLEMENTED(!recording, "srmi.rows: the operators cannot be traced or exported, a replay would return memory that nobody wrote");
+    for (const Tensor* t : operands)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::Functionalize})),
+                                    "srmi.rows: a tensor subclass with its own dispatch has no storage that a kernel can read");
+}
 // autograd counts the tensors a node was given, not its optional arguments
 typedef std::optional<Tensor> Opt;
 Opt opt(const Tensor& t) { return t.defined() ? Opt(t) : std::nullopt; }
 constexpr char ONCE[] = "srmi.rows: the backward passes are not differentiable themselves";
 void once(const Tensor& dy) {
+    check_recorders({&dy});
     check_tangents({&dy});
     TORCH_CHECK(!(at::GradMode::is_enabled() && dy.requires_grad()), ONCE);
 }
@@ -232,6 +248,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 
 Tensor linear(const Tensor& x, const Tensor& w, const Opt& bias, const Opt& residual, int64_t act, double param) {
     const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+    check_recorders({&x, &w, &b, &r});
     check_tangents({&x, &w, &b, &r});
     check_x(x);
     TORCH_CHECK_VALUE(w.dim() == 2, "srmi.rows.linear: weight must be [out_features, in_features]");
@@ -315,6 +332,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
 
 Tensor layer_norm(const Tensor& x, const Opt& weight, const Opt& bias, double eps) {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    check_recorders({&x, &w, &b});
     check_tangents({&x, &w, &b});
     check_x(x);
     const int64_t C = x.size(-1);
@@ -372,6 +390,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
 
 Tensor dropout(const Tensor& x, const Opt& residual, double p, uint64_t seed, uint64_t offset, const Opt& device_rng) {
     const Tensor r = residual.value_or(Tensor()), rng = device_rng.value_or(Tensor());
+    check_recorders({&x, &r, &rng});
     check_tangents({&x, &r});
     check_x(x);
     TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "srmi.rows.dropout: p must be in [0, 1], got ", p);

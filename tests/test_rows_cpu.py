@@ -170,3 +170,24 @@ def test_tangents_are_refused():
             for call in _calls(x, v, w):
                 with pytest.raises(RuntimeError, match="no CPU fallback"):
                     call()
+
+
+def test_recorders_and_wrapper_tensors_are_refused():
+    # a replay would return the memory that the recorded call allocated, unwritten
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, v, w = torch.randn(8, 8), torch.randn(8), torch.randn(8, 8)
+    for k in range(9):
+        with pytest.raises(NotImplementedError, match="traced"):
+            torch.jit.trace(lambda t: _calls(t, v, w)[k](), (x,))
+        for mode in ("real", "fake"):
+            with pytest.raises(NotImplementedError, match="traced"):
+                make_fx(lambda t: _calls(t, v, w)[k](), tracing_mode=mode)(x)
+        with FakeTensorMode() as fake:
+            t = fake.from_tensor(x)
+            with pytest.raises(NotImplementedError, match="traced"):
+                _calls(t, v, w)[k]()
+        with pytest.raises(NotImplementedError, match="own dispatch"):
+            _calls(t, v, w)[k]()
+        with pytest.raises(RuntimeError, match="no CPU fallback"):          # as before outside
+            _calls(x, v, w)[k]()

@@ -961,3 +961,57 @@ def test_tangents_are_refused_in_both_passes():
                 torch.autograd.grad(y, leaf, dy)
             with pytest.raises(RuntimeError, match="forward-mode"):
                 f(fwAD.make_dual(x, torch.ones_like(x)))
+
+
+def test_recorders_are_refused_in_both_passes():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w = torch.randn(5, 8, device=DEV, requires_grad=True), torch.randn(6, 8, device=DEV)
+    for f in (lambda t: rows.linear(t, w), lambda t: rows.layer_norm(t), lambda t: rows.dropout(t, 0.5, 1)):
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                with pytest.raises(NotImplementedError, match="traced"):
+                    torch.jit.trace(f, (x.detach(),))
+                with pytest.raises(NotImplementedError, match="traced"):
+                    make_fx(f)(x.detach())
+        y = f(x)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(lambda dy: torch.autograd.grad(y, x, dy))(torch.ones_like(y))
+
+
+def test_modes_that_watch_or_recompute_get_the_results():
+    from functools import partial
+    from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
+    from torch.utils.flop_counter import FlopCounterMode
+    gen = torch.Generator().manual_seed(61)
+    p = _mixer_params(64, 96, "f32", gen)
+    t = make((50, 64), "f32", gen).requires_grad_()
+    dy = make((50, 64), "f32", gen)
+
+    def step(f):
+        y = f(t)
+        return [y] + list(torch.autograd.grad(y, [t] + list(p.values()), dy))
+
+    want = step(lambda u: _mixer(u, p))
+    with FlopCounterMode(display=False):
+        got = step(lambda u: _mixer(u, p))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for policy in (CheckpointPolicy.MUST_SAVE, CheckpointPolicy.PREFER_RECOMPUTE):
+        contexts = partial(create_selective_checkpoint_contexts, lambda ctx, op, *a, **k: policy)
+        got = step(lambda u: checkpoint(lambda q: _mixer(q, p), u, use_reentrant=False, context_fn=contexts))
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), policy
+
+
+def test_compiled_programs_call_the_operators_outside_their_graphs():
+    gen = torch.Generator().manual_seed(62)
+    p = _mixer_params(64, 96, "f32", gen)
+    t = make((50, 64), "f32", gen).requires_grad_()
+    dy = make((50, 64), "f32", gen)
+
+    def f(u):
+        return _mixer(u * 2.0, p) + 1.0
+
+    y = f(t)
+    want = [y] + list(torch.autograd.grad(y, [t] + list(p.values()), dy))
+    y = torch.compile(f, backend="aot_eager")(t)
+    got = [y] + list(torch.autograd.grad(y, [t] + list(p.values()), dy))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
