@@ -128,8 +128,13 @@ void check_capture(std::initializer_list<const Tensor*> operands) {
     }
 }
 
+// Kernels read what lies in memory: a view that negates it (the imaginary part of a conjugate) is written out first.
+Tensor as_stored(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+Tensor dense(const Tensor& t) { return t.defined() ? as_stored(t).contiguous() : t; }
+
 // `t` as [rows, last axis]: in place if the last axis is dense and the leading ones walk with one stride, else a copy
-std::tuple<Tensor, int64_t> strided_rows(const Tensor& t) {
+std::tuple<Tensor, int64_t> strided_rows(const Tensor& view) {
+    const Tensor t = as_stored(view);
     const int64_t c = t.size(-1);
     if (t.is_contiguous()) return {t, c};
     if (t.stride(-1) == 1 || c <= 1) {
@@ -167,9 +172,9 @@ LinearOut linear_run(const Tensor& x, const Tensor& w, const Tensor& b, const Te
     int64_t ldx, ldw, ldr = 0;
     std::tie(o.x, ldx) = strided_rows(x);
     std::tie(o.w, ldw) = strided_rows(w);
-    Tensor rr, bb;
+    Tensor rr;
     if (r.defined()) std::tie(rr, ldr) = strided_rows(r);
-    if (b.defined()) bb = b.contiguous();
+    const Tensor bb = dense(b);
     auto shape = x.sizes().vec();
     int64_t M = 1;
     for (size_t i = 0; i + 1 < shape.size(); ++i) M *= shape[i];
@@ -228,7 +233,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
             std::tie(dyr, lddy) = strided_rows(dy);
             if (saved[0].defined()) std::tie(x, ldx) = strided_rows(saved[0]);
             if (saved[1].defined()) std::tie(w, ldw) = strided_rows(saved[1]);
-            const Tensor s = saved[2].defined() ? saved[2].contiguous() : Tensor();
+            const Tensor s = dense(saved[2]);
             if (asked(0)) dx = at::empty(xshape, dy.options());
             if (asked(1)) dw = at::empty({N, K}, dy.options());
             if (asked(2)) db = at::empty({N}, dy.options());
@@ -280,7 +285,7 @@ NormOut norm_run(const Tensor& x, const Tensor& w, const Tensor& b, double eps, 
     if (keep) stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
     if (rows) {
         TORCH_CHECK_VALUE(C <= INT32_MAX, "srmi.rows.layer_norm: more than 2^31 features");
-        const Tensor wc = w.defined() ? w.contiguous() : w, bc = b.defined() ? b.contiguous() : b;
+        const Tensor wc = dense(w), bc = dense(b);
         const srmi_norm_desc d = {rows, (int32_t)C, dtype_code(x), param_code(w, b), (float)eps, ldx, 0};
         float* st = (float*)ptr(stats);
         check(srmi_layer_norm_fwd(&d, ptr(xr), ptr(wc), ptr(bc), ptr(y), st, keep ? st + rows : nullptr, stream_of(x)));
@@ -314,7 +319,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
         const c10::OptionalDeviceGuard guard(dy.device());
         const auto [xr, ldx] = strided_rows(saved[0]);
         const auto [dyr, lddy] = strided_rows(dy);
-        const Tensor stats = saved[2].contiguous(), w = saved[1].defined() ? saved[1].contiguous() : Tensor();
+        const Tensor stats = dense(saved[2]), w = dense(saved[1]);
         const auto popt = dy.options().dtype(pcode == SRMI_F32 ? at::kFloat : at::kBFloat16);
         Tensor dx = asked(0) ? at::empty(xshape, dy.options()) : Tensor(), dw = asked(1) ? at::empty({C}, popt) : Tensor();
         const Tensor db = asked(2) ? at::empty({C}, popt) : Tensor();
@@ -352,7 +357,7 @@ Tensor layer_norm(const Tensor& x, const Opt& weight, const Opt& bias, double ep
 
 // ---- dropout ---------------------------------------------------------------------------------------------------------------
 Tensor dropout_run(const Tensor& x_, const Tensor& residual, double p, uint64_t seed, uint64_t offset, const Tensor& rng) {
-    const Tensor x = x_.contiguous(), r = residual.defined() ? residual.contiguous() : residual;
+    const Tensor x = dense(x_), r = dense(residual);
     Tensor y = at::empty(x.sizes(), x.options());
     if (x.numel())
         check(srmi_dropout(ptr(x), ptr(r), ptr(y), (size_t)x.numel(), dtype_code(x), p, seed, offset, (const uint64_t*)ptr(rng), stream_of(x)));
@@ -375,7 +380,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
         Tensor rng = ctx->get_saved_variables()[0];
         if (rng.defined()) {
             check_restored(rng, "dropout's [seed, offset]", at::kLong, dy.device(), {2});
-            rng = rng.contiguous();
+            rng = dense(rng);
         }
         const int64_t need = ctx->saved_data["need"].toInt();
         auto asked = [&](int i) { return (need >> i & 1) && ctx->needs_input_grad(i); };

@@ -1015,3 +1015,25 @@ def test_compiled_programs_call_the_operators_outside_their_graphs():
     y = torch.compile(f, backend="aot_eager")(t)
     got = [y] + list(torch.autograd.grad(y, [t] + list(p.values()), dy))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_negated_views_are_written_out():
+    # the imaginary part of a conjugate is a view of the unconjugated memory with its sign still to be turned
+    gen = torch.Generator().manual_seed(63)
+
+    def both(shape):
+        t = make(shape, "f32", gen)
+        return torch._neg_view(-t), t
+
+    (xn, x), (wn, w), (bn, b), (rn, r), (gn, g) = (both(s) for s in ((9, 16), (24, 16), (24,), (9, 24), (16,)))
+    assert xn.is_neg() and torch.equal(xn, x)
+    assert torch.equal(rows.linear(xn, wn, bn, act=nn.Tanh(), residual=rn), rows.linear(x, w, b, act=nn.Tanh(), residual=r))
+    assert torch.equal(rows.layer_norm(xn, gn, gn), rows.layer_norm(x, g, g))
+    assert torch.equal(rows.dropout(rn, 0.25, 4, residual=rn), rows.dropout(r, 0.25, 4, residual=r))
+    for f in (lambda t: rows.linear(t, w), lambda t: rows.layer_norm(t), lambda t: rows.dropout(t, 0.5, 1)):
+        x_ = x.clone().requires_grad_()
+        dn, d = both(tuple(f(x_).shape))
+        assert torch.equal(*(torch.autograd.grad(f(x_), x_, v)[0] for v in (dn, d)))
+    z = make((8, 2), "f32", gen)
+    col = torch.view_as_complex(z)[:, None].conj().imag                      # [8, 1], in place for a row operator
+    assert col.is_neg() and torch.equal(rows.linear(col, torch.ones(1, 1, device=DEV)), -z[:, 1:])
