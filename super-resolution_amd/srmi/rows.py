@@ -124,26 +124,51 @@ class LayerNorm(nn.LayerNorm):
 
 
 class Dropout(nn.Module):
-    """Dropout with a residual add; call number k of this module in training draws with offset k under its seed (``calls``, reset or
-    restore it to repeat a run).  Give every module - and every data-parallel rank - its own seed.  Identity (plus the residual)
-    in eval mode.  While a graph is being captured a host-side count would repeat one mask at every replay: pass ``rng``, the device
-    tensor of `dropout`, there."""
+    """Dropout with a residual add; identity (plus the residual) in eval mode.
 
-    def __init__(self, p=0.5, seed=0):
+    ``seed=None``: every call in training draws a seed and an offset from torch's host generator.  ``torch.manual_seed`` repeats a run, modules
+    differ, and activation checkpointing (`torch.utils.checkpoint` restores that generator) recomputes with the forward's mask.
+    Seed the generator differently on every data-parallel rank.
+
+    With an integer ``seed`` nothing else decides: call number k of this module in training draws with offset k (``calls``, reset or
+    restore it to repeat a run).  Give every module - and every rank - its own.  A call that is recomputed inside a backward
+    pass would count again and draw another mask: it raises, pass ``offset`` there, a number that names the call (a step), instead of
+    the count.
+
+    While a HIP graph is being captured any host-side number would repeat one mask at every replay: pass ``rng``, the device tensor
+    of `dropout`."""
+
+    def __init__(self, p=0.5, seed=None):
         super().__init__()
         if not 0.0 <= float(p) <= 1.0:
             raise ValueError(f"srmi.rows.Dropout: p must be in [0, 1], got {p}")
-        self.p, self.seed, self.calls = float(p), int(seed), 0
+        if seed is not None and not 0 <= int(seed) < 1 << 64:
+            raise ValueError(f"srmi.rows.Dropout: seed must be None or an integer in [0, 2^64), got {seed}")
+        self.p, self.seed, self.calls = float(p), None if seed is None else int(seed), 0
 
     def extra_repr(self):
         return f"p={self.p}, seed={self.seed}"
 
-    def forward(self, x, residual=None, rng=None):
+    @torch.compiler.disable
+    def _draw(self, offset):
+        """(seed, offset) of this call"""
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("srmi.rows.Dropout: pass rng=[seed, offset] (int64 device tensor) inside a graph capture")
+        if self.seed is None:
+            if offset is not None:
+                raise ValueError("srmi.rows.Dropout: offset goes with a seed, this module has none")
+            return [v % (1 << 64) for v in torch.randint(-(1 << 63), (1 << 63) - 1, (2,), dtype=torch.int64, device="cpu").tolist()]
+        if offset is not None:
+            return self.seed, offset
+        if torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("srmi.rows.Dropout: a module with a seed counts its calls, and this one is recomputed inside a backward pass "
+                               "(activation checkpointing): pass offset, or leave seed=None")
+        self.calls += 1
+        return self.seed, self.calls
+
+    def forward(self, x, residual=None, rng=None, offset=None):
         if not self.training:
             return x if residual is None else dropout(x, 0.0, 0, residual=residual)
         if rng is not None:
-            return dropout(x, self.p, rng, residual=residual)
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("srmi.rows.Dropout: pass rng=[seed, offset] (int64 device tensor) inside a graph capture")
-        self.calls += 1
-        return dropout(x, self.p, self.seed, self.calls, residual=residual)
+            return dropout(x, self.p, rng, 0 if offset is None else offset, residual=residual)
+        return dropout(x, self.p, *self._draw(offset), residual=residual)

@@ -191,3 +191,21 @@ def test_recorders_and_wrapper_tensors_are_refused():
             _calls(t, v, w)[k]()
         with pytest.raises(RuntimeError, match="no CPU fallback"):          # as before outside
             _calls(x, v, w)[k]()
+
+
+def test_dropout_seeds():
+    assert rows.Dropout(0.5).seed is None and rows.Dropout(0.5).state_dict() == {}
+    for bad in (-1, 1 << 64):
+        with pytest.raises(ValueError, match="seed"):
+            rows.Dropout(0.5, seed=bad)
+    with pytest.raises(ValueError, match="offset goes with a seed"):
+        rows.Dropout(0.5)(torch.randn(3), offset=1)
+
+
+def test_dropout_draws_follow_the_host_generator():
+    a, b = rows.Dropout(0.5), rows.Dropout(0.5)
+    torch.manual_seed(7)
+    first = [a._draw(None), b._draw(None), a._draw(None)]
+    torch.manual_seed(7)
+    assert first == [a._draw(None), b._draw(None), a._draw(None)]
+    assert all(0 <= v < 1 << 64 for pair in first for v in pair) and len({v for pair in first for v in pair}) == 6

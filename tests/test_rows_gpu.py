@@ -1037,3 +1037,65 @@ def test_negated_views_are_written_out():
     z = make((8, 2), "f32", gen)
     col = torch.view_as_complex(z)[:, None].conj().imag                      # [8, 1], in place for a row operator
     assert col.is_neg() and torch.equal(rows.linear(col, torch.ones(1, 1, device=DEV)), -z[:, 1:])
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_dropout_under_activation_checkpointing(reentrant):
+    # the recomputed pass must draw the forward's mask: with another one the gradients belong to a different function
+    from torch.utils.checkpoint import checkpoint
+    x = torch.randn(40, 64, device=DEV, requires_grad=True)
+    w = torch.randn(64, 64, device=DEV, requires_grad=True)
+    dy = torch.randn(40, 64, device=DEV)
+    free = [rows.Dropout(0.5), rows.Dropout(0.5)]
+    seeded = rows.Dropout(0.5, seed=5)
+
+    def step(block, through):
+        torch.manual_seed(8)
+        out = [through(block, x), through(block, x)]
+        return out + [g for y in out for g in torch.autograd.grad(y, (x, w), dy, retain_graph=True)]
+
+    def drawn(t):
+        return free[1](rows.linear(free[0](t), w, act=nn.GELU()))
+
+    def stepped(t):
+        return seeded(rows.linear(seeded(t, offset=11), w, act=nn.GELU()), offset=12)
+
+    def counted(t):
+        return rows.linear(seeded(t), w, act=nn.GELU())
+
+    def again(block, t):
+        return checkpoint(block, t, use_reentrant=reentrant)
+
+    if reentrant:                                                            # that form supports .backward() alone
+        def step(block, through):
+            torch.manual_seed(8)
+            out = [through(block, x), through(block, x)]
+            x.grad = w.grad = None
+            ((out[0] + 2 * out[1]) * dy).sum().backward()
+            return [o.detach() for o in out] + [x.grad, w.grad]
+
+    for block in (drawn, stepped):
+        want = step(block, lambda f, t: f(t))
+        assert all(torch.equal(a, b) for a, b in zip(step(block, again), want))
+    assert seeded.calls == 0
+    y = again(counted, x)
+    with pytest.raises(RuntimeError, match="recomputed inside a backward pass"):
+        y.sum().backward()
+    assert seeded.calls == 1
+
+
+def test_dropout_modules_differ():
+    x = torch.randn(64, 32, device=DEV)
+    a, b = rows.Dropout(0.5), rows.Dropout(0.5)
+    assert not torch.equal(a(x), b(x)) and not torch.equal(a(x), a(x))
+    m = rows.Dropout(0.5, seed=3)
+    assert torch.equal(m(x, offset=1), rows.dropout(x, 0.5, 3, 1)) and m.calls == 0
+    rng = torch.tensor([3, 1], device=DEV)
+    assert torch.equal(a(x, rng=rng), rows.dropout(x, 0.5, 3, 1))
+    with pytest.raises(ValueError, match="no other offset"):
+        m(x, rng=rng, offset=2)
+    net = torch.compile(lambda t: a(t * 2.0) + 1.0, backend="aot_eager")
+    torch.manual_seed(9)
+    got = net(x)
+    torch.manual_seed(9)
+    assert torch.equal(got, a(x * 2.0) + 1.0)
