@@ -130,8 +130,8 @@ class Dropout(nn.Module):
     differ, and activation checkpointing (`torch.utils.checkpoint` restores that generator) recomputes with the forward's mask.
     Seed the generator differently on every data-parallel rank.
 
-    With an integer ``seed`` nothing else decides: call number k of this module in training draws with offset k (``calls``, reset or
-    restore it to repeat a run).  Give every module - and every rank - its own.  A call that is recomputed inside a backward
+    With an integer ``seed`` nothing else decides: call number k of this module in training draws with offset k (``calls``, kept in the
+    state_dict so that a resumed run goes on).  Give every module - and every rank - its own.  A call that is recomputed inside a backward
     pass would count again and draw another mask: it raises, pass ``offset`` there, a number that names the call (a step), instead of
     the count.
 
@@ -148,6 +148,19 @@ class Dropout(nn.Module):
 
     def extra_repr(self):
         return f"p={self.p}, seed={self.seed}"
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        if self.seed is not None:
+            destination[prefix + "calls"] = torch.tensor(self.calls, dtype=torch.int64, device="cpu")
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        key = prefix + "calls"
+        if self.seed is not None and key in state_dict:
+            self.calls = int(state_dict[key])
+            if key in unexpected_keys:
+                unexpected_keys.remove(key)
 
     @torch.compiler.disable
     def _draw(self, offset):

@@ -193,13 +193,26 @@ def test_recorders_and_wrapper_tensors_are_refused():
             _calls(x, v, w)[k]()
 
 
-def test_dropout_seeds():
+def test_dropout_seeds_and_state():
     assert rows.Dropout(0.5).seed is None and rows.Dropout(0.5).state_dict() == {}
     for bad in (-1, 1 << 64):
         with pytest.raises(ValueError, match="seed"):
             rows.Dropout(0.5, seed=bad)
     with pytest.raises(ValueError, match="offset goes with a seed"):
         rows.Dropout(0.5)(torch.randn(3), offset=1)
+    net = nn.Sequential(rows.Linear(2, 2), rows.Dropout(0.5, seed=3), rows.Dropout(0.5))
+    net[1].calls = (1 << 40) + 5
+    state = net.state_dict()
+    assert list(state) == ["0.weight", "0.bias", "1.calls"]
+    other = nn.Sequential(rows.Linear(2, 2), rows.Dropout(0.5, seed=3), rows.Dropout(0.5))
+    other.load_state_dict(state)
+    assert other[1].calls == (1 << 40) + 5
+    del state["1.calls"]                                                     # a state from before the count was kept
+    other.load_state_dict(state)
+    assert other[1].calls == (1 << 40) + 5
+    state["2.calls"] = torch.tensor(4)                                       # a module without a seed has no count
+    with pytest.raises(RuntimeError, match="2.calls"):
+        other.load_state_dict(state)
 
 
 def test_dropout_draws_follow_the_host_generator():

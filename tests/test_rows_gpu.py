@@ -1084,12 +1084,15 @@ def test_dropout_under_activation_checkpointing(reentrant):
     assert seeded.calls == 1
 
 
-def test_dropout_modules_differ():
+def test_dropout_modules_differ_and_resume():
     x = torch.randn(64, 32, device=DEV)
     a, b = rows.Dropout(0.5), rows.Dropout(0.5)
     assert not torch.equal(a(x), b(x)) and not torch.equal(a(x), a(x))
     m = rows.Dropout(0.5, seed=3)
-    assert torch.equal(m(x, offset=1), rows.dropout(x, 0.5, 3, 1)) and m.calls == 0
+    m(x)
+    resumed = rows.Dropout(0.5, seed=3)
+    resumed.load_state_dict(m.state_dict())
+    assert torch.equal(m(x), resumed(x)) and torch.equal(m(x, offset=1), rows.dropout(x, 0.5, 3, 1)) and m.calls == 2
     rng = torch.tensor([3, 1], device=DEV)
     assert torch.equal(a(x, rng=rng), rows.dropout(x, 0.5, 3, 1))
     with pytest.raises(ValueError, match="no other offset"):
