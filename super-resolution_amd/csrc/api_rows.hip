@@ -142,7 +142,7 @@ int srmi_layer_norm_bwd(const srmi_norm_desc* d, const void* x, const void* weig
                         void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes, void* stream) {
     const int rc = check_norm(d, "layer_norm_bwd");
     if (rc) return rc;
-    if (!dx && !dweight && !dbias) return SRMI_OK;
+    if (!dweight && !dbias && (!dx || d->rows == 0)) return SRMI_OK;      // (gradients of the parameters are zeros then, and written)
     if (d->rows > 0 && (!x || !mean || !rstd || !dy || d->lddy < d->C)) { set_error("layer_norm_bwd: NULL argument, or dy without its row stride"); return SRMI_EINVAL; }
     if (!element_aligned(x, d->dtype) || !element_aligned(dy, d->dtype) || !element_aligned(dx, d->dtype) ||
         !element_aligned(weight, d->param_dtype) || !element_aligned(dweight, d->param_dtype) || !element_aligned(dbias, d->param_dtype) ||

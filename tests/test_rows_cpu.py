@@ -222,3 +222,13 @@ def test_dropout_draws_follow_the_host_generator():
     torch.manual_seed(7)
     assert first == [a._draw(None), b._draw(None), a._draw(None)]
     assert all(0 <= v < 1 << 64 for pair in first for v in pair) and len({v for pair in first for v in pair}) == 6
+
+
+@pytest.mark.parametrize("c", [8, 4096, 9000])
+@pytest.mark.parametrize("dt", [L.F32, L.BF16])
+def test_norm_backward_of_no_rows_is_nothing_to_do(dt, c):
+    # dx of no rows: nothing is launched, so this passes without a GPU
+    lib, big = L.load(), 1 << 40
+    d = L.NormDesc(0, c, dt, dt, 1e-5, c, c)
+    assert lib.srmi_layer_norm_bwd(C.byref(d), big, big, big, big, big, big, None, None, None, 0, None) == 0, lib.srmi_last_error()
+    assert lib.srmi_layer_norm_bwd(C.byref(d), None, None, None, None, None, big, None, None, None, 0, None) == 0, lib.srmi_last_error()

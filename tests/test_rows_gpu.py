@@ -1102,3 +1102,22 @@ def test_dropout_modules_differ_and_resume():
     got = net(x)
     torch.manual_seed(9)
     assert torch.equal(got, a(x * 2.0) + 1.0)
+
+
+# ---- the C entry points ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("c", [8, 4096, 9000])
+def test_norm_backward_of_no_rows(c, dt):
+    import ctypes as C
+
+    from srmi import _lib as L
+    lib, n = L.load(), C.c_size_t(0)
+    d = L.NormDesc(0, c, L.F32 if dt == "f32" else L.BF16, L.F32, 1e-5, c, c)
+    L.check(lib.srmi_layer_norm_workspace_bytes(C.byref(d), C.byref(n)))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=DEV)
+    dx, dw, db = (torch.full((c,), 7.0, device=DEV) for _ in range(3))
+    stream = torch.cuda.current_stream().cuda_stream
+    L.check(lib.srmi_layer_norm_bwd(C.byref(d), None, None, None, None, None, dx.data_ptr(), None, None, None, 0, stream))
+    L.check(lib.srmi_layer_norm_bwd(C.byref(d), None, None, None, None, None, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n.value, stream))
+    torch.cuda.synchronize()
+    assert not dw.any() and not db.any() and bool((dx == 7).all())           # sums of nothing; no row of dx to write
