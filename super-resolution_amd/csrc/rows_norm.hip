@@ -368,36 +368,41 @@ __global__ __launch_bounds__(256) void norm_wide_dw_kernel(NormArgs a) {
 // out[c] = sum over slots of part[slot][c], n columns.  16 columns x 64 lanes per workgroup: lane k adds slots k, k + 64, ... in order, then
 // four lanes at a time and the sixteen sums are added in order.  (Many lanes per column because the launch waits on memory, not on
 // bandwidth: 512 slots of 512 columns took 20 us with 8 lanes.)  Two outputs: columns [0, n0) to o0, [n0, n) to o1.
+// A launch has fewer than 2^32 threads, 64 for a column: the widest rows (n = 2^26) walk the grid more than once.
 __global__ __launch_bounds__(1024) void slot_sum_kernel(const float* part, int slots, int n, int n0, void* o0, void* o1, int out_bf16) {
     __shared__ float red[64][17];
     const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4;
-    const int c = blockIdx.x * 16 + cl;
-    float s = 0.f;
-    if (c < n) {
+    for (int c0 = blockIdx.x * 16; c0 < n; c0 += gridDim.x * 16) {
+        const int c = c0 + cl;
+        float s = 0.f;
+        if (c < n) {
 #pragma unroll 4
-        for (int k = sl; k < slots; k += 64) s += part[(size_t)k * n + c];
-    }
-    red[sl][cl] = s;
-    __syncthreads();
-    if (sl < 16) s = red[4 * sl][cl] + red[4 * sl + 1][cl] + red[4 * sl + 2][cl] + red[4 * sl + 3][cl];
-    __syncthreads();
-    if (sl < 16) red[sl][cl] = s;
-    __syncthreads();
-    if (sl == 0 && c < n) {
-#pragma unroll
-        for (int k = 1; k < 16; ++k) s += red[k][cl];
-        void* o = c < n0 ? o0 : o1;
-        const int i = c < n0 ? c : c - n0;
-        if (o) {
-            if (out_bf16) ((bf16_t*)o)[i] = f2bf(s);
-            else ((float*)o)[i] = s;
+            for (int k = sl; k < slots; k += 64) s += part[(size_t)k * n + c];
         }
+        red[sl][cl] = s;
+        __syncthreads();
+        if (sl < 16) s = red[4 * sl][cl] + red[4 * sl + 1][cl] + red[4 * sl + 2][cl] + red[4 * sl + 3][cl];
+        __syncthreads();
+        if (sl < 16) red[sl][cl] = s;
+        __syncthreads();
+        if (sl == 0 && c < n) {
+#pragma unroll
+            for (int k = 1; k < 16; ++k) s += red[k][cl];
+            void* o = c < n0 ? o0 : o1;
+            const int i = c < n0 ? c : c - n0;
+            if (o) {
+                if (out_bf16) ((bf16_t*)o)[i] = f2bf(s);
+                else ((float*)o)[i] = s;
+            }
+        }
+        __syncthreads();                     // red is written again
     }
 }
 
 int slot_sum_launch(const float* part, int slots, int n, int n0, void* o0, void* o1, int out_bf16, hipStream_t s) {
     if (n == 0) return SRMI_OK;
-    hipLaunchKernelGGL(slot_sum_kernel, dim3((n + 15) / 16), dim3(1024), 0, s, part, slots, n, n0, o0, o1, out_bf16);
+    const int blocks = (n + 15) / 16, most = 1 << 21;
+    hipLaunchKernelGGL(slot_sum_kernel, dim3(blocks < most ? blocks : most), dim3(1024), 0, s, part, slots, n, n0, o0, o1, out_bf16);
     return hip_check(hipGetLastError(), "slot_sum");
 }
 

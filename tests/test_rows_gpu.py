@@ -1121,3 +1121,41 @@ def test_norm_backward_of_no_rows(c, dt):
     L.check(lib.srmi_layer_norm_bwd(C.byref(d), None, None, None, None, None, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n.value, stream))
     torch.cuda.synchronize()
     assert not dw.any() and not db.any() and bool((dx == 7).all())           # sums of nothing; no row of dx to write
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_norm_widest_rows(dt):
+    # the columns of dw and db together are 2^26, one launch adds them up
+    c = 1 << 25
+    x = torch.randn((2, c), device=DEV).to(DT[dt]).requires_grad_()
+    w = torch.ones(c, device=DEV, dtype=DT[dt]).requires_grad_()
+    b = torch.zeros(c, device=DEV, dtype=DT[dt]).requires_grad_()
+    dy = (torch.arange(2 * c, device=DEV) % 251 - 125).reshape(2, c).to(DT[dt])
+    y = rows.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    x64, dy64 = x.detach().double(), dy.double()
+    mean = x64.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x64 - mean) ** 2).mean(1, keepdim=True) + 1e-5)
+    xh = (x64 - mean) * rstd
+    s, e = half_step(dt), (c / 256 + 64) * U                                 # 256 lanes: c / 256 sums one after another, |x| and deviation alike
+    for got, want, big in ((y, xh, xh.abs() + 1), (dw, (dy64 * xh).sum(0), (dy64.abs() * (xh.abs() + 1)).sum(0)), (db, dy64.sum(0), dy64.abs().sum(0)),
+                           (dx, rstd * (dy64 - dy64.mean(1, keepdim=True) - xh * (dy64 * xh).mean(1, keepdim=True)), 250 * (xh.abs() + 1))):
+        assert float(((got.double() - want).abs() - e * big * (1 + s) - s * want.abs()).max()) <= 0
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_linear_most_features(dt):
+    # 2^22 outputs of few rows: the bias gradient's strips of columns are one axis of the grid
+    m, n = 3, 1 << 22
+    x = torch.tensor([[1.0], [2.0], [-1.0]], device=DEV, dtype=DT[dt]).requires_grad_()
+    w = (torch.arange(n, device=DEV) % 15 - 7).to(DT[dt])[:, None].requires_grad_()
+    b = torch.zeros(n, device=DEV, dtype=DT[dt]).requires_grad_()
+    dy = (torch.arange(m * n, device=DEV) % 7 - 3).reshape(m, n).to(DT[dt])
+    y = rows.linear(x, w, b, act=nn.ReLU())
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    z = x.detach().double() * w.detach().double()[:, 0]                      # small integers: exact, but for the sum over n
+    dz = dy.double() * (z > 0)
+    assert torch.equal(y.double(), z.clamp(min=0)) and torch.equal(db.double(), dz.sum(0))
+    assert torch.equal(dw.double(), (dz * x.detach().double()).sum(0)[:, None])
+    want = (dz * w.detach().double()[:, 0]).sum(1, keepdim=True)
+    assert bool(((dx.double() - want).abs() <= half_step(dt) * want.abs()).all())    # integers below 2^24 in every partial sum
