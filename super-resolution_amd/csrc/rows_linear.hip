@@ -18,7 +18,7 @@ static int up8(int n) { return (n + 7) & ~7; }
 
 // ---- the tile product: shape -> kernel, tile, split --------------------------------------------------------------------------
 enum TileKind { TILE_256, TILE_128, TILE_128_SHORT, TILE_32, STAGED_128, STAGED_64 };
-struct TilePlan { TileKind kind; long long tiles_m; int tiles_n, splits; size_t part_bytes; };
+struct TilePlan { TileKind kind; int bm; long long tiles_m; int tiles_n, splits; size_t part_bytes; };
 
 // direct: both operands can be read by the DMA
 static TilePlan tile_plan(bool direct, long long M, int N, long long K) {
@@ -32,7 +32,7 @@ static TilePlan tile_plan(bool direct, long long M, int N, long long K) {
     if (direct) t.kind = M <= 32 ? TILE_32 : steps >= 8 && tiles(256, 256) >= 200 ? TILE_256 : steps >= 32 ? TILE_128 : TILE_128_SHORT;
     // the larger tile needs half the LDS traffic (190 against 120 TFLOP/s in f32), if it leaves every CU two workgroups of eight steps
     else t.kind = M >= 8 && N >= 8 && tiles(128, 128) * (steps < 8 ? 1 : steps / 8) >= 512 ? STAGED_128 : STAGED_64;
-    const int bm = t.kind == TILE_256 ? 256 : t.kind == TILE_32 ? 32 : t.kind == STAGED_64 ? 64 : 128;
+    const int bm = t.bm = t.kind == TILE_256 ? 256 : t.kind == TILE_32 ? 32 : t.kind == STAGED_64 ? 64 : 128;
     const int bn = t.kind == TILE_256 ? 256 : t.kind == STAGED_64 ? 64 : 128;
     t.tiles_m = (M + bm - 1) / bm;
     t.tiles_n = (N + bn - 1) / bn;
@@ -84,17 +84,10 @@ static void staged_go(const TileArgs& p, unsigned grid, hipStream_t s) {
     else hipLaunchKernelGGL((gemm_staged_kernel<B, AT, BT, NARROW, T, false>), dim3(grid), dim3(256), 0, s, p);
 }
 
-// other: partial rows that are to be added as well, by the join if there is one
+// the product's launch for the rows that `p` names
 template <bool AT, bool BT, typename T>
-static int tile_gemm(bool direct, TileArgs& p, float* part, hipStream_t s, const SlotSum& other = {}) {
-    if (p.M == 0 || p.N == 0) return slot_sum(other, sizeof(T) == 2, s);
-    const TilePlan t = tile_plan(direct, p.M, p.N, p.K);
-    const long long grid = t.tiles_m * t.tiles_n * t.splits;
-    if (grid > 0x7fffffff) { set_error("linear: more than 2^31 tiles"); return SRMI_EUNSUPPORTED; }
-    p.tiles_m = (int)t.tiles_m; p.tiles_n = t.tiles_n; p.splits = t.splits;
-    p.part = part; p.part_ld = up8(p.N);
-    p.past = stream_past<T>(p.M, p.N);
-    const unsigned g = (unsigned)grid;
+static int tile_launch(const TilePlan& t, const TileArgs& p, hipStream_t s) {
+    const unsigned g = (unsigned)p.tiles_m * p.tiles_n * p.splits;
     if constexpr (sizeof(T) == 2) {
         switch (t.kind) {
             case TILE_256: tile_go<256, 256, 2, 4, 64, 2, true, AT, BT, T>(p, g, s); break;
@@ -110,7 +103,36 @@ static int tile_gemm(bool direct, TileArgs& p, float* part, hipStream_t s, const
     else if constexpr (AT || BT) {
         if (t.kind == STAGED_64) staged_go<64, AT, BT, true, T>(p, g, s);
     }
-    const int rc = hip_check(hipGetLastError(), "linear product");
+    return hip_check(hipGetLastError(), "linear product");
+}
+
+// A launch has fewer than 2^32 threads, of which a workgroup has 512 at most.
+constexpr long long LAUNCH_GROUPS = 0xffffffffll / 512;
+
+// other: partial rows that are to be added as well, by the join if there is one
+template <bool AT, bool BT, typename T>
+static int tile_gemm(bool direct, TileArgs& p, float* part, hipStream_t s, const SlotSum& other = {}) {
+    if (p.M == 0 || p.N == 0) return slot_sum(other, sizeof(T) == 2, s);
+    const TilePlan t = tile_plan(direct, p.M, p.N, p.K);
+    p.tiles_n = t.tiles_n; p.splits = t.splits;
+    p.part = part; p.part_ld = up8(p.N);
+    p.past = stream_past<T>(p.M, p.N);
+    // more tiles than a launch may have workgroups (they are not split then): runs of whole tile rows, one launch each
+    const long long most = LAUNCH_GROUPS / ((long long)t.tiles_n * t.splits), per = t.tiles_m < most ? t.tiles_m : most;
+    int rc = SRMI_OK;
+    for (long long t0 = 0; t0 < t.tiles_m && !rc; t0 += per) {
+        const long long m0 = t0 * t.bm, left = p.M - m0;
+        TileArgs q = p;
+        q.tiles_m = (int)(t.tiles_m - t0 < per ? t.tiles_m - t0 : per);
+        if (per < t.tiles_m) {
+            q.M = left < per * t.bm ? left : per * t.bm;
+            q.a = (const T*)p.a + (AT ? m0 : m0 * p.lda);
+            q.y = (T*)p.y + m0 * p.ldy;
+            if (p.z) q.z = (typename KeptZ<T>::type*)p.z + m0 * p.N;
+            if (p.residual) q.residual = (const T*)p.residual + m0 * p.ldr;
+        }
+        rc = tile_launch<AT, BT, T>(t, q, s);
+    }
     return rc ? rc : t.splits == 1 ? slot_sum(other, sizeof(T) == 2, s) : join<T>(p, other, s);
 }
 

@@ -1159,3 +1159,31 @@ def test_linear_most_features(dt):
     assert torch.equal(dw.double(), (dz * x.detach().double()).sum(0)[:, None])
     want = (dz * w.detach().double()[:, 0]).sum(1, keepdim=True)
     assert bool(((dx.double() - want).abs() <= half_step(dt) * want.abs()).all())    # integers below 2^24 in every partial sum
+
+
+def test_linear_more_tiles_than_a_launch_takes():
+    # 2^30 rows of one column are 2^24 tiles of 64 rows and 256 threads: 2^32 threads, one too many for one launch
+    m, far = (1 << 30) + 1000, 1000
+    x = (torch.arange(m, device=DEV, dtype=torch.int32) % 17 - 8).float()[:, None].requires_grad_()
+    w = torch.full((1, 1), 0.5, device=DEV, requires_grad=True)
+    b = torch.ones(1, device=DEV, requires_grad=True)
+    dy = torch.zeros(m, 1, device=DEV)
+    dy[:far] = 3.0
+    dy[-far:] = (torch.arange(far, device=DEV) % 7 - 3).float()[:, None]
+    y = rows.linear(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    with torch.no_grad():                                                    # halves and small integers: every sum is exact
+        assert torch.equal(y, x * 0.5 + 1) and torch.equal(dx, dy * 0.5)
+        ends = torch.cat((x[:far], x[-far:])), torch.cat((dy[:far], dy[-far:]))
+        assert float(dw) == float((ends[0] * ends[1]).sum()) and float(db) == float(ends[1].sum())
+    del x, y, dy, dx
+    # the tiles of the DMA, residual and all: 128 rows each, more than 2^23 of them
+    period, times = 1 << 15, (1 << 15) + 3
+    gen = torch.Generator().manual_seed(72)
+    x0, w, b, r0 = make((period, 8), "bf16", gen), make((8, 8), "bf16", gen), make((8,), "bf16", gen), make((period, 8), "bf16", gen)
+    x, r = x0.repeat(times, 1).requires_grad_(), r0.repeat(times, 1)
+    x0.requires_grad_()
+    y0, y = rows.linear(x0, w, b, act=nn.GELU(), residual=r0), rows.linear(x, w, b, act=nn.GELU(), residual=r)
+    assert bool((y.detach().view(times, period, 8) == y0.detach()).all())
+    (dx0,), (dx,) = torch.autograd.grad(y0, x0, r0), torch.autograd.grad(y, x, r)
+    assert bool((dx.view(times, period, 8) == dx0).all())
