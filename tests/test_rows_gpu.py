@@ -1187,3 +1187,66 @@ def test_linear_more_tiles_than_a_launch_takes():
     assert bool((y.detach().view(times, period, 8) == y0.detach()).all())
     (dx0,), (dx,) = torch.autograd.grad(y0, x0, r0), torch.autograd.grad(y, x, r)
     assert bool((dx.view(times, period, 8) == dx0).all())
+
+
+# ---- every tile kernel, with what its epilogue can do ------------------------------------------------------------------------
+def check_linear_64(leaves, dy, dt, act):
+    """check_linear with the 64-bit products on the GPU, for sizes that take the large tiles; the same bounds"""
+    x, w, b, r = leaves
+    (M, K), N = x.shape, w.shape[0]
+    wanted = [t for t in leaves if t is not None]
+    y = rows.linear(x, w, b, act=ACTS[act], residual=r)
+    grads = dict(zip([k for k, t in zip("xwbr", leaves) if t is not None], torch.autograd.grad(y, wanted, dy)))
+    with torch.no_grad():
+        x64, w64, dy64 = x.double(), w.double(), dy.double()
+        b64 = b.double() if b is not None else torch.zeros(N, dtype=torch.float64, device=DEV)
+        wt = w64.t().contiguous()
+        z = x64 @ wt + b64
+    f, g = act64(z, act)
+    s, fn = half_step(dt), FN[dt]
+    with torch.no_grad():
+        ez = (K + 8) * U * (x64.abs() @ wt.abs() + b64.abs())
+        out = f + (r.double() if r is not None else 0)
+        ey = LIP[act] * ez + fn * (f.abs() + 0.01 * z.abs()) + 2 * U * out.abs() + s * out.abs() + TINY
+
+        def within(got, want, bound, what):
+            assert got.shape == want.shape and bool(torch.isfinite(got).all()), what
+            assert float(((got.double() - want).abs() - bound).max()) <= 0, what
+
+        within(y, out, ey + s * ey, "y")
+        dz = dy64 * g
+        zq = (2.0 ** -11 * z.abs() + 2.0 ** -25 if dt == "bf16" else 0) + ez
+        edz = dy64.abs() * (CURV[act] * zq + fn * (g.abs() + 0.01) * (act != "none"))
+        if act in ("relu", "lrelu"):
+            edz = edz + dy64.abs() * (z.abs() <= ez)
+        edz_q = edz + (s if act != "none" else 0) * (dz.abs() + edz)
+        if b is not None:
+            want = dz.sum(0)
+            within(grads["b"], want, (edz.sum(0) + (M + 8) * U * dz.abs().sum(0)) * (1 + s) + s * want.abs() + TINY, "db")
+        for name, p, q, ep, n in (("x", dz, w64, edz_q, N), ("w", dz.t().contiguous(), x64, edz_q.t().contiguous(), M)):
+            want = p @ q
+            e = ep @ q.abs() + (n + 8) * U * ((p.abs() + ep) @ q.abs())
+            within(grads[name], want, e * (1 + s) + s * want.abs() + TINY, "d" + name)
+        assert r is None or torch.equal(grads["r"], dy)
+
+
+# bf16 tiles of 128 x 128 with 64 k per stage, not split: prompt-sized products, all three of them
+@pytest.mark.parametrize("act,bias,res", [("none", False, False), ("gelu", True, True), ("relu", True, False), ("silu", False, True)])
+def test_linear_unsplit_128_tiles(act, bias, res):
+    leaves, dy = linear_case(2040, 2200, 2056, "bf16", act, bias, res, 0, 81)
+    check_linear_64(leaves, dy, "bf16", act)
+
+
+# 256 x 256 in the forward product
+@pytest.mark.parametrize("act,bias,res", [("gelu", True, True), ("lrelu", True, False), ("relu", False, True), ("tanh", False, False)])
+def test_linear_256_tiles_with_epilogue(act, bias, res):
+    leaves, dy = linear_case(3590, 520, 3608, "bf16", act, bias, res, 8, 82)
+    check_linear_64(leaves, dy, "bf16", act)
+
+
+# 32 x 128, not split: the forward of a wide head, its input gradient, and the weight gradient of a narrow one
+@pytest.mark.parametrize("M,K,N", [(20, 2112, 33000), (20, 33000, 72), (500, 33000, 24)])
+@pytest.mark.parametrize("act,bias,res", [("gelu", True, True), ("relu", True, False)])
+def test_linear_unsplit_32_tiles(M, K, N, act, bias, res):
+    leaves, dy = linear_case(M, K, N, "bf16", act, bias, res, 0, 83)
+    check_linear_64(leaves, dy, "bf16", act)
