@@ -232,3 +232,40 @@ def test_norm_backward_of_no_rows_is_nothing_to_do(dt, c):
     d = L.NormDesc(0, c, dt, dt, 1e-5, c, c)
     assert lib.srmi_layer_norm_bwd(C.byref(d), big, big, big, big, big, big, None, None, None, 0, None) == 0, lib.srmi_last_error()
     assert lib.srmi_layer_norm_bwd(C.byref(d), None, None, None, None, None, big, None, None, None, 0, None) == 0, lib.srmi_last_error()
+
+
+# ---- how far an f32 product may be off in the root mean square --------------------------------------------------------------
+def f32_product_rms(K, sigma, out_rms):
+    """root mean square error of a sum of K random products (root mean square `sigma` each) in f32, u = 2^-24.  Added one after the other,
+    step k rounds a partial sum of sigma sqrt(k) by at most u of it, evenly: u sigma sqrt(k / 3); the squares add up to
+    u^2 sigma^2 K (K + 1) / 6.  Then one rounding of the result.  Sums in blocks or splits stay below."""
+    u = 2.0 ** -24
+    return u * (sigma * (K * (K + 1) / 6) ** 0.5 + out_rms / 3 ** 0.5)
+
+
+def _planes(t):
+    hi = (t.view(torch.int32) & -65536).view(torch.float32)
+    mid = (t - hi).bfloat16().float()
+    return hi, mid, (t - hi - mid).bfloat16().float()
+
+
+@pytest.mark.parametrize("K", [96, 264, 300, 1090, 2100, 2950])
+def test_f32_bound_sees_a_missing_plane(K):
+    # the kernels multiply f32 as three bf16 planes, six products.  Without the low plane (the three largest products, summed exactly) the
+    # error is over the bound at every K the kernels are checked at; with it, and f32 sums of 32 products at a time, under it.
+    gen = torch.Generator().manual_seed(K)
+    a, b = torch.randn(96, K, generator=gen), torch.randn(160, K, generator=gen)
+    want = a.double() @ b.double().t()
+    bound = f32_product_rms(K, float(a.double().square().mean().sqrt() * b.double().square().mean().sqrt()), float(want.square().mean().sqrt()))
+    pa, pb = _planes(a), _planes(b)
+
+    def total(pairs, exact):
+        out = torch.zeros(96, 160, dtype=torch.float64 if exact else torch.float32)
+        for k in range(0, K, 32):
+            for i, j in pairs:
+                part = pa[i][:, k:k + 32].double() @ pb[j][:, k:k + 32].double().t()
+                out = out + (part if exact else part.float())
+        return float((out.double() - want).square().mean().sqrt())
+
+    assert total([(0, 0), (0, 1), (1, 0)], True) > 1.5 * bound
+    assert total([(0, 0), (0, 1), (1, 0), (0, 2), (2, 0), (1, 1)], False) <= bound

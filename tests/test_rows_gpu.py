@@ -12,6 +12,7 @@ import torch.nn as nn
 
 from srmi import autograd as AG
 from srmi import rows
+from test_rows_cpu import f32_product_rms
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -1250,3 +1251,19 @@ def test_linear_256_tiles_with_epilogue(act, bias, res):
 def test_linear_unsplit_32_tiles(M, K, N, act, bias, res):
     leaves, dy = linear_case(M, K, N, "bf16", act, bias, res, 0, 83)
     check_linear_64(leaves, dy, "bf16", act)
+
+
+# f32: tiles of 64 (unsplit and split) and of 128 (unsplit in the forward, split; dx and dw split), and the few-row kernels
+@pytest.mark.parametrize("M,K,N", [(700, 96, 200), (700, 264, 200), (2900, 300, 2950), (1100, 2100, 1090), (16, 2950, 300), (24, 300, 1090)])
+def test_linear_f32_products_keep_24_bits(M, K, N):
+    # the per-element bound of check_linear grows with K until it no longer sees 16-bit operands; this one does (test_rows_cpu.py)
+    leaves, dy = linear_case(M, K, N, "f32", "none", False, False, 0, 84)
+    x, w = leaves[0], leaves[1]
+    y = rows.linear(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    x64, w64, dy64 = x.detach().double(), w.detach().double(), dy.double()
+    for got, a, b in ((y, x64, w64.t().contiguous()), (dx, dy64, w64), (dw, dy64.t().contiguous(), x64)):
+        want = a @ b
+        sigma = float(a.square().mean().sqrt() * b.square().mean().sqrt())
+        err = float((got.detach().double() - want).square().mean().sqrt())
+        assert err <= f32_product_rms(a.shape[1], sigma, float(want.square().mean().sqrt()))
