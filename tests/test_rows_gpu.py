@@ -1267,3 +1267,108 @@ def test_linear_f32_products_keep_24_bits(M, K, N):
         sigma = float(a.square().mean().sqrt() * b.square().mean().sqrt())
         err = float((got.detach().double() - want).square().mean().sqrt())
         assert err <= f32_product_rms(a.shape[1], sigma, float(want.square().mean().sqrt()))
+
+
+class Guarded:
+    """`n` bytes of 0xff (NaN in every storage type) with 64 KiB of a pattern on either side"""
+    EDGE = 1 << 16
+
+    def __init__(self, n):
+        self.n, whole = n, 2 * self.EDGE + n
+        self.buf = torch.full((whole,), 0xA5, dtype=torch.uint8, device=DEV)
+        self.buf[self.EDGE:self.EDGE + n] = 0xFF
+
+    def ptr(self):
+        assert self.buf.data_ptr() % 256 == 0
+        return self.buf.data_ptr() + self.EDGE
+
+    def view(self, dt):
+        return self.buf[self.EDGE:self.EDGE + self.n].view(dt)
+
+    def intact(self):
+        return bool((self.buf[:self.EDGE] == 0xA5).all()) and bool((self.buf[self.EDGE + self.n:] == 0xA5).all())
+
+
+def _guarded(**sizes):
+    return {k: Guarded(n) for k, n in sizes.items()}
+
+
+def _check_guarded(bufs, written):
+    torch.cuda.synchronize()
+    for name, g in bufs.items():
+        assert g.intact(), f"written past {name}"
+    for name, dt in written.items():
+        assert bool(torch.isfinite(bufs[name].view(dt).float()).all()), f"{name} is not written whole"
+
+
+@pytest.mark.parametrize("M,K,N,dt,act", [(1, 1, 1, "bf16", "gelu"), (1, 1, 1, "f32", "gelu"), (17, 33, 5, "bf16", "relu"), (17, 33, 5, "f32", "silu"),
+                                          (5, 4101, 35, "f32", "tanh"), (5, 4104, 35, "bf16", "tanh"), (63, 264, 41, "bf16", "gelu"), (20, 2112, 33001, "bf16", "none"),
+                                          (300, 520, 203, "bf16", "gelu"), (301, 519, 203, "bf16", "gelu"), (500, 33000, 21, "bf16", "relu"),
+                                          (2039, 2200, 2053, "bf16", "silu"), (3591, 520, 3603, "bf16", "gelu"), (1100, 2101, 1091, "f32", "none"),
+                                          (2901, 300, 2950, "f32", "gelu"), (700, 96, 201, "f32", "lrelu"), (203, 5, 3, "f32", "sigmoid"), (203, 5, 3, "bf16", "gelu_tanh")])
+def test_linear_writes_its_outputs_and_nothing_else(M, K, N, dt, act):
+    import ctypes as C
+
+    from srmi import _lib as L
+    lib, n = L.load(), C.c_size_t(0)
+    leaves, dy = linear_case(M, K, N, dt, act, True, True, 0, 85)
+    x, w, b, r = (t.detach() for t in leaves)
+    code, param = rows._act_of(ACTS[act])
+    e = 2 if dt == "bf16" else 4
+    d = L.LinearDesc(M, N, K, L.BF16 if dt == "bf16" else L.F32, code, param, 16, K, K, N, N)
+    stream = torch.cuda.current_stream().cuda_stream
+    L.check(lib.srmi_linear_workspace_bytes(C.byref(d), L.PASS_FWD, C.byref(n)))
+    bufs = _guarded(y=M * N * e, z=M * N * e, ws=n.value)
+    L.check(lib.srmi_linear_fwd(C.byref(d), x.data_ptr(), w.data_ptr(), b.data_ptr(), r.data_ptr(), bufs["y"].ptr(), bufs["z"].ptr(), bufs["ws"].ptr(),
+                                n.value, stream))
+    kept = torch.float16 if dt == "bf16" else torch.float32
+    _check_guarded(bufs, {"y": DT[dt], "z": kept})
+    y = rows.linear(x, w, b, act=ACTS[act], residual=r)
+    assert torch.equal(bufs["y"].view(DT[dt]), y.flatten())
+    z = bufs["z"]
+    L.check(lib.srmi_linear_workspace_bytes(C.byref(d), L.PASS_BWD, C.byref(n)))
+    for wanted in ("dx dw db", "dx", "dw", "db", "dw db"):
+        bufs = _guarded(dx=M * K * e, dw=N * K * e, db=N * e, ws=n.value)
+        L.check(lib.srmi_linear_bwd(C.byref(d), x.data_ptr(), w.data_ptr(), z.ptr(), dy.data_ptr(),
+                                    *(bufs[k].ptr() if k in wanted.split() else None for k in ("dx", "dw", "db")), bufs["ws"].ptr(), n.value, stream))
+        _check_guarded(bufs, {k: DT[dt] for k in wanted.split()})
+        for k in ("dx", "dw", "db"):
+            assert k in wanted.split() or bool((bufs[k].view(torch.uint8) == 0xFF).all())
+
+
+@pytest.mark.parametrize("dt,pdt", [("bf16", "f32"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("n,c", [(1, 1), (3, 7), (37, 65), (1111, 257), (9, 1025), (600, 2049), (5, 8193), (700, 20001)])
+def test_norm_writes_its_outputs_and_nothing_else(n, c, dt, pdt):
+    import ctypes as C
+
+    from srmi import _lib as L
+    lib, size = L.load(), C.c_size_t(0)
+    x, w, b, dy = norm_case(n, c, dt, pdt, True, 0, 86)
+    x, w, b = x.detach(), w.detach(), b.detach()
+    code = {"bf16": L.BF16, "f32": L.F32}
+    e, pe = torch.finfo(DT[dt]).bits // 8, torch.finfo(DT[pdt]).bits // 8
+    d = L.NormDesc(n, c, code[dt], code[pdt], 1e-5, c, c)
+    stream = torch.cuda.current_stream().cuda_stream
+    kept = _guarded(y=n * c * e, mean=n * 4, rstd=n * 4)
+    L.check(lib.srmi_layer_norm_fwd(C.byref(d), x.data_ptr(), w.data_ptr(), b.data_ptr(), *(kept[k].ptr() for k in ("y", "mean", "rstd")), stream))
+    _check_guarded(kept, {"y": DT[dt], "mean": torch.float32, "rstd": torch.float32})
+    assert torch.equal(kept["y"].view(DT[dt]), rows.layer_norm(x, w, b).flatten())
+    L.check(lib.srmi_layer_norm_workspace_bytes(C.byref(d), C.byref(size)))
+    for wanted in ("dx dw db", "dx", "dw", "db"):
+        bufs = _guarded(dx=n * c * e, dw=c * pe, db=c * pe, ws=size.value)
+        L.check(lib.srmi_layer_norm_bwd(C.byref(d), x.data_ptr(), w.data_ptr(), kept["mean"].ptr(), kept["rstd"].ptr(), dy.data_ptr(),
+                                        *(bufs[k].ptr() if k in wanted.split() else None for k in ("dx", "dw", "db")), bufs["ws"].ptr(), size.value, stream))
+        _check_guarded(bufs, {k: DT[dt] if k == "dx" else DT[pdt] for k in wanted.split()})
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [1, 5, 2047, 100003])
+def test_dropout_writes_its_output_and_nothing_else(n, dt):
+    from srmi import _lib as L
+    lib, e = L.load(), 2 if dt == "bf16" else 4
+    x = torch.ones(n, device=DEV, dtype=DT[dt])
+    bufs = _guarded(y=n * e)
+    L.check(lib.srmi_dropout(x.data_ptr(), x.data_ptr(), bufs["y"].ptr(), n, L.BF16 if dt == "bf16" else L.F32, 0.5, 1, 2, None,
+                             torch.cuda.current_stream().cuda_stream))
+    _check_guarded(bufs, {"y": DT[dt]})
+    assert torch.equal(bufs["y"].view(DT[dt]), rows.dropout(x, 0.5, 1, 2, residual=x))
