@@ -511,8 +511,9 @@ typedef struct srmi_linear_desc {
 } srmi_linear_desc;
 
 /* y = act(x w^T + bias) + residual:  x [M, K], w [N, K] (nn.Linear's layout), bias [N] or NULL, residual [M, N] or NULL,
- * y [M, N].  z (NULL, or dense [M, N]) also receives x w^T + bias, which the backward of a smooth activation needs: f32 in f32
- * calls, IEEE half in bf16 calls (cut to +-65504).
+ * y [M, N].  z (NULL, or dense [M, N]) also receives x w^T + bias for the backward pass: f32 in f32 calls, IEEE half in bf16 calls,
+ * where values beyond +-65504 become infinities (every slope has its limit there) and RELU and LRELU promise the sign alone: a positive
+ * value below 2^-24, a half's least, is stored as that.
  * K == 0 is a product of nothing: y = act(bias) + residual.  N, K <= 2^22.
  * ws: srmi_linear_workspace_bytes(d, pass) bytes, 256-byte aligned, written and read by this call alone. */
 int srmi_linear_workspace_bytes(const srmi_linear_desc* d, int32_t pass, size_t* bytes);

@@ -103,18 +103,16 @@ template <typename T> struct KeptZ { typedef float type; };
 template <> struct KeptZ<bf16_t> { typedef _Float16 type; };
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-// ReLU and LeakyReLU need to know whether z > 0, of every z: below its least half, 2^-24, a positive z is kept as that.
-__device__ __forceinline__ _Float16 keep_half(float v) { return (_Float16)v; }
 template <int V>
 __device__ __forceinline__ void store_vec(_Float16* p, const float* v, bool past = false) {
     if constexpr (V == 1) {
-        p[0] = keep_half(v[0]);
+        p[0] = (_Float16)v[0];
     } else if constexpr (V == 4) {
-        put((u32x2_any*)p, __builtin_bit_cast(u32x2, f16x4{keep_half(v[0]), keep_half(v[1]), keep_half(v[2]), keep_half(v[3])}), past);
+        put((u32x2_any*)p, __builtin_bit_cast(u32x2, f16x4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]}), past);
     } else {
         f16x8 h;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = keep_half(v[j]);
+        for (int j = 0; j < 8; ++j) h[j] = (_Float16)v[j];
         const u32x4 q = __builtin_bit_cast(u32x4, h);
         put<1>((u32x4_any*)p, &q, past);
     }

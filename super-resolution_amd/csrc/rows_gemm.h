@@ -59,7 +59,7 @@ __device__ __forceinline__ void row_epilogue(const TileArgs& p, float* v, const 
         float k[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) k[j] = v[j];
-        if (sizeof(T) == 2 && is_kink(p.act)) {
+        if (sizeof(T) == 2 && is_kink(p.act)) {      // their slope asks whether z > 0, of every z: below the least half a positive one is kept as that
 #pragma unroll
             for (int j = 0; j < V; ++j) k[j] = v[j] > 0.f ? fmaxf(v[j], 0x1p-24f) : v[j];
         }
