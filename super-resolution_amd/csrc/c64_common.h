@@ -25,8 +25,8 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // Pixel pitches are multiples of 8 (or the key is taken from the column), so the key does not change with the row.
 __host__ __device__ constexpr int c64_key(int P) { return ((P >> 1) & 3) << 1; }
 
-// Slope activation on a channel pair:  z = a*sc + sh;  z >= 0 ? z : z*sl  with the multiply-adds as packed-f32
-// instructions (v_pk_fma_f32 / v_pk_mul_f32): three VALU instructions per value instead of four.
+// Slope activation on a channel pair:  z = a*sc + sh;  z >= 0 ? z : z*sl.  Four VALU instructions per value (FMA,
+// multiply, compare, select): packed-f32 instructions, which would halve the first two, are switched off in the build.
 __device__ __forceinline__ f32x2 slope_act2(f32x2 a, f32x2 sc, f32x2 sh, f32x2 sl) {
     const f32x2 z = __builtin_elementwise_fma(a, sc, sh);
     const f32x2 zs = z * sl;

@@ -18,7 +18,7 @@
 
 namespace srmi {
 
-typedef float thin_f2 __attribute__((ext_vector_type(2)));      // packed pairs: v_pk_fma_f32 retires two FMAs per lane and issue slot
+typedef float thin_f2 __attribute__((ext_vector_type(2)));      // pairs of channels (the build emits scalar FMAs for them)
 
 void f32t_magic(int d, unsigned* mul, int* sh);          // conv_f32_tiled.hip: multiply-shift constants of n / d
 
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256) void thinf_out_kernel(GenericParams p) {
 #pragma unroll
         for (int t = 0; t < T; ++t) vn[t] = *(const f32x4*)(x + tpn.off[t] + 4 * cg);
         float acc[P];
-        thin_f2 a01 = {0.f, 0.f}, a23 = {0.f, 0.f};          // produced channels in packed pairs (v_pk_fma_f32)
+        thin_f2 a01 = {0.f, 0.f}, a23 = {0.f, 0.f};          // produced channels in pairs
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             const bool ok = (tp.ok >> t) & 1u;
