@@ -7,7 +7,6 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
@@ -103,12 +102,12 @@ void check_restored(const Tensor& t, const char* what, at::ScalarType dtype, at:
                 " as ", t.scalar_type(), " ", t.sizes(), " on ", t.device(), ", saved was ", dtype, " ", shape, " on ", device);
 }
 
-// A backward pass that is captured must not meet a leaf whose accumulation node an eager graph, still alive, made on another stream:
-// autograd would make the capturing stream wait for that one, which ends the capture and with it the process.  Looked for in
-// the operands and in everything they were computed from.
+// A backward pass that is captured must not meet a node that was made on the default stream: an operation before the capture, or a leaf's
+// accumulation node that an eager graph, still alive, refers to.  Autograd would make that stream wait for the capturing one, which
+// the default stream cannot, and the process ends.  (Another stream, such as the one of warm-up runs whose last graph is still
+// referred to, joins the capture and is fine.)  Looked for in the operands and in everything they were computed from.
 void check_capture(std::initializer_list<const Tensor*> operands) {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    const auto here = c10::hip::getCurrentHIPStream();
     std::vector<std::shared_ptr<torch::autograd::Node>> todo;
     std::unordered_set<torch::autograd::Node*> seen;
     auto push = [&](std::shared_ptr<torch::autograd::Node> node) {
@@ -119,11 +118,9 @@ void check_capture(std::initializer_list<const Tensor*> operands) {
     while (!todo.empty()) {
         const auto node = todo.back();
         todo.pop_back();
-        if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) {
-            const auto stream = node->stream();
-            TORCH_CHECK(!stream || stream->id() == here.id(),
-                        "srmi.rows: graph capture over a leaf that an eager autograd graph of another stream still refers to; delete that graph first");
-        }
+        const auto stream = node->stream();
+        TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(stream->device_index()).id(),
+                    "srmi.rows: graph capture over a leaf that an eager autograd graph of the default stream still refers to; delete that graph first");
         for (const auto& edge : node->next_edges()) push(edge.function);
     }
 }

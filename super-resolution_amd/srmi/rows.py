@@ -12,8 +12,8 @@ Storage is float32 or bfloat16 (one type per call); sums, statistics and activat
 channel slice of a wider buffer is read in place); anything whose last axis is not dense is copied first.  Outputs are dense.
 Results do not depend on timing: no atomics, the same call gives the same bits.  Calls may be captured into a HIP graph; nothing is
 kept between calls (workspaces come from torch's allocator, call by call), so graphs and streams share nothing.  Capturing a
-differentiable call whose leaves an eager autograd graph of another stream still refers to is refused (autograd would end the process in
-the captured backward pass): delete that graph first.  Gradients are first derivatives in reverse mode; a tensor with a tangent of
+differentiable call whose leaves an eager autograd graph of the default stream still refers to is refused (autograd would end the process
+in the captured backward pass): delete that graph first, or run warm-ups on a side stream.  Gradients are first derivatives in reverse mode; a tensor with a tangent of
 forward-mode AD raises.  So does a call that is being traced or exported, and a tensor subclass with its own dispatch (DTensor, FakeTensor).
 
 Reference call sites these stand next to: ``nn.Linear`` + LeakyReLU (P/srgan_model.py:57-60), ``nn.BatchNorm2d`` (P/ops.py:24-26).

@@ -1372,3 +1372,76 @@ def test_dropout_writes_its_output_and_nothing_else(n, dt):
                              torch.cuda.current_stream().cuda_stream))
     _check_guarded(bufs, {"y": DT[dt]})
     assert torch.equal(bufs["y"].view(DT[dt]), rows.dropout(x, 0.5, 1, 2, residual=x))
+
+
+# ---- capture after warm-up runs on a side stream ------------------------------------------------------------------------------
+def _block(dt):
+    torch.manual_seed(90)
+    return nn.Sequential(rows.LayerNorm(64), rows.Linear(64, 160, act=nn.GELU()), rows.Linear(160, 64)).to(DEV).to(DT[dt])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_graphed_callables(dt):
+    # the warm-up's last graph is still referred to while the capture runs: its leaves' nodes belong to the warm-up stream
+    a, b = _block(dt), _block(dt)
+    graphed = torch.cuda.make_graphed_callables(a, (torch.randn(300, 64, device=DEV, dtype=DT[dt], requires_grad=True),))
+    for _ in range(4):
+        x = torch.randn(300, 64, device=DEV, dtype=DT[dt])
+        dy = torch.randn(300, 64, device=DEV, dtype=DT[dt])
+        got, want = [], []
+        for f, net, out in ((graphed, a, got), (b, b, want)):
+            net.zero_grad(set_to_none=True)
+            leaf = x.clone().requires_grad_()
+            y = f(leaf)
+            y.backward(dy)
+            out += [y.detach().clone(), leaf.grad] + [p.grad.clone() for p in net.parameters()]
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_captured_training_step_after_warm_up(dt):
+    a, b = _block(dt), _block(dt)
+    x, dy = (torch.randn(300, 64, device=DEV, dtype=DT[dt]) for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            a.zero_grad(set_to_none=True)
+            alive = a(x)
+            alive.backward(dy)
+    torch.cuda.current_stream().wait_stream(side)
+    a.zero_grad(set_to_none=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = a(x)
+        y.backward(dy)
+    assert alive.grad_fn is not None
+    for _ in range(4):
+        x.copy_(torch.randn(300, 64, device=DEV))
+        graph.replay()
+        b.zero_grad(set_to_none=True)
+        want = b(x)
+        want.backward(dy)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and all(torch.equal(p.grad, q.grad) for p, q in zip(a.parameters(), b.parameters()))
+
+
+def test_capture_refuses_operands_computed_on_the_default_stream():
+    # the leaf's node belongs to a side stream, the operation between it and the captured call to the default one
+    x = torch.randn(80, 64, device=DEV, requires_grad=True)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        alive = rows.layer_norm(x)
+    torch.cuda.synchronize()
+    h = x * 2.0
+    for f in (lambda t: rows.linear(t, t), lambda t: rows.layer_norm(t), lambda t: rows.dropout(t, 0.5, 1)):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager autograd graph"):
+            with torch.cuda.graph(graph):
+                f(h)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):                                        # the leaf itself is fine
+            f(x)
+    assert alive.grad_fn is not None
