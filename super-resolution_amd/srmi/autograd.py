@@ -308,6 +308,8 @@ class FusedConvFn(torch.autograd.Function):
         lib = L.load()
         st = Fn.stream_ptr()
         x, w, z, mean, rstd, gamma, beta, alpha = ctx.saved_tensors
+        x, z = nhwc(x), nhwc(z)                    # saved-tensor hooks keep values, not memory formats
+        w, mean, rstd, gamma, beta, alpha = (t.contiguous() if t is not None else None for t in (w, mean, rstd, gamma, beta, alpha))
         cfg, desc, ed, plan = ctx.cfg, ctx.desc, ctx.ed, ctx.plan
         dev = x.device
         dy = nhwc(dy)
@@ -391,7 +393,7 @@ class MaxPool2x2Fn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         (x,) = ctx.saved_tensors
-        dy = nhwc(dy)
+        x, dy = nhwc(x), nhwc(dy)
         N, Cc, H, W = x.shape
         dx = torch.empty_like(x)
         L.check(L.load().srmi_maxpool2x2_bwd(x.data_ptr(), dy.data_ptr(), dx.data_ptr(), N, H, W, Cc, Fn.stream_ptr()))

@@ -58,7 +58,7 @@ class _MSEFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        a, b = ctx.saved_tensors
+        a, b = _same_storage_order(*ctx.saved_tensors)      # saved-tensor hooks keep values, not memory formats
         g = g.contiguous()
         da = torch.empty_like(a) if ctx.needs_input_grad[0] else None
         db = torch.empty_like(b) if ctx.needs_input_grad[1] else None
@@ -81,7 +81,7 @@ class _BCEFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        p, t = ctx.saved_tensors
+        p, t = (v.contiguous() for v in ctx.saved_tensors)
         dp = torch.empty_like(p)
         L.check(L.load().srmi_bce_loss_bwd(p.data_ptr(), t.data_ptr(), g.contiguous().data_ptr(), p.numel(),
                                            dp.data_ptr(), stream_ptr()))
@@ -126,7 +126,7 @@ class _TVFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        (x,) = ctx.saved_tensors
+        x = ctx.saved_tensors[0].contiguous()
         N, C_, H, W = x.shape
         dx = torch.empty_like(x)
         L.check(L.load().srmi_tv_loss_bwd(x.data_ptr(), g.contiguous().data_ptr(), N, C_, H, W, ctx.weight,
