@@ -16,7 +16,8 @@
 // Operands this kernel cannot take - f32, or bf16 rows off 16-byte boundaries - go through gemm_staged_kernel: the same tiles and fragments,
 // loaded through registers at any alignment.  f32 values are split there into three bf16 (x = hi + mid + lo to 24 bits) and
 // multiplied as six products hi hi, hi mid, mid hi, hi lo, mid mid, lo hi: the matrix cores run bf16 sixteen times as fast as f32, the
-// dropped products are below 2^-22 of the largest and of either sign.  hi hi has an accumulator of its own, so that a sum over K is
+// dropped products are below 2^-22 of the largest and of either sign.  bf16 has nothing below 2^-133: operands under 2^-110 are taken to the
+// nearest multiple of that, instead of to 24 bits.  hi hi has an accumulator of its own, so that a sum over K is
 // rounded once per 32 k as an f32 sum would be, not six times.
 #pragma once
 #include "rows_common.h"

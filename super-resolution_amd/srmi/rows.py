@@ -13,8 +13,10 @@ channel slice of a wider buffer is read in place); anything whose last axis is n
 Results do not depend on timing: no atomics, the same call gives the same bits.  Calls may be captured into a HIP graph; nothing is
 kept between calls (workspaces come from torch's allocator, call by call), so graphs and streams share nothing.  Capturing a
 differentiable call whose leaves an eager autograd graph of the default stream still refers to is refused (autograd would end the process
-in the captured backward pass): delete that graph first, or run warm-ups on a side stream.  Gradients are first derivatives in reverse mode; a tensor with a tangent of
-forward-mode AD raises.  So does a call that is being traced or exported, and a tensor subclass with its own dispatch (DTensor, FakeTensor).
+in the captured backward pass): delete that graph first, or run warm-ups on a side stream.
+
+Gradients are first derivatives in reverse mode; a tensor with a tangent of forward-mode AD raises.  So does a call that is being traced
+or exported, and a tensor subclass with its own dispatch (DTensor, FakeTensor).
 
 Reference call sites these stand next to: ``nn.Linear`` + LeakyReLU (P/srgan_model.py:57-60), ``nn.BatchNorm2d`` (P/ops.py:24-26).
 The checks, tensors and autograd nodes are in csrc/rows_torch.cpp.  No fallback: CPU tensors raise; no ATen arithmetic.
@@ -55,7 +57,7 @@ def _strided_rows(t):
 def linear(x, weight, bias=None, act=None, residual=None):
     """``act(x @ weight.T + bias) + residual`` in one pass.  x [..., K], weight [N, K], bias [N], residual [..., N]; ``act``: None, or
     an nn.ReLU / LeakyReLU / Tanh / Sigmoid / GELU (either form) / SiLU module.  All tensors share x's dtype (float32: the products
-    have float32's accuracy; bfloat16: bf16 operands, f32 sums).
+    have float32's accuracy, operands below 2^-110 being taken to the nearest 2^-133; bfloat16: bf16 operands, f32 sums).
 
     Training in bfloat16 rounds ``dy * act'(z)`` to bfloat16 once, as the products' operand (the bias gradient sums it before that
     rounding); the pre-activation is kept as an IEEE half.  A float32 infinity in x or weight may come out as NaN."""

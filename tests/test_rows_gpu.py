@@ -1445,3 +1445,19 @@ def test_capture_refuses_operands_computed_on_the_default_stream():
         with torch.cuda.graph(graph):                                        # the leaf itself is fine
             f(x)
     assert alive.grad_fn is not None
+
+
+@pytest.mark.parametrize("M", [8, 200])                                      # the f32 matrix instruction, and three bf16 planes
+@pytest.mark.parametrize("e", [-148, -140, -133, -126, -120, -115, -110, -100, -60, 60, 100, 120])
+def test_linear_f32_range(e, M):
+    # x = hi + mid + lo has 24 bits unless the low plane ends at bf16's least step, 2^-133: off by half of that at most
+    gen = torch.Generator().manual_seed(91)
+    K, N = 40, 64
+    x = (1 + torch.rand(M, K, generator=gen, dtype=torch.float64)) * (torch.randint(0, 2, (M, K), generator=gen) * 2 - 1)
+    x = (x * 2.0 ** e).float()
+    w = torch.randn(N, K, generator=gen)
+    x64, w64 = x.double(), w.double()
+    want = x64 @ w64.t()
+    mag = x64.abs() @ w64.abs().t()
+    bound = (K + 8) * U * mag + 2.0 ** -134 * (w64.abs().sum(1) + K)[None] + 2.0 ** -148
+    assert_within(rows.linear(x.to(DEV), w.to(DEV)), want, bound, "y")
